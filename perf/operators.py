@@ -1,0 +1,240 @@
+"""The loss at the end of a language model, head included: what a training or scoring step does with the last hidden
+states. Two operators, each forward and backward:
+
+  xent     cross entropy of the labels under softmax(x . w), the logits [rows, vocabulary] never kept
+  distill  Kullback-Leibler divergence from a teacher's top logits to the student's softmax(x . w / temperature)
+
+Each gives a loss and a log-sum-exp a row; a training step gives the gradients of x and w too. A row without a target
+(a label below zero; no teacher entry with an id of zero or more and a logit above minus infinity) has loss 0,
+log-sum-exp 0 and gradient 0, whatever its x holds.
+"""
+import torch
+
+own = False  # False: the plain forms below; True: the executor's launches
+
+_DTYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+
+
+def listed():
+    return [
+        # the scores of one decode step's tokens (16 sequences, the 7B head): the smallest call, bound by the head's bytes
+        _case("score a decode step", op="xent", step=False, dtype="bf16", batch=16, seq=1, model=4096, vocab=32000),
+        # perplexity of one window of 2048 positions under the 7B head
+        _case("score a window", op="xent", step=False, dtype="bf16", batch=1, seq=2048, model=4096, vocab=32000),
+        # a small model's whole head, f32 throughout, as the small test models are
+        _case("train small f32", op="xent", step=True, dtype="f32", batch=8, seq=32, model=128, vocab=1000, ignored=0.1),
+        # f32 training of a wider model: next-token labels, so the last position of every sequence is left out
+        _case("train f32", op="xent", step=True, dtype="f32", batch=4, seq=511, model=1024, vocab=16384, shift=True),
+        # the training benchmark's rows (4 sequences of 2048) under the 7B head: the largest call
+        _case("train 7B head", op="xent", step=True, dtype="bf16", batch=4, seq=2048, model=4096, vocab=32000),
+        # a vocabulary of 2^17, the head stored as the embedding is ([vocabulary, model]), a third of the batch padding
+        _case("train large vocabulary", op="xent", step=True, dtype="bf16", batch=2, seq=2048, model=2048, vocab=131072, tied=True, ignored=0.33),
+        # sizes that fit nothing: odd rows, an odd vocabulary whose rows start at any 2-byte address
+        _case("train odd sizes", op="xent", step=True, dtype="f16", batch=3, seq=509, model=1000, vocab=30011, shift=True, ignored=0.05),
+        # distillation's loss on one token: latency
+        _case("distill one token", op="distill", step=False, dtype="bf16", batch=1, seq=1, model=4096, vocab=32000, top=8, temperature=1.0),
+        # distillation's loss over an evaluation batch
+        _case("distill score", op="distill", step=False, dtype="bf16", batch=1, seq=1024, model=4096, vocab=32000, top=64, temperature=2.0),
+        # a distillation step of a few answer tokens, a tied head with an odd vocabulary
+        _case("distill few rows", op="distill", step=True, dtype="bf16", batch=3, seq=17, model=2048, vocab=50021, tied=True, top=20, temperature=1.0, ignored=0.1),
+        # a distillation step under the 7B head
+        _case("distill train", op="distill", step=True, dtype="bf16", batch=2, seq=2048, model=4096, vocab=32000, top=64, temperature=2.0, ignored=0.02),
+        # odd sizes, f16, teachers of other lengths a row
+        _case("distill odd sizes", op="distill", step=True, dtype="f16", batch=7, seq=111, model=776, vocab=32001, top=33, temperature=1.5, shift=True, ignored=0.2),
+    ]
+
+
+def _case(name, **c):
+    return {"name": name, "tied": False, "shift": False, "ignored": 0.0, "top": 0, "temperature": 1.0, **c}
+
+
+def draw(rng):
+    def log(lo, hi):
+        return int(round(lo * (hi / lo) ** rng.random()))
+
+    while True:
+        c = _case("", op=rng.choice(["xent", "distill"]), step=rng.random() < 0.7, dtype=rng.choice(["bf16", "bf16", "f16", "f32"]),
+                  batch=log(1, 16), seq=log(1, 4096), model=log(64, 4096), vocab=log(64, 131072), tied=rng.random() < 0.4, shift=rng.random() < 0.3,
+                  ignored=rng.choice([0.0, 0.02, 0.3]))
+        del c["name"]
+        if rng.random() < 0.6:  # most models' widths are multiples of 64; the others stay as drawn, odd ones among them
+            c["model"] = max(64, c["model"] // 64 * 64)
+        if rng.random() < 0.5:
+            c["vocab"] = max(64, c["vocab"] // 64 * 64)
+        if c["op"] == "distill":
+            c["top"] = min(log(1, 128), c["vocab"])
+            c["temperature"] = rng.choice([1.0, 2.0, round(rng.uniform(0.5, 4.0), 2)])
+        work = c["batch"] * c["seq"] * c["model"] * c["vocab"] * (3 if c["step"] else 1) * (2 if c["dtype"] == "f32" else 1)
+        if work <= 4 * 2048 * 4096 * 32000 * 3 and c["batch"] * c["seq"] <= 16384 and c["batch"] * c["seq"] * c["vocab"] <= 4096 * 131072:
+            return c
+
+
+def prepare(case, seed):
+    """What a training or scoring loop holds before the call: the last norm's output, the head, the targets, each row's
+    weight in the batch's loss, and buffers for the results."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    dt, b, t, d, v = _DTYPES[case["dtype"]], case["batch"], case["seq"], case["model"], case["vocab"]
+    n, top = b * t, case["top"]
+
+    def normal(*shape):
+        return torch.randn(*shape, generator=g, device="cuda")
+
+    def whole(lo, hi, *shape):
+        return torch.randint(lo, hi, shape, generator=g, device="cuda")
+
+    s = {"case": dict(case)}
+    w = (normal(v, d) if case["tied"] else normal(d, v)) * (2.0 / d**0.5)  # logits of a spread of about 2
+    s["w"] = w.to(dt)
+    labels = whole(0, v, b, t)
+    # normed hidden states that lean towards their label's row of the head, as a trained model's do
+    full = normal(b, t + 1 if case["shift"] else t, d)
+    head_rows = (w if case["tied"] else w.t())[labels.reshape(-1)].reshape(b, t, d)
+    full[:, :t] += 1.5 * head_rows
+    s["x"] = full.to(dt)[:, :t]  # with `shift`, every sequence's last position has no label: rows lie t + 1 apart
+    gone = torch.rand(b, t, generator=g, device="cuda") < case["ignored"]
+    if case["op"] == "xent":
+        s["labels"] = torch.where(gone, torch.full_like(labels, -1), labels)
+        here = ~gone
+    else:
+        # the teacher's ids: its own best among them, distinct in a row; rows end early where the teacher kept fewer
+        step = whole(1, max(2, v // top + 1), b, t, top)
+        ids = (labels[..., None] + (step.cumsum(-1) - step[..., :1])) % v
+        s["teacher"] = (2.5 * normal(b, t, top)).sort(dim=-1, descending=True).values.to(torch.bfloat16 if case["dtype"] == "bf16" else torch.float32)
+        kept = torch.where(whole(0, 4, b, t, 1) == 0, whole(1, top + 1, b, t, 1), torch.full((b, t, 1), top, device="cuda"))
+        off = (torch.arange(top, device="cuda") >= kept) | gone[..., None]
+        s["ids"] = torch.where(off, torch.full_like(ids, -1), ids).contiguous()
+        here = ~gone
+    # the mean over the rows that have a target: each row's share of the loss, its cotangent in the backward pass
+    s["ct"] = torch.full((b, t), 1.0, device="cuda") / here.sum().clamp(min=1)
+    s["loss"], s["lse"] = (torch.empty(b, t, device="cuda") for _ in range(2))
+    if case["step"]:
+        s["dx"], s["dw"] = torch.empty(b, t, d, dtype=dt, device="cuda"), torch.empty_like(s["w"])
+    return s
+
+
+def run(state):
+    return _own(state) if own else _plain(state)
+
+
+def _plain(s):
+    c = s["case"]
+    tau = c["temperature"]
+    x, w = s["x"].float().reshape(-1, c["model"]), s["w"].float()
+    if c["tied"]:
+        w = w.t()
+    rows = torch.arange(x.shape[0], device=x.device)
+    if c["op"] == "xent":
+        ids = s["labels"].reshape(-1, 1)
+        off = ids < 0
+        p, plogp = (~off).float(), torch.zeros_like(rows, dtype=torch.float32)
+    else:
+        ids = s["ids"].reshape(-1, c["top"])
+        t = s["teacher"].float().reshape(-1, c["top"]) / tau
+        off = (ids < 0) | (t == -float("inf"))
+        best = torch.where(off, -float("inf"), t).amax(1, keepdim=True)
+        e = torch.where(off, 0.0, torch.exp(t - torch.where(off.all(1, keepdim=True), 0.0, best)))
+        z = e.sum(1, keepdim=True)
+        p = torch.where(off, 0.0, e / z)
+        plogp = torch.where(off, 0.0, p * (t - best - torch.log(z))).sum(1)
+    gone = off.all(1)
+    x = torch.where(gone[:, None], 0.0, x)
+    logits = (x @ w) / tau
+    m = logits.amax(1, keepdim=True)
+    lse = m[:, 0] + torch.log(torch.exp(logits - m).sum(1))
+    at = torch.where(off, 0, ids)
+    hit = logits[rows[:, None], at]
+    loss = plogp + torch.where(off, 0.0, p * (lse[:, None] - hit)).sum(1)
+    out = {"loss": torch.where(gone, 0.0, loss).reshape(s["loss"].shape), "lse": torch.where(gone, 0.0, lse).reshape(s["lse"].shape)}
+    if c["step"]:
+        g = torch.exp(logits - lse[:, None])
+        g.view(-1).index_add_(0, (rows[:, None] * g.shape[1] + at).reshape(-1), -torch.where(off, 0.0, p).reshape(-1))
+        g *= torch.where(gone, 0.0, s["ct"].reshape(-1) / tau)[:, None]
+        out["dx"] = (g @ w.t()).to(s["dx"].dtype).reshape(s["dx"].shape)
+        out["dw"] = (g.t() @ x if c["tied"] else x.t() @ g).to(s["dw"].dtype)
+    return out
+
+
+_executor = None
+
+
+def _own(s):
+    global _executor
+    import presk_b200
+
+    c = s["case"]
+    if _executor is None:
+        _executor = presk_b200.Executor(s["x"].device.index or 0)
+    if "plan" not in s:  # the launches' descriptions, which depend on sizes and strides alone: kept beside the buffers
+        abi = presk_b200.abi
+        codes = {torch.bfloat16: abi.BF16, torch.float16: abi.F16, torch.float32: abi.F32}
+        what = dict(outer=(c["batch"], c["seq"]), vocab=c["vocab"], model=c["model"], dtype=codes[s["x"].dtype], x_strides=s["x"].stride(),
+                    vocab_major=c["tied"], temperature=c["temperature"])
+        given = [s["x"], s["w"]]
+        if c["op"] == "xent":
+            given += [s["labels"]]
+        else:
+            what.update(top=c["top"], teacher_dtype=codes[s["teacher"].dtype])
+            given += [s["ids"], s["teacher"]]
+        s["plan"] = [(presk_b200.head_loss_launch(**what), [a.data_ptr() for a in given + [s["lse"], s["loss"]]])]
+        if c["step"]:
+            s["plan"] += [(presk_b200.head_loss_vjp_launch(**what), [a.data_ptr() for a in given + [s["ct"], s["lse"], s["dw"], s["dx"]]])]
+    for launch, table in s["plan"]:
+        _executor.run(launch, table)
+    return {k: s[k] for k in ("loss", "lse", "dx", "dw") if k in s}
+
+
+def work(case):
+    """Each input once, each output once; the head's product forward, and two products of its size backward."""
+    n, d, v = case["batch"] * case["seq"], case["model"], case["vocab"]
+    e = 4 if case["dtype"] == "f32" else 2
+    targets = 8 if case["op"] == "xent" else case["top"] * (8 + (2 if case["dtype"] == "bf16" else 4))
+    moved = e * (n * d + d * v) + n * (targets + 8)
+    flops = 2.0 * n * d * v
+    if case["step"]:
+        moved += e * (n * d + d * v) + 4 * n
+        flops *= 3
+    return {"bytes": moved, "flops": flops}
+
+
+def exact(case, seed):
+    """In 64 bits, a block of rows at a time, from the definitions."""
+    s = prepare(case, seed)
+    n, d, v, tau, step = case["batch"] * case["seq"], case["model"], case["vocab"], float(case["temperature"]), case["step"]
+    x = s["x"].double().reshape(n, d)
+    w = s["w"].double()  # [vocabulary, model] from here on
+    w = w if case["tied"] else w.t()
+    loss, lse = (torch.zeros(n, dtype=torch.float64, device="cuda") for _ in range(2))
+    dx, dw = torch.zeros(n, d, dtype=torch.float64, device="cuda"), torch.zeros(v, d, dtype=torch.float64, device="cuda")
+    block = max(1, (1 << 27) // v)
+    for lo in range(0, n, block):
+        hi = min(n, lo + block)
+        xb = x[lo:hi]
+        target = torch.zeros(hi - lo, v, dtype=torch.float64, device="cuda")  # the distribution a row is held to
+        if case["op"] == "xent":
+            y = s["labels"].reshape(n)[lo:hi]
+            target.scatter_add_(1, y.clamp(min=0)[:, None], (y >= 0).double()[:, None])
+            entropy = torch.zeros(hi - lo, dtype=torch.float64, device="cuda")
+        else:
+            ids, t = s["ids"].reshape(n, -1)[lo:hi], s["teacher"].double().reshape(n, -1)[lo:hi]
+            logp = torch.log_softmax(torch.where(ids < 0, -float("inf"), t / tau), 1)
+            p = torch.where(ids < 0, 0.0, torch.exp(logp))
+            p = torch.where(torch.isnan(p), 0.0, p)
+            entropy = -torch.where(p > 0, p * logp, 0.0).sum(1)
+            target.scatter_add_(1, ids.clamp(min=0), p)
+        has = target.sum(1) > 0.5
+        xb = torch.where(has[:, None], xb, 0.0)
+        z = xb @ w.t() / tau
+        ls = torch.logsumexp(z, 1)
+        z -= ls[:, None]
+        loss[lo:hi] = torch.where(has, -(target * z).sum(1) - entropy, 0.0)
+        lse[lo:hi] = torch.where(has, ls, 0.0)
+        if step:
+            g = z.exp_().sub_(target).mul_((torch.where(has, s["ct"].reshape(n)[lo:hi].double(), 0.0) / tau)[:, None])
+            dx[lo:hi] = g @ w
+            dw += g.t() @ xb
+    shape = (case["batch"], case["seq"])
+    out = {"loss": loss.reshape(shape), "lse": lse.reshape(shape)}
+    if step:
+        out["dx"] = dx.reshape(*shape, d)
+        out["dw"] = dw if case["tied"] else dw.t().contiguous()
+    return out
