@@ -126,11 +126,36 @@ typedef enum {
                              the classes). Inputs: logits, labels, the cotangent over the outer axes. Output over the
                              whole space: (exp(x - m) / z - [k == y]) * ct, m and z as in PSK_OP_XENT (the maximum from
                              the row's first element, z summed in index order), each operation rounded. */
-    PSK_OP_EMBED_VJP = 16 /* lower.rs:1444-1457: embed_vjp. Space as PSK_OP_EMBED: (the indices' axes..., d). Inputs: the
+    PSK_OP_EMBED_VJP = 16, /* lower.rs:1444-1457: embed_vjp. Space as PSK_OP_EMBED: (the indices' axes..., d). Inputs: the
                              table (its shape only: never read), the indices, the cotangent over the space. Output: a
                              table of iparam[0] rows (strides in out.stride[0], out.stride[1]), zero-filled, then
                              row idx[iv] += ct[iv, :] for every iv in index order, each sum kept in the output's
                              storage type (rounded there after every addition). */
+    PSK_OP_HEAD_XENT = 17, /* the head's contraction and cross_entropy (examples/coverage/llama.psk:133, 140-142) as one
+                             launch that takes the vocabulary in pieces and never stores the logits. Space: the rows'
+                             axes, then two inner ones, (classes, model). Inputs: x (rows, model; stride 0 on classes), w
+                             (classes, model; either may be the contiguous one), labels (i64, over the rows) and, as a
+                             fourth, the place of a second result over the rows, each row's log-sum-exp (f32). Output:
+                             the loss over the rows, ln sum_v exp(l_v) - l_label with l = x.w in binary32 (the logits'
+                             site is not rounded to its type: the declared departure of this launch, as `online`
+                             attention's). A label below zero is a row without a target: loss, log-sum-exp and gradient 0,
+                             whatever x holds there; one that the vocabulary does not have is reported at the next
+                             psk_exec_sync (E7001) and counts as none. x and w are both bf16, f16 or f32. PSK_ORDER_DEVICE
+                             only; an executor may decline the launch (E7005), and the caller then issues the two. */
+    PSK_OP_HEAD_XENT_VJP = 18, /* its gradients. Space as PSK_OP_HEAD_XENT. Inputs: x, w, labels, ct (over the rows, any
+                             stride), the log-sum-exp of the forward launch and, as a sixth, the place of a second result,
+                             dw over (classes, model). Output: dx over (rows, model). With g = (exp(l - lse) -
+                             [v = label])·ct, dx = g·wᵀ and dw = xᵀ·g, both stored in the operands' type; 16-bit
+                             operands have g rounded to their type before the two products. */
+    PSK_OP_HEAD_DISTILL = 19, /* Kullback-Leibler divergence from a teacher's top logits to the student's distribution:
+                             inner axes (classes, model, top), fparam[0] the temperature τ. Inputs: x, w, the teacher's
+                             classes (i64) and logits (bf16, f16 or f32) over (rows, top), and, as a fifth, the place of
+                             the log-sum-exp. With p = softmax(t / τ) over a row's entries and lse = ln sum_v exp(l_v / τ):
+                             loss = sum_j p_j (ln p_j - l_j / τ + lse). Entries with a class below zero or a logit of
+                             minus infinity are left out; a row without any has loss 0. A class may appear twice (its
+                             probabilities add). At most 1024 entries a row. No counterpart in the reference. */
+    PSK_OP_HEAD_DISTILL_VJP = 20 /* inputs: x, w, classes, teacher, ct, lse and, as a seventh, the place of dw; as
+                             PSK_OP_HEAD_XENT_VJP with g = (exp(l / τ - lse) - sum_{j: class_j = v} p_j)·ct / τ. */
 } psk_op;
 
 /* Elementary operations of a fusion group's steps (lower.rs:184-226). */

@@ -554,6 +554,114 @@ static int attention_unfused(const psk_launch *l, void *const *table, uint32_t *
     return rc;
 }
 
+/* The head's losses, forward and backward, from their formulas (include/presk_cuda.h, PSK_OP_HEAD_*): every sum and
+ * function in binary64 over the stored operands, one rounding at the store. They are declared-order launches, so what
+ * an executor returns agrees with this within a tolerance. */
+static int head_loss(const psk_launch *l, void *const *table, uint32_t *overflow)
+{
+    const int vjp = l->op == PSK_OP_HEAD_XENT_VJP || l->op == PSK_OP_HEAD_DISTILL_VJP;
+    const int distill = l->op == PSK_OP_HEAD_DISTILL || l->op == PSK_OP_HEAD_DISTILL_VJP;
+    if (l->order != PSK_ORDER_DEVICE) return PSK_E7005;
+    const int no = l->n_outer, first = distill ? 4 : 3, lse_at = vjp ? first + 1 : first, dw_at = first + 2;
+    if (l->n_inner != (distill ? 3 : 2)) return PSK_E7001;
+    const psk_operand *X = &l->in[0], *W = &l->in[1];
+    if (X->dtype != W->dtype || (X->dtype != PSK_F32 && X->dtype != PSK_BF16 && X->dtype != PSK_F16)) return PSK_E7005;
+    const int64_t V = l->dims[no], D = l->dims[no + 1], K = distill ? l->dims[no + 2] : 1;
+    const double tau = distill ? l->fparam[0] : 1.0;
+    const uint8_t *base[PSK_MAX_INPUTS + 1];
+    for (int i = 0; i <= l->n_inputs; ++i) {
+        const psk_operand *o = i < l->n_inputs ? &l->in[i] : &l->out;
+        base[i] = (const uint8_t *)table[i] + o->offset * (int64_t)elem_bytes(o->dtype);
+    }
+    int64_t rows = 1;
+    for (int a = 0; a < no; ++a) rows *= l->dims[a];
+    double *dw = NULL;
+    const int has_dw = vjp && l->n_inputs > dw_at;
+    if (has_dw) dw = (double *)calloc((size_t)(V * D), sizeof(double));
+    double *z = (double *)malloc((size_t)V * sizeof(double)), *q = (double *)malloc((size_t)V * sizeof(double)), *x = (double *)malloc((size_t)D * sizeof(double)), *dx = (double *)malloc((size_t)D * sizeof(double));
+    uint32_t ovf = 0;
+    int bad = 0;
+    for (int64_t row = 0; row < rows; ++row) {
+        memset(q, 0, (size_t)V * sizeof(double));
+        int n = 0;
+        double entropy = 0.0;
+        const int64_t ibase = offset_of(l->in[2].stride, l->dims, 0, no, row);
+        const int64_t *ids = (const int64_t *)base[2] + ibase;
+        const int64_t ik = distill ? l->in[2].stride[no + 2] : 0;
+        if (!distill) {
+            if (ids[0] >= V) bad = 1;
+            else if (ids[0] >= 0) { q[ids[0]] = 1.0; n = 1; }
+        } else {
+            const int64_t tbase = offset_of(l->in[3].stride, l->dims, 0, no, row), tk = l->in[3].stride[no + 2];
+            double m = -INFINITY, sum = 0.0;
+            for (int pass = 0; pass < 3; ++pass)
+                for (int64_t j = 0; j < K; ++j) {
+                    const int64_t id = ids[j * ik];
+                    const double t = (double)load_real(base[3], l->in[3].dtype, tbase + j * tk) / tau;
+                    if (id >= V) bad = 1;
+                    if (id < 0 || id >= V || t == -INFINITY) continue;
+                    if (pass == 0) { ++n; if (t > m) m = t; }
+                    else if (pass == 1) sum += exp(t - m);
+                    else {
+                        const double p = exp(t - m) / sum;
+                        q[id] += p;
+                        if (p != 0.0) entropy -= p * (t - m - log(sum));
+                    }
+                }
+        }
+        const int64_t xbase = offset_of(X->stride, l->dims, 0, no, row), obase = offset_of(l->out.stride, l->dims, 0, no, row);
+        const int64_t lbase = l->n_inputs > lse_at ? offset_of(l->in[lse_at].stride, l->dims, 0, no, row) : 0;
+        if (n == 0) {
+            if (vjp) for (int64_t d = 0; d < D; ++d) store_out(l, (uint8_t *)base[l->n_inputs], obase + d * l->out.stride[no + 1], 0.0f);
+            else {
+                store_out(l, (uint8_t *)base[l->n_inputs], obase, 0.0f);
+                if (l->n_inputs > lse_at) ((float *)base[lse_at])[lbase] = 0.0f;
+            }
+            continue;
+        }
+        for (int64_t d = 0; d < D; ++d) x[d] = load_real(base[0], X->dtype, xbase + d * X->stride[no + 1]);
+#pragma omp parallel for schedule(static)
+        for (int64_t v = 0; v < V; ++v) {
+            double acc = 0.0;
+            for (int64_t d = 0; d < D; ++d) acc += x[d] * (double)load_real(base[1], W->dtype, v * W->stride[no] + d * W->stride[no + 1]);
+            z[v] = acc / tau;
+        }
+        if (!vjp) {
+            double m = -INFINITY, sum = 0.0, loss = -entropy;
+            for (int64_t v = 0; v < V; ++v) if (z[v] > m) m = z[v];
+            for (int64_t v = 0; v < V; ++v) sum += exp(z[v] - m);
+            const double lse = m + log(sum);
+            for (int64_t v = 0; v < V; ++v) if (q[v] != 0.0) loss += q[v] * (lse - z[v]);
+            ovf |= store_out(l, (uint8_t *)base[l->n_inputs], obase, (float)loss);
+            if (l->n_inputs > lse_at) ((float *)base[lse_at])[lbase] = (float)lse;
+        } else {
+            const double ct = (double)load_real(base[first], l->in[first].dtype, offset_of(l->in[first].stride, l->dims, 0, no, row)) / tau, lse = ((const float *)base[lse_at])[lbase];
+            for (int64_t v = 0; v < V; ++v) z[v] = (exp(z[v] - lse) - q[v]) * ct;
+#pragma omp parallel for schedule(static)
+            for (int64_t d = 0; d < D; ++d) {
+                double acc = 0.0;
+                for (int64_t v = 0; v < V; ++v) acc += z[v] * (double)load_real(base[1], W->dtype, v * W->stride[no] + d * W->stride[no + 1]);
+                dx[d] = acc;
+            }
+            for (int64_t d = 0; d < D; ++d) ovf |= store_out(l, (uint8_t *)base[l->n_inputs], obase + d * l->out.stride[no + 1], (float)dx[d]);
+            if (dw)
+#pragma omp parallel for schedule(static)
+                for (int64_t v = 0; v < V; ++v)
+                    for (int64_t d = 0; d < D; ++d) dw[v * D + d] += z[v] * x[d];
+        }
+    }
+    if (dw) {
+        psk_launch to = *l;
+        to.out = l->in[dw_at];
+        to.dtype = to.out.dtype;
+        for (int64_t v = 0; v < V; ++v)
+            for (int64_t d = 0; d < D; ++d) ovf |= store_out(&to, (uint8_t *)base[dw_at], v * to.out.stride[no] + d * to.out.stride[no + 1], (float)dw[v * D + d]);
+    }
+    free(dw); free(z); free(q); free(x); free(dx);
+    if (l->guarded) *overflow |= ovf;
+    return bad ? PSK_E7001 : PSK_OK;
+}
+
 /* PSK_OP_RMSNORM is by definition RMSNorm.apply's four launches (examples/coverage/llama.psk:34-40): mul, mean over
  * the last axis, [add eps; sqrt], [div; mul gamma], each the reference's own nest with its result in its site's type. */
 static int rmsnorm_unfused(const psk_launch *l, void *const *table, uint32_t *overflow)
@@ -695,6 +803,7 @@ int psk_oracle_run(const psk_launch *l, void *const *table, uint32_t *overflow)
     if (l->op == PSK_OP_ROPE) return rope_unfused(l, table, overflow);
     if (l->op == PSK_OP_ATTENTION) return attention_unfused(l, table, overflow);
     if (l->op == PSK_OP_RMSNORM) return rmsnorm_unfused(l, table, overflow);
+    if (l->op >= PSK_OP_HEAD_XENT && l->op <= PSK_OP_HEAD_DISTILL_VJP) return head_loss(l, table, overflow);
     if (l->op == PSK_OP_CONTRACT && l->order == PSK_ORDER_CHUNKED && l->n_inner != 1) return PSK_E7005; /* lower.rs:429-431: a chunked order sums ONE summed axis */
     if (l->op == PSK_OP_CONTRACT && l->n_inner > 1) {
         psk_launch m = *l;

@@ -383,3 +383,74 @@ def launch_desc(op, dtype, dims_outer, dims_inner=(), order=abi.ORDER_SEQUENTIAL
     for i, d in enumerate(list(dims_outer) + list(dims_inner)):
         l.dims[i] = d
     return l
+
+
+def _head_launch(vjp, outer, vocab, model, dtype, x_strides, vocab_major, top, teacher_dtype, temperature, loss_dtype, ct_dtype, second, dx_strides):
+    outer = (outer,) if isinstance(outer, int) else tuple(int(n) for n in outer)
+    no = len(outer)
+
+    def dense(shape):
+        st, acc = [], 1
+        for n in reversed(shape):
+            st.append(acc)
+            acc *= n
+        return list(reversed(st))
+
+    if top:
+        op, name = (abi.OP_HEAD_DISTILL_VJP, b"head_distill_vjp") if vjp else (abi.OP_HEAD_DISTILL, b"head_distill")
+    else:
+        op, name = (abi.OP_HEAD_XENT_VJP, b"head_xent_vjp") if vjp else (abi.OP_HEAD_XENT, b"head_xent")
+    l = launch_desc(op, dtype if vjp else loss_dtype, outer, (vocab, model) + ((top,) if top else ()), order=abi.ORDER_DEVICE, name=name)
+    l.fparam[0] = float(temperature)
+    rows = 1
+    for n in outer:
+        rows *= n
+
+    def fill(o, dt, numel, stride, index=0):
+        o.dtype, o.is_index, o.numel = dt, index, numel
+        for a, st in enumerate(stride):
+            o.stride[a] = st
+
+    def over_x(strides):
+        strides = dense(outer + (model,)) if strides is None else [int(n) for n in strides]
+        if len(strides) != no + 1:
+            raise ValueError(f"strides over {no} axes of rows and the model, not {len(strides)}")
+        return strides[:no] + [0, strides[no]]
+
+    w_strides = [0] * no + ([model, 1] if vocab_major else [1, vocab])
+    operands = [(dtype, rows * model, over_x(x_strides), 0), (dtype, vocab * model, w_strides, 0)]
+    if top:
+        listed = [n * top for n in dense(outer)] + [0, 0, 1]
+        operands += [(abi.I64, rows * top, listed, 1), (teacher_dtype, rows * top, listed, 0)]
+    else:
+        operands += [(abi.I64, rows, dense(outer), 1)]
+    if vjp:
+        operands += [(ct_dtype, rows, dense(outer), 0)]
+    if vjp or second:
+        operands += [(abi.F32, rows, dense(outer), 0)]
+    if vjp and second:
+        operands += [(dtype, vocab * model, w_strides, 0)]
+    l.n_inputs = len(operands)
+    for i, o in enumerate(operands):
+        fill(l.inputs[i], *o)
+    if vjp:
+        fill(l.out, dtype, rows * model, over_x(dx_strides))
+    else:
+        fill(l.out, loss_dtype, rows, dense(outer))
+    return l
+
+
+def head_loss_launch(outer, vocab, model, dtype=abi.BF16, *, x_strides=None, vocab_major=False, top=0, teacher_dtype=abi.F32, temperature=1.0, loss_dtype=abi.F32, lse=True):
+    """The launch of the loss through the head: `PSK_OP_HEAD_XENT`, or with `top` > 0 `PSK_OP_HEAD_DISTILL` from a
+    teacher's `top` logits a row at `temperature`. `outer`: the rows, a number or their axes; x lies dense over them
+    unless `x_strides` (elements, over the rows' axes and the model) says otherwise; w is [model, vocab], or [vocab,
+    model] with `vocab_major`. The pointer table of `Executor.run`: x, w, labels (or classes, teacher), the rows'
+    log-sum-exp (f32; left out with lse=False), the loss. Every operand's strides may be set anew in the result."""
+    return _head_launch(False, outer, vocab, model, dtype, x_strides, vocab_major, top, teacher_dtype, temperature, loss_dtype, None, lse, None)
+
+
+def head_loss_vjp_launch(outer, vocab, model, dtype=abi.BF16, *, x_strides=None, vocab_major=False, top=0, teacher_dtype=abi.F32, temperature=1.0, ct_dtype=abi.F32, dw=True, dx_strides=None):
+    """The launch of its gradients (`PSK_OP_HEAD_XENT_VJP`, `PSK_OP_HEAD_DISTILL_VJP`). The pointer table: x, w, labels
+    (or classes, teacher), the loss's cotangent a row, the log-sum-exp that the forward launch wrote, dw (laid out as
+    w; left out with dw=False: a head that is not trained), dx (dense unless `dx_strides`)."""
+    return _head_launch(True, outer, vocab, model, dtype, x_strides, vocab_major, top, teacher_dtype, temperature, None, ct_dtype, dw, dx_strides)

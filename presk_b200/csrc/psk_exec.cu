@@ -26,14 +26,13 @@
 #include "psk_attn_step.cuh"
 #include "psk_gemm_i8.cuh"
 #include "psk_gemm_tc2.cuh"
+#include "psk_head.h"
 
 using namespace psk;
 
 namespace {
 
 constexpr int kFlagSlots = 4096;
-
-typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
 std::string g_create_error;
 
@@ -954,6 +953,9 @@ int psk_exec_run(psk_exec *e, const psk_launch *l, void *const *table)
     const int naxes = l->n_outer + l->n_inner;
     if (!e->causal.empty() && l->op != PSK_OP_MAGNITUDE) e->causal.erase(table[l->n_inputs]); // whatever this launch writes is no longer known to be a causal mask
     if (!e->widened.empty() && l->op != PSK_OP_MAGNITUDE && (l->out.dtype == PSK_I8 || l->out.dtype == PSK_E4M3)) forget_widened(e, table[l->n_inputs]);
+    const bool head = l->op >= PSK_OP_HEAD_XENT && l->op <= PSK_OP_HEAD_DISTILL_VJP;
+    if (head && !e->causal.empty()) // its second results are among the inputs
+        for (int i = 3; i < l->n_inputs; ++i) e->causal.erase(table[i]);
     DevLaunch L;
     memset(&L, 0, sizeof L);
     L.n_in = l->n_inputs; L.n_outer = l->n_outer; L.n_inner = l->n_inner; L.kdtype = l->dtype;
@@ -981,7 +983,7 @@ int psk_exec_run(psk_exec *e, const psk_launch *l, void *const *table)
     L.fparam = (float)l->fparam[0];
     L.status = e->status;
     L.ovf = L.guarded ? next_flag(e, l) : e->flags;
-    if (l->op != PSK_OP_EMBED && l->op != PSK_OP_EMBED_VJP && l->op != PSK_OP_IOTA && l->op != PSK_OP_MAGNITUDE && l->op != PSK_OP_ATTENTION && l->op != PSK_OP_RMSNORM && l->op != PSK_OP_ROPE) coalesce_outer(L);
+    if (!head && l->op != PSK_OP_EMBED && l->op != PSK_OP_EMBED_VJP && l->op != PSK_OP_IOTA && l->op != PSK_OP_MAGNITUDE && l->op != PSK_OP_ATTENTION && l->op != PSK_OP_RMSNORM && l->op != PSK_OP_ROPE) coalesce_outer(L);
     L.total = 1;
     for (int a = 0; a < L.n_outer; ++a) L.total *= L.dims[a];
     L.inner = 1;
@@ -1007,7 +1009,7 @@ int psk_exec_run(psk_exec *e, const psk_launch *l, void *const *table)
     e->last_kernel = "other";
     e->last_flops = 0;
     int rc = PSK_OK;
-    if (L.total == 0 && l->op != PSK_OP_MAGNITUDE && l->op != PSK_OP_EMBED_VJP) {
+    if (L.total == 0 && !head && l->op != PSK_OP_MAGNITUDE && l->op != PSK_OP_EMBED_VJP) {
         // an empty result: nothing to store (embed_vjp still zero-fills its table)
     } else switch (l->op) {
     case PSK_OP_FUSED: {
@@ -1664,6 +1666,15 @@ int psk_exec_run(psk_exec *e, const psk_launch *l, void *const *table)
             k_embed_vjp<<<(int)std::min<int64_t>(l->iparam[0], (int64_t)e->sms * 8), 256, 0, e->stream>>>(L);
             e->kernels += 1;
         }
+        break;
+    }
+    case PSK_OP_HEAD_XENT: case PSK_OP_HEAD_XENT_VJP: case PSK_OP_HEAD_DISTILL: case PSK_OP_HEAD_DISTILL_VJP: {
+        e->last_kernel = "k_head";
+        HeadContext x{e, e->stream, e->encode, e->sms, e->status, L.ovf, L.guarded != 0};
+        rc = head_run(x, l, table);
+        if (rc != PSK_OK) e->error = x.error;
+        e->kernels += x.kernels;
+        e->last_flops = x.flops;
         break;
     }
     case PSK_OP_ARGMAX:

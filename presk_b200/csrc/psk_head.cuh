@@ -1,0 +1,663 @@
+// The loss at the end of a language model, taken through the head in pieces of the vocabulary (PSK_OP_HEAD_XENT,
+// PSK_OP_HEAD_DISTILL and their _VJP): the logits l = x·w exist only as accumulators in tensor memory and registers.
+//
+// Forward. One pass over the vocabulary: a tile of 128 rows by 256 classes is multiplied on the tensor cores, and its
+// epilogue reduces each row's 128 columns a thread to a maximum m and z = sum of 2^((l - m)·c), c = log2 e / τ, which
+// k_head_join puts together over the tiles: ln sum exp(l / τ) = (M + log2 sum z·2^(m - M)) ln 2 with m in units of c.
+// The targets' logits are picked out of the same registers. Backward. The tile is multiplied again, the epilogue
+// writes g = ct/τ (2^(l·c - lse) - p) of a piece of the vocabulary, and two more products give dx and dw from it.
+//
+// Why the sums are kept twice. tcgen05 adds into its f32 accumulator by truncation: measured here, a sum of 4096
+// products comes out 4.4e-6 (products of both signs) to 1.4e-5 (of one sign) too small, always towards zero, where a
+// loss is the difference of two logits. So the accumulator holds `chunk` steps of the summed axis only, and the
+// epilogue's threads add it, rounded to nearest, into registers while the next chunk runs in the other accumulator.
+// f32 operands are three bf16 planes each (x = hi + mid + lo exactly) and six of the nine partial products (those
+// of 2^-16 and up; the three left out are below 2^-24 of the product), one after the other inside a chunk.
+#pragma once
+#include "psk_dev.cuh"
+#include "psk_gemm_tc.cuh"
+
+namespace psk {
+namespace head {
+
+constexpr int BM = 128, BN = 256, BK = 64;
+// Three warpgroups: warp 0 issues the TMA loads, warp 1 the products (2 and 3 idle); warps 4 to 11 are the epilogue, two
+// a quadrant of tensor memory, 128 columns each. An epilogue thread keeps its 128 sums in registers, so the first
+// warpgroup gives most of its share up: 128·40 + 256·232 = 384·168, what the block is launched with.
+constexpr int THREADS = 384;
+constexpr int REGS_FEW = 40, REGS_MANY = 232, REGS_LAUNCH = 168;
+static_assert(128 * REGS_FEW + 256 * REGS_MANY <= THREADS * REGS_LAUNCH, "setmaxnreg waits for registers that the block does not have");
+constexpr int STAGES = 4;
+constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2;
+constexpr int TILE_BYTES = STAGES * (A_BYTES + B_BYTES);
+constexpr int STAGE_OUT = 8 * 32 * 128;
+constexpr int SMEM_TOTAL = TILE_BYTES + 256 + STAGE_OUT + 1024;
+constexpr int COLS = 128; // columns of a tile an epilogue thread holds
+
+enum { MODE_STATS = 0, MODE_GRAD = 1, MODE_OUT = 2 };
+
+// Planes of the partial product q of an f32 contraction: (a, b) = (0,0) (0,1) (1,0) (0,2) (2,0) (1,1).
+PSK_DEV int plane_a(int q) { return (0x120100 >> (4 * q)) & 15; }
+PSK_DEV int plane_b(int q) { return (0x102010 >> (4 * q)) & 15; }
+
+struct Params {
+    int64_t m, n;                 // rows and columns of the product
+    int64_t tiles_m, tiles_n, splits, panel;
+    int32_t kb_k, nprod;          // blocks of 64 along the summed axis; partial products a block (1, or 6 for f32 planes)
+    int32_t kb_split;             // blocks of the summed axis a split
+    int32_t chunk;                // steps (block, partial product) in one accumulator before it is added into registers
+    int32_t in_f16, a_m_major, b_n_major;
+    uint32_t *status;
+    // MODE_STATS, MODE_GRAD
+    float c;                      // log2 e / τ
+    int64_t rows;                 // rows with a target list (m may be larger: rows of zeros)
+    int64_t col0;                 // the class of column 0: where the piece begins
+    const int32_t *label;         // one class a row, or -1; or null, and then
+    const int32_t *ids;           // rows x top classes in ascending order, absent entries last as 0x7fffffff
+    const float *p;               // their weights
+    int32_t top;
+    // MODE_STATS
+    float2 *part;                 // [2·tile column][row]: (max·c, sum of 2^(l·c - max·c))
+    float *hit;                   // label: [row], the label's logit; list: [2·tile column][row], sum of p·l
+    int64_t part0;                // index of the piece's first half-tile column
+    // MODE_GRAD
+    const float *lse2, *coef;     // a row's log-sum-exp in base 2, and ct/τ (0 where it has no target)
+    const uint32_t *scale;        // binary16: the exponent (biased, see k_head_scale) g is multiplied up by; or null
+    uint16_t *g;
+    int64_t g_ld, g_plane;        // row stride; distance of the planes of an f32 operand's g (0: one plane)
+    int64_t g_lo;                 // rows further down where g - (g as stored) goes too (0: nowhere)
+    // MODE_OUT
+    float *out;                   // [split][m][out_ld]
+    int64_t out_ld;
+    int32_t accumulate;           // add to what is there (a later piece of the summed axis)
+};
+
+PSK_DEV float ex2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+PSK_DEV float bf16_up(uint32_t h) { return __uint_as_float(h << 16); }
+
+// First entry of a row's ascending list that is at least `c`.
+PSK_DEV int lower_bound(const int32_t *ids, int n, int32_t c)
+{
+    int lo = 0, hi = n;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (ids[mid] < c) lo = mid + 1;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// 128 bytes of each of this warp's 32 rows: from the threads' packed words through a staging tile (16-byte units
+// swizzled by the row), so that a store instruction writes whole lines (8 lanes a row, 4 rows an instruction).
+// `units`: how many of the 8 units of 16 bytes lie inside the matrix.
+template <bool ADD>
+PSK_DEV void store_rows(uint4 *stage, int lane, const uint32_t (&w)[32], uint8_t *base, int64_t ld_bytes, int rows_live, int units)
+{
+#pragma unroll
+    for (int q = 0; q < 8; ++q) stage[lane * 8 + (q ^ (lane & 7))] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+    __syncwarp();
+    const int unit = lane & 7;
+#pragma unroll
+    for (int it = 0; it < 8; ++it) {
+        const int rr = it * 4 + (lane >> 3);
+        if (rr < rows_live && unit < units) {
+            uint4 v = stage[rr * 8 + (unit ^ (rr & 7))];
+            uint4 *dst = reinterpret_cast<uint4 *>(base + rr * ld_bytes + unit * 16);
+            if (ADD) {
+                const uint4 o = *dst;
+                v = make_uint4(__float_as_uint(__fadd_rn(__uint_as_float(o.x), __uint_as_float(v.x))), __float_as_uint(__fadd_rn(__uint_as_float(o.y), __uint_as_float(v.y))),
+                               __float_as_uint(__fadd_rn(__uint_as_float(o.z), __uint_as_float(v.z))), __float_as_uint(__fadd_rn(__uint_as_float(o.w), __uint_as_float(v.w))));
+            }
+            *dst = v;
+        }
+    }
+    __syncwarp();
+}
+
+// The product of a persistent CTA's tiles, and what MODE makes of it. Bounds: the tensor pipe (2·m·n·k flops) for many
+// rows; for few, the bytes of the second operand.
+template <int MODE>
+__global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ Params P)
+{
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint8_t *smem_a = smem, *smem_b = smem + STAGES * A_BYTES;
+    uint64_t *bars = (uint64_t *)(smem + TILE_BYTES);
+    // full[STAGES], empty[STAGES], accumulator full[2], accumulator empty[2]
+    uint32_t *tmem_slot = (uint32_t *)(bars + 2 * STAGES + 4);
+    volatile int *abort_flag = (volatile int *)(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t full0 = tc::smem_u32(bars), empty0 = tc::smem_u32(bars + STAGES);
+    const uint32_t tfull0 = tc::smem_u32(bars + 2 * STAGES), tempty0 = tc::smem_u32(bars + 2 * STAGES + 2);
+
+    if (threadIdx.x == 0) {
+        *abort_flag = 0;
+        for (int s = 0; s < STAGES; ++s) { tc::mbar_init(full0 + 8 * s, 1); tc::mbar_init(empty0 + 8 * s, 1); }
+        for (int s = 0; s < 2; ++s) { tc::mbar_init(tfull0 + 8 * s, 1); tc::mbar_init(tempty0 + 8 * s, 8); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(tmem_slot)), "r"(2 * BN) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem_base = *tmem_slot;
+
+    const int64_t per_split = P.tiles_m * P.tiles_n, total = per_split * P.splits;
+    // the steps of a split: blocks kb_first .. of the summed axis, nprod partial products each
+    auto steps_of = [&](int64_t sp, int &kb_first) {
+        kb_first = (int)sp * P.kb_split;
+        const int left = P.kb_k - kb_first;
+        return (left < P.kb_split ? left : P.kb_split) * P.nprod;
+    };
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_FEW));
+        if (warp == 0 && lane == 0) {
+            uint32_t stage = 0, phase = 0;
+            bool ok = true;
+            for (int64_t t = blockIdx.x; t < total && ok; t += gridDim.x) {
+                int64_t mt, nt;
+                tc::tile_of(t % per_split, P.tiles_m, P.tiles_n, P.panel, mt, nt);
+                const int m0 = (int)mt * BM, n0 = (int)nt * BN;
+                int kb0;
+                const int steps = steps_of(t / per_split, kb0);
+                int kb = kb0, q = 0;
+                for (int s = 0; s < steps; ++s) {
+                    ok = tc::mbar_wait(empty0 + 8 * stage, phase ^ 1u, abort_flag, P.status, 1u);
+                    if (!ok) break;
+                    const uint32_t fb = full0 + 8 * stage;
+                    tc::mbar_expect_tx(fb, A_BYTES + B_BYTES);
+                    const int k0 = kb * BK, pa = P.nprod == 1 ? 0 : plane_a(q), pb = P.nprod == 1 ? 0 : plane_b(q);
+                    const uint32_t sa = tc::smem_u32(smem_a + stage * A_BYTES), sb = tc::smem_u32(smem_b + stage * B_BYTES);
+                    if (!P.a_m_major) tc::tma_load_4d(sa, &map_a, fb, k0, m0, pa, 0);
+                    else
+#pragma unroll
+                        for (int c = 0; c < BM / 64; ++c) tc::tma_load_4d(sa + c * 8192, &map_a, fb, m0 + c * 64, k0, pa, 0);
+                    if (!P.b_n_major) tc::tma_load_4d(sb, &map_b, fb, k0, n0, pb, 0);
+                    else
+#pragma unroll
+                        for (int c = 0; c < BN / 64; ++c) tc::tma_load_4d(sb + c * 8192, &map_b, fb, n0 + c * 64, k0, pb, 0);
+                    if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                    if (++q == P.nprod) { q = 0; ++kb; }
+                }
+            }
+        }
+        if (warp == 1 && lane == 0) {
+            const uint32_t idesc = tc::instr_desc(P.in_f16, P.b_n_major, BN, P.a_m_major);
+            uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
+            bool ok = true;
+            for (int64_t t = blockIdx.x; t < total && ok; t += gridDim.x) {
+                int kb0;
+                const int steps = steps_of(t / per_split, kb0);
+                int in_chunk = 0;
+                for (int s = 0; s < steps; ++s) {
+                    if (in_chunk == 0) {
+                        ok = tc::mbar_wait(tempty0 + 8 * acc, acc_phase ^ 1u, abort_flag, P.status, 2u);
+                        if (!ok) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    }
+                    ok = tc::mbar_wait(full0 + 8 * stage, phase, abort_flag, P.status, 3u);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t sa = tc::smem_u32(smem_a + stage * A_BYTES), sb = tc::smem_u32(smem_b + stage * B_BYTES);
+#pragma unroll
+                    for (int k = 0; k < BK / tc::UMMA_K; ++k) {
+                        const uint64_t ad = P.a_m_major ? tc::smem_desc(sa + k * 2048, 8192, 1024) : tc::smem_desc(sa + k * 32, 16, 1024);
+                        const uint64_t bd = P.b_n_major ? tc::smem_desc(sb + k * 2048, 8192, 1024) : tc::smem_desc(sb + k * 32, 16, 1024);
+                        tc::umma(tmem_base + acc * BN, ad, bd, idesc, (in_chunk | k) != 0 ? 1u : 0u);
+                    }
+                    tc::umma_commit(empty0 + 8 * stage);
+                    if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                    if (++in_chunk == P.chunk || s + 1 == steps) {
+                        tc::umma_commit(tfull0 + 8 * acc);
+                        in_chunk = 0;
+                        if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+                    }
+                }
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_MANY));
+        const int quad = warp & 3, half = (warp - 4) >> 2;
+        uint4 *stage_out = reinterpret_cast<uint4 *>(smem + TILE_BYTES + 256) + (warp - 4) * 32 * 8;
+        uint32_t acc = 0, acc_phase = 0;
+        bool ok = true;
+        for (int64_t t = blockIdx.x; t < total && ok; t += gridDim.x) {
+            int64_t mt, nt;
+            tc::tile_of(t % per_split, P.tiles_m, P.tiles_n, P.panel, mt, nt);
+            const int64_t sp = t / per_split, row0 = mt * BM + quad * 32, row = row0 + lane, cbase = nt * BN + half * COLS;
+            int kb0;
+            const int steps = steps_of(sp, kb0), chunks = (steps + P.chunk - 1) / P.chunk;
+            float v[COLS];
+            for (int ch = 0; ch < chunks; ++ch) {
+                ok = tc::mbar_wait(tfull0 + 8 * acc, acc_phase, abort_flag, P.status, 4u);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t ta = tmem_base + ((uint32_t)(quad * 32) << 16) + acc * BN + half * COLS;
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    uint32_t r[32];
+                    tc::tmem_ld32(ta + g * 32, r);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    if (ch == 0) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[g * 32 + i] = __uint_as_float(r[i]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[g * 32 + i] = __fadd_rn(v[g * 32 + i], __uint_as_float(r[i]));
+                    }
+                }
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(tempty0 + 8 * acc);
+                if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+            }
+            if (!ok) break;
+            const int rows_live = P.m - row0 < 32 ? (int)(P.m - row0) : 32;
+            if (rows_live <= 0 || cbase >= P.n) continue; // the whole warp
+            const int live = P.n - cbase < COLS ? (int)(P.n - cbase) : COLS; // columns inside the matrix
+            if constexpr (MODE == MODE_STATS || MODE == MODE_GRAD) {
+                if (live < COLS) {
+#pragma unroll
+                    for (int i = 0; i < COLS; ++i)
+                        if (i >= live) v[i] = -INFINITY;
+                }
+            }
+            const int32_t first = (int32_t)(P.col0 + cbase); // the class of v[0]
+            const bool own = row < P.rows;
+            if constexpr (MODE == MODE_STATS) {
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int i = 0; i < COLS; ++i) mx[i & 3] = fmaxf(mx[i & 3], v[i]);
+                const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                const float mc = __fmul_rn(m, P.c), shift = m == -INFINITY ? 0.0f : mc;
+                float hit = 0.0f;
+                const int64_t th = P.part0 + 2 * nt + half;
+                if (own) {
+                    if (P.label) {
+                        const int32_t y = P.label[row] - first;
+                        if (y >= 0 && y < live) {
+#pragma unroll
+                            for (int i = 0; i < COLS; ++i)
+                                if (i == y) hit = v[i];
+                            P.hit[row] = hit;
+                        }
+                    } else {
+                        const int32_t *ids = P.ids + row * P.top;
+                        const float *p = P.p + row * P.top;
+                        for (int j = lower_bound(ids, P.top, first); j < P.top; ++j) {
+                            const int32_t y = ids[j] - first;
+                            if (y >= live) break;
+                            float l = 0.0f;
+#pragma unroll
+                            for (int i = 0; i < COLS; ++i)
+                                if (i == y) l = v[i];
+                            hit = __fmaf_rn(p[j], l, hit);
+                        }
+                        P.hit[th * P.rows + row] = hit;
+                    }
+                }
+                float z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int i = 0; i < COLS; ++i) z[i & 3] = __fadd_rn(z[i & 3], ex2(__fmaf_rn(v[i], P.c, -shift)));
+                if (own) P.part[th * P.rows + row] = make_float2(mc, __fadd_rn(__fadd_rn(z[0], z[1]), __fadd_rn(z[2], z[3])));
+            } else if constexpr (MODE == MODE_GRAD) {
+                const float lse2 = own ? P.lse2[row] : 0.0f;
+                float coef = own ? P.coef[row] : 0.0f;
+                const bool none = !own || (P.label ? P.label[row] < 0 : P.ids[row * P.top] == 0x7fffffff); // no target: zeros, whatever the row holds
+                if (P.scale) coef = __fmul_rn(coef, __uint_as_float(*P.scale));
+#pragma unroll
+                for (int i = 0; i < COLS; ++i) v[i] = ex2(__fmaf_rn(v[i], P.c, -lse2));
+                if (!none) {
+                    if (P.label) {
+                        const int32_t y = P.label[row] - first;
+                        if (y >= 0 && y < live) {
+#pragma unroll
+                            for (int i = 0; i < COLS; ++i)
+                                if (i == y) v[i] = __fadd_rn(v[i], -1.0f);
+                        }
+                    } else {
+                        const int32_t *ids = P.ids + row * P.top;
+                        const float *p = P.p + row * P.top;
+                        for (int j = lower_bound(ids, P.top, first); j < P.top; ++j) {
+                            const int32_t y = ids[j] - first;
+                            if (y >= live) break;
+                            const float pj = p[j];
+#pragma unroll
+                            for (int i = 0; i < COLS; ++i)
+                                if (i == y) v[i] = __fsub_rn(v[i], pj);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < COLS; ++i) v[i] = none ? 0.0f : __fmul_rn(v[i], coef);
+                // Rounded to the operand's type for the two products that read it (2^-9 an entry on average, of terms
+                // of both signs). Where the rest of a rounding is kept too (few rows; the planes of f32), it is the
+                // exact remainder rounded again.
+                uint8_t *base = (uint8_t *)(P.g + row0 * P.g_ld + cbase);
+                const int planes = P.g_plane ? 3 : P.g_lo ? 2 : 1;
+                const int64_t step = (P.g_plane ? P.g_plane : P.g_lo * P.g_ld) * 2;
+                for (int pl = 0; pl < planes; ++pl) {
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+                        uint32_t w[32];
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            float a = v[g * 64 + 2 * i], b = v[g * 64 + 2 * i + 1];
+                            w[i] = P.in_f16 ? pack_f16x2_hw(a, b) : pack_bf16x2_hw(a, b);
+                            if (planes > 1) {
+                                if (P.in_f16) {
+                                    v[g * 64 + 2 * i] = __fsub_rn(a, f16_to_f32((uint16_t)(w[i] & 0xffffu)));
+                                    v[g * 64 + 2 * i + 1] = __fsub_rn(b, f16_to_f32((uint16_t)(w[i] >> 16)));
+                                } else {
+                                    v[g * 64 + 2 * i] = __fsub_rn(a, bf16_up(w[i] & 0xffffu));
+                                    v[g * 64 + 2 * i + 1] = __fsub_rn(b, bf16_up(w[i] >> 16));
+                                }
+                            }
+                        }
+                        const int64_t left = (P.g_ld - cbase - g * 64) / 8; // the rows are padded to whole lines, the padding zeros
+                        store_rows<false>(stage_out, lane, w, base + g * 128 + pl * step, P.g_ld * 2, rows_live, left < 8 ? (int)left : 8);
+                    }
+                }
+            } else {
+                float *base = P.out + sp * P.m * P.out_ld + row0 * P.out_ld + cbase;
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    uint32_t w[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(v[g * 32 + i]);
+                    const int64_t left = ((P.n + 3) / 4 * 4 - cbase - g * 32) / 4;
+                    if (P.accumulate) store_rows<true>(stage_out, lane, w, (uint8_t *)(base + g * 32), P.out_ld * 4, rows_live, left < 8 ? (int)left : 8);
+                    else store_rows<false>(stage_out, lane, w, (uint8_t *)(base + g * 32), P.out_ld * 4, rows_live, left < 8 ? (int)left : 8);
+                }
+            }
+        }
+    }
+
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(2 * BN) : "memory");
+    }
+}
+
+// ---- what stands around the products -----------------------------------------------------------------------------
+
+// A strided operand over the launch's rows (axes 0 .. no - 1 of `dims`).
+struct RowOperand {
+    const void *p;
+    int32_t dtype;
+    int64_t stride[PSK_MAX_AXES];
+};
+
+struct RowSpace {
+    int32_t no;
+    int64_t dims[PSK_MAX_AXES];
+    int64_t rows;
+};
+
+PSK_DEV int64_t row_offset(const RowSpace &s, const int64_t *stride, int64_t row)
+{
+    int64_t off = 0;
+    for (int a = s.no - 1; a >= 0; --a) {
+        off += row % s.dims[a] * stride[a];
+        row /= s.dims[a];
+    }
+    return off;
+}
+
+// Labels as classes (32 bits; -1 where a row has none) and, backward, a row's factor ct/τ and its log-sum-exp in
+// base 2. A class that the vocabulary does not have is reported and counts as no target.
+struct LabelParams {
+    RowSpace s;
+    RowOperand ids, ct, lse;
+    int64_t classes;
+    float inv_tau;
+    int32_t *label;
+    float *coef, *lse2;
+    uint32_t *status, *ctmax;
+};
+
+// ct and lse of a row, for either kind of target. Rows that a launch's weight leaves out keep the value they have.
+PSK_DEV void row_factors(const RowSpace &s, const RowOperand &ct, const RowOperand &lse, int64_t row, bool none, float inv_tau, float *coef, float *lse2, uint32_t *ctmax)
+{
+    if (!coef) return;
+    const float c = none ? 0.0f : __fmul_rn(load_real(ct.p, ct.dtype, row_offset(s, ct.stride, row)), inv_tau);
+    coef[row] = c;
+    lse2[row] = none ? 0.0f : (float)((double)load_real(lse.p, lse.dtype, row_offset(s, lse.stride, row)) * 1.4426950408889634);
+    if (ctmax && !none && fabsf(c) <= 3.4e38f) atomicMax(ctmax, __float_as_uint(fabsf(c))); // non-negative floats order as their bits do: no order of the rows changes it
+}
+
+static __global__ void __launch_bounds__(256) k_head_labels(const __grid_constant__ LabelParams P)
+{
+    const int64_t row = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (row >= P.s.rows) return;
+    const int64_t y = ((const int64_t *)P.ids.p)[row_offset(P.s, P.ids.stride, row)];
+    if (y >= P.classes) atomicOr(P.status, 2u);
+    const bool none = y < 0 || y >= P.classes;
+    P.label[row] = none ? -1 : (int32_t)y;
+    row_factors(P.s, P.ct, P.lse, row, none, P.inv_tau, P.coef, P.lse2, P.ctmax);
+}
+
+// A teacher's entries of one row a block: p = softmax(t/τ) over those kept (an id of zero or more, a logit above
+// minus infinity), sum of p·ln p, and the entries by ascending class (each entry counts those before it: top² integer
+// comparisons in shared memory), so that a tile's epilogue finds its own by bisection.
+struct TeacherParams {
+    RowSpace s;
+    RowOperand ids, t, ct, lse;
+    int64_t ids_k, t_k; // strides along the list
+    int64_t classes;
+    int32_t top;
+    float inv_tau;
+    int32_t *out_ids;
+    float *out_p, *plogp;
+    float *coef, *lse2;
+    uint32_t *status, *ctmax;
+};
+
+template <bool MAX>
+PSK_DEV float block_all(float x, float *red)
+{
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const float y = __shfl_xor_sync(0xffffffffu, x, o);
+        x = MAX ? fmaxf(x, y) : __fadd_rn(x, y);
+    }
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = x;
+    __syncthreads();
+    float r = red[0];
+    for (int w = 1; w < (int)(blockDim.x >> 5); ++w) r = MAX ? fmaxf(r, red[w]) : __fadd_rn(r, red[w]);
+    __syncthreads();
+    return r;
+}
+
+static __global__ void __launch_bounds__(1024) k_head_teacher(const __grid_constant__ TeacherParams P)
+{
+    extern __shared__ int32_t list[]; // top ids
+    __shared__ float red[32];
+    const int64_t row = blockIdx.x;
+    const int j = threadIdx.x;
+    int32_t id = 0x7fffffff;
+    float t = -INFINITY;
+    if (j < P.top) {
+        const int64_t raw = ((const int64_t *)P.ids.p)[row_offset(P.s, P.ids.stride, row) + j * P.ids_k];
+        if (raw >= P.classes) atomicOr(P.status, 2u);
+        if (raw >= 0 && raw < P.classes) {
+            t = __fmul_rn(load_real(P.t.p, P.t.dtype, row_offset(P.s, P.t.stride, row) + j * P.t_k), P.inv_tau);
+            if (!(t == -INFINITY)) id = (int32_t)raw;
+        }
+        list[j] = id;
+    }
+    __syncthreads();
+    const bool here = id != 0x7fffffff;
+    const float m = block_all<true>(here ? t : -INFINITY, red);
+    // a NaN among the entries makes the row NaN: the maximum passes it over, the sum does not
+    const float e = here ? expf(__fsub_rn(t, m)) : 0.0f;
+    const float z = block_all<false>(e, red);
+    const bool none = __syncthreads_count(here) == 0;
+    const float p = here ? __fdiv_rn(e, z) : 0.0f;
+    const float pl = here && p != 0.0f ? __fmul_rn(p, __fsub_rn(__fsub_rn(t, m), logf(z))) : 0.0f;
+    const float sum = block_all<false>(pl, red);
+    if (j < P.top) {
+        int at = 0;
+        for (int i = 0; i < P.top; ++i) at += list[i] < id || (list[i] == id && i < j);
+        P.out_ids[row * P.top + at] = id;
+        P.out_p[row * P.top + at] = p;
+    }
+    if (j == 0) {
+        P.plogp[row] = sum;
+        row_factors(P.s, P.ct, P.lse, row, none, P.inv_tau, P.coef, P.lse2, P.ctmax);
+    }
+}
+
+// The scale of binary16 g: the power of two that brings the largest |ct/τ| into [2^14, 2^15), written as an f32's
+// bits (and its reciprocal). A gradient spread over a vocabulary is far below binary16's least number otherwise; g
+// itself is at most that maximum, so nothing overflows.
+static __global__ void k_head_scale(const uint32_t *ctmax, uint32_t *scale)
+{
+    const int e = (int)(*ctmax >> 23); // biased exponent of the maximum; 0 for zero and subnormals
+    int up = 14 + 127 - e;             // 2^up
+    if (e == 0 || up > 120) up = e == 0 ? 0 : 120;
+    if (up < -120) up = -120;
+    scale[0] = (uint32_t)(127 + up) << 23;
+    scale[1] = (uint32_t)(127 - up) << 23;
+}
+
+// The tiles' (m, z) of a row put together, and its loss. 32 rows a block, the half-tile columns over the block's y.
+struct JoinParams {
+    RowSpace s;
+    int64_t halves; // half-tile columns
+    const float2 *part;
+    const float *hit;
+    const int32_t *label, *ids;
+    const float *plogp;
+    int32_t top;
+    float inv_tau;
+    RowOperand loss, lse; // lse.p may be null
+    uint32_t *ovf;
+    int32_t guarded;
+};
+
+static __global__ void __launch_bounds__(256) k_head_join(const __grid_constant__ JoinParams P)
+{
+    __shared__ float sm[8][33], sz[8][33], sh[8][33];
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+    const int64_t row = (int64_t)blockIdx.x * 32 + x;
+    float m = -INFINITY, z = 0.0f, h = 0.0f;
+    if (row < P.s.rows)
+        for (int64_t th = y; th < P.halves; th += 8) {
+            const float2 a = P.part[th * P.s.rows + row];
+            if (!P.label) h = __fadd_rn(h, P.hit[th * P.s.rows + row]);
+            // (m, z) + (a.x, a.y) about the greater of the two; an empty part has m = -inf and z = 0
+            const float g = fmaxf(m, a.x);
+            if (!(g == -INFINITY)) z = __fadd_rn(__fmul_rn(z, exp2f(__fsub_rn(m, g))), __fmul_rn(a.y, exp2f(__fsub_rn(a.x, g))));
+            m = g;
+        }
+    sm[y][x] = m; sz[y][x] = z; sh[y][x] = h;
+    __syncthreads();
+    if (y != 0 || row >= P.s.rows) return;
+    for (int i = 1; i < 8; ++i) {
+        const float am = sm[i][x], g = fmaxf(m, am);
+        if (!(g == -INFINITY)) z = __fadd_rn(__fmul_rn(z, exp2f(__fsub_rn(m, g))), __fmul_rn(sz[i][x], exp2f(__fsub_rn(am, g))));
+        m = g;
+        h = __fadd_rn(h, sh[i][x]);
+    }
+    const bool none = P.label ? P.label[row] < 0 : P.ids[row * P.top] == 0x7fffffff;
+    const double lse = ((double)m + log2((double)z)) * 0.6931471805599453;
+    double loss;
+    if (P.label) loss = lse - (double)P.hit[row];
+    else loss = (double)P.plogp[row] - (double)h * (double)P.inv_tau + lse;
+    uint32_t ovf = store_real(const_cast<void *>(P.loss.p), P.loss.dtype, row_offset(P.s, P.loss.stride, row), none ? 0.0f : (float)loss);
+    if (P.lse.p) store_real(const_cast<void *>(P.lse.p), P.lse.dtype, row_offset(P.s, P.lse.stride, row), none ? 0.0f : (float)lse);
+    if (P.guarded && ovf) atomicOr(P.ovf, 1u);
+}
+
+// A matrix laid out for the tensor maps: rows of `cols` elements from any strides into rows of `ld` (a multiple of 8),
+// the padding zeros; f32 as three bf16 planes one after the other. Rows without a target (of x, backward) become
+// zeros, so that nothing they hold reaches dw. `copies`: the rows again below themselves (the second operand of a
+// product over g and its remainder).
+struct PackParams {
+    RowSpace s;       // the rows (for w: one axis)
+    RowOperand src;
+    int64_t col_stride, cols, ld, plane;
+    uint16_t *dst;
+    int32_t f32, copies;
+    const int32_t *label, *ids;
+    int32_t top;
+};
+
+static __global__ void __launch_bounds__(256) k_head_pack(const __grid_constant__ PackParams P)
+{
+    const int64_t vecs = P.ld / 8, total = P.s.rows * vecs, step = (int64_t)gridDim.x * blockDim.x;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += step) {
+        const int64_t row = i / vecs, c0 = (i - row * vecs) * 8;
+        bool none = false;
+        if (P.label) none = P.label[row] < 0;
+        else if (P.ids) none = P.ids[row * P.top] == 0x7fffffff;
+        const int64_t off = row_offset(P.s, P.src.stride, row) + c0 * P.col_stride;
+        uint16_t w[3][8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const bool in = !none && c0 + j < P.cols;
+            if (P.f32) {
+                const float x = in ? ((const float *)P.src.p)[off + j * P.col_stride] : 0.0f;
+                const uint32_t hi = pack_bf16x2_hw(x, 0.0f) & 0xffffu;
+                const float r = __fsub_rn(x, bf16_up(hi));
+                const uint32_t mid = pack_bf16x2_hw(r, 0.0f) & 0xffffu;
+                const uint32_t lo = pack_bf16x2_hw(__fsub_rn(r, bf16_up(mid)), 0.0f) & 0xffffu;
+                const bool whole = fabsf(x) <= 3.38e38f; // an infinity or a NaN (or what rounds to one) stays in its first plane
+                w[0][j] = (uint16_t)hi; w[1][j] = whole ? (uint16_t)mid : 0; w[2][j] = whole ? (uint16_t)lo : 0;
+            } else w[0][j] = in ? ((const uint16_t *)P.src.p)[off + j * P.col_stride] : 0;
+        }
+        for (int k = 0; k < P.copies; ++k)
+#pragma unroll
+            for (int pl = 0; pl < 3; ++pl)
+                if (pl == 0 || P.f32)
+                    *reinterpret_cast<uint4 *>(P.dst + pl * P.plane + (k * P.s.rows + row) * P.ld + c0) =
+                        make_uint4(w[pl][0] | (uint32_t)w[pl][1] << 16, w[pl][2] | (uint32_t)w[pl][3] << 16, w[pl][4] | (uint32_t)w[pl][5] << 16, w[pl][6] | (uint32_t)w[pl][7] << 16);
+    }
+}
+
+// A gradient from its f32 partial sums into its place: the splits' sums in their order (and, of few rows, those of g's
+// remainder `fold` rows below), times the binary16 scale's reciprocal, rounded once.
+struct SumParams {
+    RowSpace s;
+    const float *part;
+    int64_t parts, part_rows, ld, fold, cols, col_stride;
+    const uint32_t *scale;
+    RowOperand dst;
+    uint32_t *ovf;
+    int32_t guarded;
+};
+
+static __global__ void __launch_bounds__(256) k_head_sum(const __grid_constant__ SumParams P)
+{
+    const int64_t total = P.s.rows * P.cols, step = (int64_t)gridDim.x * blockDim.x;
+    const float un = P.scale ? __uint_as_float(P.scale[1]) : 1.0f;
+    uint32_t ovf = 0;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += step) {
+        const int64_t row = i / P.cols, c = i - row * P.cols;
+        const float *src = P.part + row * P.ld + c;
+        float a = 0.0f;
+        for (int64_t k = 0; k < P.parts; ++k) {
+            a = __fadd_rn(a, src[k * P.part_rows * P.ld]);
+            if (P.fold) a = __fadd_rn(a, src[(k * P.part_rows + P.fold) * P.ld]);
+        }
+        ovf |= store_real(const_cast<void *>(P.dst.p), P.dst.dtype, row_offset(P.s, P.dst.stride, row) + c * P.col_stride, __fmul_rn(a, un));
+    }
+    if (P.guarded && ovf) atomicOr(P.ovf, 1u);
+}
+
+} // namespace head
+} // namespace psk

@@ -1,0 +1,82 @@
+// What a launch of the head's losses (PSK_OP_HEAD_XENT, PSK_OP_HEAD_DISTILL and their _VJP) has to be, checked before
+// anything is queued. No CUDA here: a test compiles it for the host.
+#pragma once
+#include <stdint.h>
+#include <string>
+#include "../../include/presk_cuda.h"
+
+namespace psk {
+
+struct HeadShape {
+    bool vjp, distill;
+    int first;          // inputs before ct (backward) or the log-sum-exp (forward)
+    int ct, lse, dw;    // their input numbers, -1 where the launch has none
+    int64_t classes, model, top, rows;
+    double tau;
+};
+
+inline int head_shape(const psk_launch *l, HeadShape &h, std::string &error)
+{
+    const std::string nm = l->name ? l->name : "head";
+    auto refuse = [&](int code, const std::string &what) { error = nm + ": " + what; return code; };
+    h.vjp = l->op == PSK_OP_HEAD_XENT_VJP || l->op == PSK_OP_HEAD_DISTILL_VJP;
+    h.distill = l->op == PSK_OP_HEAD_DISTILL || l->op == PSK_OP_HEAD_DISTILL_VJP;
+    if (l->order != PSK_ORDER_DEVICE) return refuse(PSK_E7005, "the head's loss in pieces of the vocabulary is a declared order (device)");
+    h.first = h.distill ? 4 : 3;
+    const int no = l->n_outer, ax_v = no, ax_d = no + 1, ax_k = no + 2, extra = l->n_inputs - h.first;
+    if (no < 1 || no > PSK_MAX_RANK || l->n_inner != (h.distill ? 3 : 2) || (h.vjp ? extra != 2 && extra != 3 : extra != 0 && extra != 1))
+        return refuse(PSK_E7001, std::string("x, w, ") + (h.distill ? "classes, teacher" : "labels") + (h.vjp ? ", ct, lse and at most the place of dw" : " and at most the place of lse") + " over (rows | classes, model" + (h.distill ? ", top)" : ")"));
+    h.ct = h.vjp ? h.first : -1;
+    h.lse = h.vjp ? h.first + 1 : extra == 1 ? h.first : -1;
+    h.dw = h.vjp && extra == 3 ? h.first + 2 : -1;
+    h.classes = l->dims[ax_v]; h.model = l->dims[ax_d]; h.top = h.distill ? l->dims[ax_k] : 1;
+    const int64_t most = 0x7fff0000; // tile coordinates are 32-bit
+    if (h.classes < 1 || h.model < 1 || h.top < 1 || h.classes > most || h.model > most) return refuse(PSK_E7001, "a head of " + std::to_string(h.model) + " x " + std::to_string(h.classes) + ", " + std::to_string(h.top) + " entries a row");
+    if (h.top > 1024) return refuse(PSK_E7005, "at most 1024 of the teacher's entries a row, not " + std::to_string(h.top));
+    h.rows = 1;
+    for (int a = 0; a < no; ++a) {
+        if (l->dims[a] < 0 || (l->dims[a] > 0 && h.rows > (most >> 1) / l->dims[a])) return refuse(PSK_E7001, "more rows than one launch takes, or a negative length");
+        h.rows *= l->dims[a];
+    }
+    auto real = [](const psk_operand &o) { return (o.dtype == PSK_BF16 || o.dtype == PSK_F16 || o.dtype == PSK_F32) && !o.is_index && !o.affine; };
+    const psk_operand &X = l->in[0], &W = l->in[1], &I = l->in[2], &O = l->out;
+    if (!real(X) || !real(W) || X.dtype != W.dtype) return refuse(PSK_E7005, "x and w are stored in one type, bf16, f16 or f32");
+    if (I.dtype != PSK_I64 || !I.is_index) return refuse(PSK_E7001, std::string(h.distill ? "the teacher's classes" : "the labels") + " are indices (i64)");
+    if (h.distill && !real(l->in[3])) return refuse(PSK_E7005, "the teacher's logits are bf16, f16 or f32");
+    if (h.ct >= 0 && !real(l->in[h.ct])) return refuse(PSK_E7005, "the cotangent is bf16, f16 or f32");
+    if (h.lse >= 0 && (l->in[h.lse].dtype != PSK_F32 || l->in[h.lse].is_index)) return refuse(PSK_E7001, "the rows' log-sum-exp is f32");
+    if (!real(O)) return refuse(PSK_E7005, "the result is bf16, f16 or f32");
+    h.tau = h.distill ? l->fparam[0] : 1.0;
+    if (!(h.tau >= 1e-4 && h.tau <= 1e4)) return refuse(PSK_E7001, "a temperature (fparam[0]) between 1e-4 and 1e4, not " + std::to_string(h.tau));
+    const int axes = no + l->n_inner;
+    for (int i = 0; i <= l->n_inputs; ++i)
+        for (int a = 0; a < axes; ++a)
+            if ((i < l->n_inputs ? l->in[i] : O).stride[a] < 0) return refuse(PSK_E7001, "a negative stride");
+    // which axes an operand walks: a stride on any other axis is a description of something else
+    auto walks = [&](const psk_operand &o, bool rows, bool v, bool d, bool k) {
+        for (int a = 0; a < axes; ++a) {
+            const bool may = a < no ? rows : a == ax_v ? v : a == ax_d ? d : k;
+            if (!may && l->dims[a] > 1 && o.stride[a] != 0) return false;
+        }
+        return true;
+    };
+    bool ok = walks(X, true, false, true, false) && walks(W, false, true, true, false) && walks(I, true, false, false, h.distill) && (!h.distill || walks(l->in[3], true, false, false, true))
+        && (h.ct < 0 || walks(l->in[h.ct], true, false, false, false)) && (h.lse < 0 || walks(l->in[h.lse], true, false, false, false))
+        && (h.dw < 0 || walks(l->in[h.dw], false, true, true, false)) && walks(O, true, false, h.vjp, false);
+    if (!ok) return refuse(PSK_E7001, "an operand with a stride along an axis that it does not have");
+    // every element of a result has a place of its own
+    auto spread = [&](const psk_operand &o, bool rows, bool v, bool d) {
+        for (int a = 0; a < axes; ++a)
+            if (l->dims[a] > 1 && o.stride[a] == 0 && (a < no ? rows : a == ax_v ? v : a == ax_d ? d : false)) return false;
+        return true;
+    };
+    ok = spread(O, true, false, h.vjp) && (h.dw < 0 || spread(l->in[h.dw], false, true, true)) && (h.vjp || h.lse < 0 || spread(l->in[h.lse], true, false, false));
+    if (!ok) return refuse(PSK_E7005, "a result with a broadcast axis");
+    if (h.vjp) {
+        // g is rounded to the operands' type before it is multiplied: a result in more bits would claim what it does not hold
+        if (O.dtype != X.dtype || (h.dw >= 0 && (!real(l->in[h.dw]) || l->in[h.dw].dtype != X.dtype))) return refuse(PSK_E7005, "the gradients are stored in the operands' type");
+    }
+    return PSK_OK;
+}
+
+} // namespace psk
