@@ -79,30 +79,33 @@ int fail(HeadContext &x, int code, const std::string &msg)
         if (err__ != cudaSuccess) return fail(x, PSK_E10001, std::string(#call) + ": " + cudaGetErrorString(err__)); \
     } while (0)
 
-template <int MODE>
+template <int MODE, int MT = 1>
 int product(HeadContext &x, Params P, const Operand &a, const Operand &b, int f16)
 {
     CUtensorMap ma, mb;
-    if (!map_of(x, &ma, a, f16, BM) || !map_of(x, &mb, b, f16, BN)) return fail(x, PSK_E10001, "head: an operand's layout does not make a tensor map");
+    if (!map_of(x, &ma, a, f16, BM * MT) || !map_of(x, &mb, b, f16, BN)) return fail(x, PSK_E10001, "head: an operand's layout does not make a tensor map");
     P.m = a.rows; P.n = b.rows;
-    P.tiles_m = (P.m + BM - 1) / BM; P.tiles_n = (P.n + BN - 1) / BN;
+    P.tiles_m = (P.m + BM * MT - 1) / (BM * MT); P.tiles_n = (P.n + BN - 1) / BN;
     P.kb_k = (int32_t)((a.k + BK - 1) / BK);
-    P.nprod = a.planes == 3 ? 6 : 1;
+    P.nprod = a.planes == 2 ? 3 : 1;
     if (MODE != MODE_OUT) { P.splits = 1; P.kb_split = P.kb_k; }
-    P.chunk = P.nprod == 6 ? 6 : 4; // about 256 products of the summed axis an accumulator (see psk_head.cuh)
+    // Steps an accumulator: 512 products of the summed axis (384 of f32's, three a block). Results of 16 bits, dx and dw, keep one
+    // accumulator throughout: what truncation loses there is far below their rounding.
+    P.chunk = MODE == MODE_OUT && P.out_dtype != PSK_F32 ? 1 << 28 : P.nprod == 3 ? 6 : 8;
     // a panel's columns of b stay in a quarter of the L2 while a's rows stream past them
-    P.panel = std::min<int64_t>(P.tiles_n, std::max<int64_t>(8, (32ll << 20) / std::max<int64_t>(1, BN * a.k * 2 * a.planes)));
+    P.panel = std::min<int64_t>(P.tiles_n, std::max<int64_t>(8, (16ll << 20) / std::max<int64_t>(1, BN * a.k * 2 * a.planes)));
     P.in_f16 = f16; P.a_m_major = !a.k_contiguous; P.b_n_major = !b.k_contiguous;
     P.status = x.status;
-    HEAD_TRY(cudaFuncSetAttribute(k_head<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_TOTAL));
+    HEAD_TRY(cudaFuncSetAttribute(k_head<MODE, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<MT>::SMEM_TOTAL));
     const int64_t tiles = P.tiles_m * P.tiles_n * P.splits;
-    k_head<MODE><<<(unsigned)std::min<int64_t>(tiles, x.sms), THREADS, SMEM_TOTAL, x.stream>>>(ma, mb, P);
+    k_head<MODE, MT><<<(unsigned)std::min<int64_t>(tiles, x.sms), THREADS, Cfg<MT>::SMEM_TOTAL, x.stream>>>(ma, mb, P);
     x.kernels += 1;
     x.flops += 2.0 * (double)P.m * (double)P.n * (double)a.k;
     return PSK_OK;
 }
 
-int grid_of(const HeadContext &x, int64_t work) { return (int)std::max<int64_t>(1, std::min<int64_t>((work + 255) / 256, (int64_t)x.sms * 8)); }
+// Blocks of eight warps for `work` warps' worth.
+int warps_of(const HeadContext &x, int64_t work) { return (int)std::max<int64_t>(1, std::min<int64_t>((work + 7) / 8, (int64_t)x.sms * 8)); }
 
 RowOperand row_operand(const psk_operand &o, void *base, int no)
 {
@@ -124,7 +127,7 @@ int head_run(HeadContext &x, const psk_launch *l, void *const *table)
     const std::string nm = l->name ? l->name : "head";
     if (!x.encode) return fail(x, PSK_E10001, "cuTensorMapEncodeTiled is not available from this driver");
     const bool vjp = h.vjp, distill = h.distill;
-    const int no = l->n_outer, ax_v = no, ax_d = no + 1, ax_k = no + 2, first = h.first, dt = l->in[0].dtype;
+    const int no = l->n_outer, ax_v = no, ax_d = no + 1, ax_k = no + 2, dt = l->in[0].dtype;
     const int64_t V = h.classes, D = h.model, K = h.top, N = h.rows;
     const double tau = h.tau;
     const psk_operand &X = l->in[0], &W = l->in[1], &I = l->in[2], &O = l->out;
@@ -137,196 +140,245 @@ int head_run(HeadContext &x, const psk_launch *l, void *const *table)
     HEAD_TRY(cudaStreamIsCapturing(x.stream, &capturing));
     if (capturing != cudaStreamCaptureStatusNone) return fail(x, PSK_E7005, nm + ": its workspace is the executor's, which a graph replayed later would share with other work; not while the stream is being captured");
 
-    const int eb = dt == PSK_F32 ? 4 : 2, f16 = dt == PSK_F16, planes = dt == PSK_F32 ? 3 : 1;
+    const int eb = dt == PSK_F32 ? 4 : 2, f32 = dt == PSK_F32, planes = f32 ? 2 : 1;
     const float inv_tau = (float)(1.0 / tau);
-    const RowOperand rx = row_operand(X, table[0], no), rids = row_operand(I, table[2], no);
+    const RowOperand rx = row_operand(X, table[0], no), rids = row_operand(I, table[2], no), rout = row_operand(O, table[l->n_inputs], no);
     const uint8_t *wp = (const uint8_t *)table[1] + W.offset * eb;
-    const int64_t w_v = W.stride[ax_v], w_d = W.stride[ax_d];
+    const int64_t w_v = W.stride[ax_v], w_d = W.stride[ax_d], Dp = up(D, 8);
     const bool v_inner = w_v == 1 || V == 1; // the head as [model, classes]; otherwise rows of a class, [classes, model]
     auto aligned = [](const void *p) { return ((uintptr_t)p & 15u) == 0; };
     // read where it lies: 16-bit, one axis contiguous, rows on 16-byte boundaries
-    const bool w_direct = planes == 1 && aligned(wp) && (v_inner ? w_v == 1 && w_d % 8 == 0 && w_d >= V : w_d == 1 && w_v % 8 == 0 && w_v >= D);
-    // the rows of x one stride apart: one level over the outer axes
-    bool x_rows = true;
-    int64_t x_ld = 0;
-    {
-        int64_t want = 0;
+    const bool w_direct = !f32 && aligned(wp) && (v_inner ? w_v == 1 && w_d % 8 == 0 && w_d >= V : w_d == 1 && w_v % 8 == 0 && w_v >= D);
+    // the stride of an operand's rows where they are one level over the outer axes; else 0
+    auto row_stride = [&](const psk_operand &o) {
+        int64_t ld = 0, want = 0;
         for (int a = no - 1; a >= 0; --a) {
             if (s.dims[a] == 1) continue;
-            if (X.stride[a] == 0) { x_rows = false; break; }
-            if (!want) { x_ld = X.stride[a]; want = x_ld * s.dims[a]; }
-            else { x_rows = x_rows && X.stride[a] == want; want *= s.dims[a]; }
+            if (o.stride[a] == 0 || (want && o.stride[a] != want)) return (int64_t)0;
+            if (!want) { ld = o.stride[a]; want = ld; }
+            want *= s.dims[a];
         }
-        if (!x_ld) x_ld = up(D, 8);
-    }
-    const bool x_direct = !vjp && planes == 1 && x_rows && X.stride[ax_d] == 1 && x_ld % 8 == 0 && x_ld >= D && aligned(rx.p);
-
-    // backward, few rows: g and what its rounding leaves as rows of their own in the same tile, which costs nothing there
-    const int64_t Ng = vjp && planes == 1 && N <= BM / 2 ? 2 * N : N;
-    const int64_t Dp = up(D, 8), Vp = up(V, 8);
-
+        return ld ? ld : up(D, 8); // one row: its stride is never walked
+    };
+    const int64_t x_ld = row_stride(X);
+    const bool x_direct = !f32 && x_ld && X.stride[ax_d] == 1 && x_ld % 8 == 0 && x_ld >= D && aligned(rx.p);
     if (N == 0 && !vjp) return PSK_OK;
 
+    // Backward, bf16 and binary16 with few rows: g's rounding error is kept as rows of its own below g, and dx and dw
+    // take both. Up to 64 rows that is the same tile of the tensor cores; up to 256 it costs less (4·N·D·V flops) than
+    // copies of x and w in binary16 (6 bytes an element of w), which is what bf16 takes for more.
+    const bool rest = vjp && !f32 && N <= 256, conv = vjp && dt == PSK_BF16 && !rest;
+    const int64_t Ng = rest ? 2 * N : N;
+    const int g_f16 = f32 || conv || dt == PSK_F16, in_f16 = f32 || dt == PSK_F16;
+    const bool g_scaled = vjp && g_f16, any_scale = f32 || g_scaled;
+
     // the vocabulary's pieces
-    int64_t per_col = (vjp ? Ng * planes * 2 : 0) + (w_direct ? 0 : D * planes * 2);
+    const int64_t per_col = (vjp ? Ng * planes * 2 : 0) + (w_direct ? 0 : D * planes * 2) + (conv ? D * 2 : 0);
     int64_t Vc = V;
     if (per_col > 0) {
-        const int64_t most = std::max<int64_t>(BN, kPieceBytes / per_col / BN * BN);
-        if (V > most) Vc = up((V + (V + most - 1) / most - 1) / ((V + most - 1) / most), BN);
+        const int64_t most = std::max<int64_t>(BN, kPieceBytes / per_col / BN * BN), n = (V + most - 1) / most;
+        if (n > 1) Vc = up((V + n - 1) / n, BN);
     }
-    const int64_t pieces = (V + Vc - 1) / Vc, halves = (V + COLS - 1) / COLS;
-    const int64_t g_ld = up(Vc, 64), g_plane = planes == 3 ? Ng * g_ld : 0;
-    const int64_t wc_ld = v_inner ? up(Vc, 8) : Dp, wc_plane = wc_ld * (v_inner ? D : Vc);
-    const bool dw_v_inner = DW && (DW->stride[ax_v] == 1 || V == 1);
-    const int64_t dwm = dw_v_inner ? D : Vc, dwn = dw_v_inner ? Vc : D, dw_ld = up(dwn, 4), dx_ld = up(D, 4);
-    // splits of a product with few tiles along its summed axis, so that every SM has some of it
-    auto splits_of = [&](int64_t m, int64_t n, int64_t k, int32_t &kb_split) {
-        const int64_t tiles = ((m + BM - 1) / BM) * ((n + BN - 1) / BN), kb = (k + BK - 1) / BK;
-        int64_t want = std::max<int64_t>(1, std::min<int64_t>(x.sms / tiles, kb / 4));
-        kb_split = (int32_t)((kb + want - 1) / want);
-        return (kb + kb_split - 1) / kb_split;
+    const int64_t pieces = (V + Vc - 1) / Vc, parts = (V + COLS - 1) / COLS;
+    const int64_t g_ld = up(Vc, 64), wc_ld = v_inner ? up(Vc, 8) : Dp, wc_plane = wc_ld * (v_inner ? D : Vc);
+
+    // Where dx and dw are stored from: straight from the products where one launch has the whole sum and the result's
+    // rows are one level; otherwise through f32 sums (k_head_sum).
+    struct Out { int64_t m, n, ld, splits; int32_t kb_split; bool straight, two; };
+    auto plan = [&](int64_t m, int64_t n, int64_t k, bool may_be_straight) {
+        Out o{m, n, up(n, 4), 1, 0, may_be_straight, false};
+        const int64_t kb = (k + BK - 1) / BK, tiles = ((m + BM - 1) / BM) * ((n + BN - 1) / BN);
+        o.two = !f32 && m >= 2 * BM && tiles >= 2 * x.sms;
+        // few tiles: cut the summed axis, so that every SM has some of it
+        const int64_t want = std::max<int64_t>(1, std::min<int64_t>(x.sms / tiles, kb / 4));
+        o.kb_split = (int32_t)((kb + want - 1) / want);
+        o.splits = (kb + o.kb_split - 1) / o.kb_split;
+        if (o.splits > 1) o.straight = false;
+        return o;
     };
-    int32_t dx_kb = 1, dw_kb = 1;
-    const int64_t dx_splits = vjp && N ? splits_of(Ng, D, Vc, dx_kb) : 1, dw_splits = DW && N ? splits_of(dwm, dwn, Ng, dw_kb) : 1;
+    const bool dw_v_inner = DW && (DW->stride[ax_v] == 1 || V == 1);
+    const int64_t dw_ld = DW ? DW->stride[dw_v_inner ? ax_d : ax_v] : 0, dx_ld = vjp ? row_stride(O) : 0;
+    Out dxo{}, dwo{};
+    if (vjp && N) dxo = plan(Ng, D, Vc, !rest && pieces == 1 && dx_ld && O.stride[ax_d] == 1);
+    if (DW && N) dwo = plan(dw_v_inner ? D : Vc, dw_v_inner ? Vc : D, Ng, DW->stride[dw_v_inner ? ax_v : ax_d] == 1);
 
     int32_t *label, *ids;
-    float *p, *plogp, *coef, *lse2, *hit, *dxp, *dwp;
+    float *p, *plogp, *coef, *lse2, *hit, *dxp, *dwp, *un_x;
     float2 *part;
-    uint16_t *xc, *wc, *g;
-    uint32_t *words;
+    uint16_t *xl, *xd, *wl, *wd, *g;
+    Scales *scales;
     Slab slab(x);
+    const bool xl_is_xd = vjp && !f32 && !conv; // the copy of x that dw reads serves the logits too
     slab.need(label, distill ? 0 : N);
     slab.need(ids, distill ? N * K : 0);
     slab.need(p, distill ? N * K : 0);
     slab.need(plogp, distill ? N : 0);
     slab.need(coef, vjp ? N : 0);
     slab.need(lse2, vjp ? N : 0);
-    slab.need(part, vjp ? 0 : halves * N);
-    slab.need(hit, vjp ? 0 : distill ? halves * N : N);
-    slab.need(xc, x_direct ? 0 : Ng * Dp * planes);
-    slab.need(wc, w_direct || !N ? 0 : wc_plane * planes);
+    slab.need(part, vjp ? 0 : parts * N);
+    slab.need(hit, vjp ? 0 : distill ? parts * N : N);
+    slab.need(un_x, f32 ? N : 0);
+    slab.need(xl, x_direct || xl_is_xd ? 0 : N * Dp * planes);
+    slab.need(xd, DW || (xl_is_xd && !x_direct) ? Ng * Dp * planes : 0);
+    slab.need(wl, w_direct || !N ? 0 : wc_plane * planes);
+    slab.need(wd, conv ? wc_plane : 0);
     slab.need(g, vjp ? Ng * g_ld * planes : 0);
-    slab.need(dxp, vjp && N ? dx_splits * Ng * dx_ld : 0);
-    slab.need(dwp, DW && N ? dw_splits * dwm * dw_ld : 0);
-    slab.need(words, 3); // the greatest |ct/τ|, binary16's scale and its reciprocal
+    slab.need(dxp, vjp && N && !dxo.straight ? dxo.splits * dxo.m * dxo.ld : 0);
+    slab.need(dwp, DW && N && !dwo.straight ? dwo.splits * dwo.m * dwo.ld : 0);
+    slab.need(scales, any_scale ? 1 : 0);
     if (!slab.take()) return fail(x, PSK_E10001, nm + ": no memory for a workspace of " + std::to_string(slab.total) + " bytes (" + psk_last_error(x.e) + ")");
+    if (any_scale) HEAD_TRY(cudaMemsetAsync(scales, 0, sizeof *scales, x.stream));
 
-    // 1. targets
-    const bool scaled = vjp && f16;
     if (N > 0) {
+        // 1. targets
         RowOperand rct{}, rlse{};
-        if (vjp) { rct = row_operand(*CT, table[first], no); rlse = row_operand(*LSE, table[first + 1], no); }
-        if (scaled) HEAD_TRY(cudaMemsetAsync(words, 0, 4, x.stream));
+        if (vjp) { rct = row_operand(*CT, table[h.ct], no); rlse = row_operand(*LSE, table[h.lse], no); }
         if (distill) {
             TeacherParams T;
             memset(&T, 0, sizeof T);
             T.s = s; T.ids = rids; T.t = row_operand(l->in[3], table[3], no); T.ct = rct; T.lse = rlse;
             T.ids_k = I.stride[ax_k]; T.t_k = l->in[3].stride[ax_k]; T.classes = V; T.top = (int32_t)K; T.inv_tau = inv_tau;
-            T.out_ids = ids; T.out_p = p; T.plogp = plogp; T.coef = coef; T.lse2 = lse2; T.status = x.status; T.ctmax = scaled ? words : nullptr;
+            T.out_ids = ids; T.out_p = p; T.plogp = plogp; T.coef = coef; T.lse2 = lse2; T.status = x.status; T.ctmax = g_scaled ? &scales->max_ct : nullptr;
             k_head_teacher<<<(unsigned)N, (unsigned)up(K, 32), (size_t)K * 4, x.stream>>>(T);
         } else {
             LabelParams T;
             memset(&T, 0, sizeof T);
             T.s = s; T.ids = rids; T.ct = rct; T.lse = rlse; T.classes = V; T.inv_tau = inv_tau;
-            T.label = label; T.coef = coef; T.lse2 = lse2; T.status = x.status; T.ctmax = scaled ? words : nullptr;
+            T.label = label; T.coef = coef; T.lse2 = lse2; T.status = x.status; T.ctmax = g_scaled ? &scales->max_ct : nullptr;
             k_head_labels<<<(unsigned)((N + 255) / 256), 256, 0, x.stream>>>(T);
         }
         x.kernels += 1;
-        if (scaled) { k_head_scale<<<1, 1, 0, x.stream>>>(words, words + 1); x.kernels += 1; }
+        // 2. the powers of two
+        if (any_scale) {
+            const bool of_x = DW && (f32 || conv), of_w = f32 || conv;
+            MaxParams M;
+            if (of_x) {
+                memset(&M, 0, sizeof M);
+                M.s = s; M.src = rx; M.col_stride = X.stride[ax_d]; M.cols = D; M.label = label; M.ids = ids; M.top = (int32_t)K; M.out = &scales->max_x;
+                M.vec = x_ld && M.col_stride == 1 && aligned(rx.p) && x_ld * eb % 16 == 0 && D * eb % 16 == 0;
+                k_head_max<<<warps_of(x, N), 256, 0, x.stream>>>(M);
+                x.kernels += 1;
+            }
+            if (of_w) {
+                memset(&M, 0, sizeof M);
+                M.s.no = 1; M.s.rows = M.s.dims[0] = v_inner ? D : V; M.src.p = wp; M.src.dtype = dt; M.src.stride[0] = v_inner ? w_d : w_v;
+                M.col_stride = v_inner ? w_v : w_d; M.cols = v_inner ? V : D; M.out = &scales->max_w;
+                M.vec = M.col_stride == 1 && aligned(wp) && M.src.stride[0] * eb % 16 == 0 && M.cols * eb % 16 == 0;
+                k_head_max<<<warps_of(x, M.s.rows), 256, 0, x.stream>>>(M);
+                x.kernels += 1;
+            }
+            k_head_scales<<<1, 1, 0, x.stream>>>(scales, (of_x ? 1 : 0) | (of_w ? 2 : 0) | (g_scaled ? 4 : 0));
+            x.kernels += 1;
+        }
     }
-
-    // 2. x where its layout (or a row without a target, backward) asks for a copy
-    Operand a{rx.p, N, D, x_ld, true, planes, 0};
-    if (!x_direct && N > 0) {
-        PackParams k;
-        memset(&k, 0, sizeof k);
-        k.s = s; k.src = rx; k.col_stride = X.stride[ax_d]; k.cols = D; k.ld = Dp; k.plane = Ng * Dp; k.dst = xc; k.f32 = planes == 3; k.copies = (int32_t)(Ng / N);
-        if (vjp) { k.label = label; k.ids = ids; k.top = (int32_t)K; }
-        k_head_pack<<<grid_of(x, N * Dp / 8), 256, 0, x.stream>>>(k);
+    // 3. x for the logits, and (rows without a target zeros) for dw
+    PackParams kx;
+    memset(&kx, 0, sizeof kx);
+    kx.s = s; kx.src = rx; kx.col_stride = X.stride[ax_d]; kx.cols = D; kx.ld = Dp; kx.label = label; kx.ids = ids; kx.top = (int32_t)K; kx.copies = 1;
+    if (xl) {
+        PackParams k = kx;
+        k.dst = xl; k.plane = N * Dp; k.to = f32 ? PACK_SPLIT : PACK_SAME; k.un = un_x;
+        k_head_pack<<<warps_of(x, N), 256, 0, x.stream>>>(k);
         x.kernels += 1;
-        a = Operand{xc, N, D, Dp, true, planes, Ng * Dp};
     }
+    if (xd && N) {
+        PackParams k = kx;
+        k.dst = xd; k.plane = N * Dp; k.to = f32 ? PACK_SPLIT : conv ? PACK_F16 : PACK_SAME; k.copies = (int32_t)(Ng / N);
+        k.scale = f32 || conv ? &scales->x : nullptr;
+        k_head_pack<<<warps_of(x, N), 256, 0, x.stream>>>(k);
+        x.kernels += 1;
+    }
+    const Operand a = x_direct ? Operand{rx.p, N, D, x_ld, true, 1, 0} : Operand{xl ? xl : xd, N, D, Dp, true, planes, N * Dp};
 
-    const RowOperand rout = row_operand(O, table[l->n_inputs], no);
     for (int64_t piece = 0; piece < pieces && N > 0; ++piece) {
         const int64_t v0 = piece * Vc, vn = std::min(Vc, V - v0);
-        // 3. the piece of the head
-        Operand b{wp + v0 * w_v * 2, vn, D, v_inner ? w_d : w_v, !v_inner, planes, 0};
-        if (!w_direct) {
+        // 4. the piece of the head
+        auto pack_w = [&](uint16_t *dst, int to, const float *scale) {
             PackParams k;
             memset(&k, 0, sizeof k);
             k.s.no = 1; k.s.rows = k.s.dims[0] = v_inner ? D : vn;
             k.src.p = wp + v0 * w_v * eb; k.src.dtype = dt; k.src.stride[0] = v_inner ? w_d : w_v;
-            k.col_stride = v_inner ? w_v : w_d; k.cols = v_inner ? vn : D; k.ld = wc_ld; k.plane = wc_plane; k.dst = wc; k.f32 = planes == 3; k.copies = 1;
-            k_head_pack<<<grid_of(x, k.s.rows * wc_ld / 8), 256, 0, x.stream>>>(k);
+            k.col_stride = v_inner ? w_v : w_d; k.cols = v_inner ? vn : D; k.ld = wc_ld; k.plane = wc_plane; k.dst = dst; k.to = to; k.scale = scale; k.copies = 1;
+            k_head_pack<<<warps_of(x, k.s.rows), 256, 0, x.stream>>>(k);
             x.kernels += 1;
-            b = Operand{wc, vn, D, wc_ld, !v_inner, planes, wc_plane};
-        }
-        // 4. the logits' tiles
+            return Operand{dst, vn, D, wc_ld, !v_inner, planes, wc_plane};
+        };
+        const Operand b = w_direct ? Operand{wp + v0 * w_v * 2, vn, D, v_inner ? w_d : w_v, !v_inner, 1, 0} : pack_w(wl, f32 ? PACK_SPLIT : PACK_SAME, f32 ? &scales->w : nullptr);
+        // 5. the logits' tiles
         Params P;
         memset(&P, 0, sizeof P);
+        P.scales = scales; P.logits_scaled = f32; P.un_x = un_x;
         P.c = (float)(1.4426950408889634 / tau); P.rows = N; P.col0 = v0;
         P.label = label; P.ids = ids; P.p = p; P.top = (int32_t)K;
         if (!vjp) {
-            P.part = part; P.hit = hit; P.part0 = 2 * (v0 / BN);
-            const int r = product<MODE_STATS>(x, P, a, b, f16);
+            P.part = part; P.hit = hit; P.part0 = v0 / COLS;
+            const int r = product<MODE_STATS>(x, P, a, b, in_f16);
             if (r != PSK_OK) return r;
             continue;
         }
-        P.lse2 = lse2; P.coef = coef; P.scale = scaled ? words + 1 : nullptr;
-        P.g = g; P.g_ld = g_ld; P.g_plane = g_plane; P.g_lo = Ng > N ? N : 0;
-        int r = product<MODE_GRAD>(x, P, a, b, f16);
+        P.lse2 = lse2; P.coef = coef; P.g = g; P.g_f16 = g_f16; P.g_ld = g_ld; P.g_rest = rest || f32 ? N * g_ld : 0;
+        int r = product<MODE_GRAD>(x, P, a, b, in_f16);
         if (r != PSK_OK) return r;
-        // 5. dx += g·wᵀ over the piece: both operands along the classes
-        Operand gk{g, Ng, vn, g_ld, true, planes, g_plane};
-        Operand wk{b.p, D, vn, b.ld, v_inner, planes, b.plane};
+        // 6. dx = g·wᵀ summed over the pieces: both operands along the classes
+        const Operand bd = conv ? pack_w(wd, PACK_F16, &scales->w) : b;
         Params Q;
         memset(&Q, 0, sizeof Q);
-        Q.splits = dx_splits; Q.kb_split = dx_kb; Q.out = dxp; Q.out_ld = dx_ld; Q.accumulate = piece > 0;
-        if ((vn + BK - 1) / BK < (Vc + BK - 1) / BK) { // the last piece is shorter: as many splits as still have a block
-            Q.splits = ((vn + BK - 1) / BK + dx_kb - 1) / dx_kb;
-        }
-        r = product<MODE_OUT>(x, Q, gk, wk, f16);
+        Q.scales = scales;
+        Q.kb_split = dxo.kb_split;
+        Q.splits = ((vn + BK - 1) / BK + dxo.kb_split - 1) / dxo.kb_split; // a shorter last piece may have fewer
+        Q.out = dxo.straight ? const_cast<void *>(rout.p) : dxp; Q.out_ld = dxo.straight ? dx_ld : dxo.ld; Q.out_dtype = dxo.straight ? dt : PSK_F32;
+        Q.un = dxo.straight ? 1 : 0; Q.accumulate = piece > 0;
+        Q.out_vec = !dxo.straight || (aligned(rout.p) && dx_ld * eb % 16 == 0 && D * eb % 16 == 0);
+        Q.ovf = x.guarded && dxo.straight ? x.ovf : nullptr;
+        const Operand gk{g, Ng, vn, g_ld, true, planes, N * g_ld}, wk{bd.p, D, vn, bd.ld, v_inner, planes, bd.plane};
+        r = dxo.two ? product<MODE_OUT, 2>(x, Q, gk, wk, g_f16) : product<MODE_OUT>(x, Q, gk, wk, g_f16);
         if (r != PSK_OK) return r;
-        // 6. dw of the piece = xᵀ·g: both operands along the rows
+        // 7. dw of the piece = xᵀ·g: both operands along the rows
         if (DW) {
-            Operand xr{xc, D, Ng, Dp, false, planes, Ng * Dp}, gr{g, vn, Ng, g_ld, false, planes, g_plane};
+            uint8_t *dst = (uint8_t *)table[h.dw] + (DW->offset + v0 * DW->stride[ax_v]) * eb;
+            const Operand xr{xd, D, Ng, Dp, false, planes, N * Dp}, gr{g, vn, Ng, g_ld, false, planes, N * g_ld};
+            const int64_t cols = dw_v_inner ? vn : D;
             memset(&Q, 0, sizeof Q);
-            Q.splits = dw_splits; Q.kb_split = dw_kb; Q.out = dwp; Q.out_ld = dw_ld;
-            r = product<MODE_OUT>(x, Q, dw_v_inner ? xr : gr, dw_v_inner ? gr : xr, f16);
+            Q.scales = scales;
+            Q.splits = dwo.splits; Q.kb_split = dwo.kb_split;
+            Q.out = dwo.straight ? (void *)dst : dwp; Q.out_ld = dwo.straight ? dw_ld : dwo.ld; Q.out_dtype = dwo.straight ? dt : PSK_F32;
+            Q.un = dwo.straight ? 2 : 0;
+            Q.out_vec = !dwo.straight || (aligned(dst) && dw_ld * eb % 16 == 0 && cols * eb % 16 == 0);
+            Q.ovf = x.guarded && dwo.straight ? x.ovf : nullptr;
+            r = dwo.two ? product<MODE_OUT, 2>(x, Q, dw_v_inner ? xr : gr, dw_v_inner ? gr : xr, g_f16) : product<MODE_OUT>(x, Q, dw_v_inner ? xr : gr, dw_v_inner ? gr : xr, g_f16);
             if (r != PSK_OK) return r;
-            SumParams S;
-            memset(&S, 0, sizeof S);
-            S.s.no = 1; S.s.rows = S.s.dims[0] = dw_v_inner ? D : vn;
-            S.part = dwp; S.parts = dw_splits; S.part_rows = S.s.rows; S.ld = dw_ld; S.cols = dw_v_inner ? vn : D;
-            S.col_stride = DW->stride[dw_v_inner ? ax_v : ax_d]; S.scale = scaled ? words + 1 : nullptr;
-            S.dst.p = (const uint8_t *)table[first + 2] + (DW->offset + v0 * DW->stride[ax_v]) * eb; S.dst.dtype = dt; S.dst.stride[0] = DW->stride[dw_v_inner ? ax_d : ax_v];
-            S.ovf = x.ovf; S.guarded = x.guarded;
-            k_head_sum<<<grid_of(x, S.s.rows * S.cols), 256, 0, x.stream>>>(S);
-            x.kernels += 1;
+            if (!dwo.straight) {
+                SumParams S;
+                memset(&S, 0, sizeof S);
+                S.s.no = 1; S.s.rows = S.s.dims[0] = dw_v_inner ? D : vn;
+                S.part = dwp; S.parts = dwo.splits; S.part_rows = S.s.rows; S.ld = dwo.ld; S.cols = cols; S.col_stride = DW->stride[dw_v_inner ? ax_v : ax_d];
+                S.scales = scales; S.un = 2; S.dst.p = dst; S.dst.dtype = dt; S.dst.stride[0] = dw_ld; S.ovf = x.ovf; S.guarded = x.guarded;
+                k_head_sum<<<warps_of(x, S.s.rows * ((S.cols + 127) / 128)), 256, 0, x.stream>>>(S);
+                x.kernels += 1;
+            }
         }
     }
     if (!vjp) {
         JoinParams J;
         memset(&J, 0, sizeof J);
-        J.s = s; J.halves = halves; J.part = part; J.hit = hit; J.label = label; J.ids = ids; J.plogp = plogp; J.top = (int32_t)K; J.inv_tau = inv_tau;
+        J.s = s; J.halves = parts; J.part = part; J.hit = hit; J.label = label; J.ids = ids; J.plogp = plogp; J.top = (int32_t)K; J.c = (float)(1.4426950408889634 / tau); J.inv_tau = 1.0 / tau;
         J.loss = rout; J.ovf = x.ovf; J.guarded = x.guarded;
-        if (LSE) J.lse = row_operand(*LSE, table[first], no);
-        k_head_join<<<(unsigned)((N + 31) / 32), 256, 0, x.stream>>>(J);
+        if (LSE) J.lse = row_operand(*LSE, table[h.lse], no);
+        k_head_join<<<(unsigned)((N + 7) / 8), 256, 0, x.stream>>>(J);
         x.kernels += 1;
-    } else if (N > 0) {
+    } else if (N > 0 && !dxo.straight) {
         SumParams S;
         memset(&S, 0, sizeof S);
-        S.s = s; S.part = dxp; S.parts = dx_splits; S.part_rows = Ng; S.ld = dx_ld; S.fold = Ng > N ? N : 0; S.cols = D; S.col_stride = O.stride[ax_d];
-        S.scale = scaled ? words + 1 : nullptr; S.dst = rout; S.ovf = x.ovf; S.guarded = x.guarded;
-        k_head_sum<<<grid_of(x, N * D), 256, 0, x.stream>>>(S);
+        S.s = s; S.part = dxp; S.parts = dxo.splits; S.part_rows = dxo.m; S.ld = dxo.ld; S.fold = rest ? N : 0; S.cols = D; S.col_stride = O.stride[ax_d];
+        S.scales = scales; S.un = 1; S.dst = rout; S.ovf = x.ovf; S.guarded = x.guarded;
+        k_head_sum<<<warps_of(x, N * ((D + 127) / 128)), 256, 0, x.stream>>>(S);
         x.kernels += 1;
-    } else if (DW) { // no rows: a gradient of zeros
+    } else if (N == 0 && DW) { // no rows: a gradient of zeros
         SumParams S;
         memset(&S, 0, sizeof S);
-        S.s.no = 1; S.s.rows = S.s.dims[0] = D; S.cols = V; S.col_stride = DW->stride[ax_v];
-        S.dst.p = (const uint8_t *)table[first + 2] + DW->offset * eb; S.dst.dtype = dt; S.dst.stride[0] = DW->stride[ax_d];
-        k_head_sum<<<grid_of(x, D * V), 256, 0, x.stream>>>(S);
+        S.s.no = 1; S.s.rows = S.s.dims[0] = dw_v_inner ? D : V; S.cols = dw_v_inner ? V : D; S.col_stride = DW->stride[dw_v_inner ? ax_v : ax_d];
+        S.dst.p = (const uint8_t *)table[h.dw] + DW->offset * eb; S.dst.dtype = dt; S.dst.stride[0] = dw_ld;
+        k_head_sum<<<warps_of(x, S.s.rows * ((S.cols + 127) / 128)), 256, 0, x.stream>>>(S);
         x.kernels += 1;
     }
     HEAD_TRY(cudaGetLastError());

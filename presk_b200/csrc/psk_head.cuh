@@ -3,7 +3,7 @@
 //
 // Forward. One pass over the vocabulary: a tile of 128 rows by 256 classes is multiplied on the tensor cores, and its
 // epilogue reduces each row's 128 columns a thread to a maximum m and z = sum of 2^((l - m)·c), c = log2 e / τ, which
-// k_head_join puts together over the tiles: ln sum exp(l / τ) = (M + log2 sum z·2^(m - M)) ln 2 with m in units of c.
+// k_head_join puts together over the tiles: ln sum exp(l / τ) = M / τ + ln sum z·2^((m - M)·c).
 // The targets' logits are picked out of the same registers. Backward. The tile is multiplied again, the epilogue
 // writes g = ct/τ (2^(l·c - lse) - p) of a piece of the vocabulary, and two more products give dx and dw from it.
 //
@@ -11,8 +11,14 @@
 // products comes out 4.4e-6 (products of both signs) to 1.4e-5 (of one sign) too small, always towards zero, where a
 // loss is the difference of two logits. So the accumulator holds `chunk` steps of the summed axis only, and the
 // epilogue's threads add it, rounded to nearest, into registers while the next chunk runs in the other accumulator.
-// f32 operands are three bf16 planes each (x = hi + mid + lo exactly) and six of the nine partial products (those
-// of 2^-16 and up; the three left out are below 2^-24 of the product), one after the other inside a chunk.
+//
+// Types. bf16 and binary16 operands are multiplied as they are. f32 operands are two binary16 planes, hi + lo, 22 bits
+// of the number, of which three partial products are taken (lo·lo is below 2^-22 of the product): half the tensor
+// work of three bf16 planes and their six products, which this was first (333 us at 2044 x 1024 x 16384, against
+// 183 us). Binary16's range is met by powers of two: w is scaled by its greatest |element|, x by a row's, g by the greatest
+// |ct|, each to the top of the range, 2^14 to 2^15, so that what falls below 2^-24 there is 2^-39 of the greatest.
+// g itself is kept in binary16 for f32 and, for many rows, for bf16 operands too, x and w being copied into it (exactly:
+// eight bits into eleven): g in bf16 would cost its 2^-9 an entry, as much again as the result's own rounding.
 #pragma once
 #include "psk_dev.cuh"
 #include "psk_gemm_tc.cuh"
@@ -27,49 +33,67 @@ constexpr int BM = 128, BN = 256, BK = 64;
 constexpr int THREADS = 384;
 constexpr int REGS_FEW = 40, REGS_MANY = 232, REGS_LAUNCH = 168;
 static_assert(128 * REGS_FEW + 256 * REGS_MANY <= THREADS * REGS_LAUNCH, "setmaxnreg waits for registers that the block does not have");
-constexpr int STAGES = 4;
-constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2;
-constexpr int TILE_BYTES = STAGES * (A_BYTES + B_BYTES);
-constexpr int STAGE_OUT = 8 * 32 * 128;
-constexpr int SMEM_TOTAL = TILE_BYTES + 256 + STAGE_OUT + 1024;
+// MT: 128-row halves of a CTA's tile. One, with the two accumulators taking turns, for sums kept in registers; two,
+// both multiplying the same tile of b (a third fewer bytes from the L2 a product), for the plain products dx and dw.
+template <int MT>
+struct Cfg {
+    static constexpr int STAGES = MT == 1 ? 4 : 3;
+    static constexpr int A_BYTES = MT * BM * BK * 2, B_BYTES = BN * BK * 2;
+    static constexpr int TILE_BYTES = STAGES * (A_BYTES + B_BYTES);
+    static constexpr int STAGE_OUT = 8 * 32 * 128;
+    static constexpr int SMEM_TOTAL = TILE_BYTES + 256 + STAGE_OUT + 1024;
+};
 constexpr int COLS = 128; // columns of a tile an epilogue thread holds
 
 enum { MODE_STATS = 0, MODE_GRAD = 1, MODE_OUT = 2 };
 
-// Planes of the partial product q of an f32 contraction: (a, b) = (0,0) (0,1) (1,0) (0,2) (2,0) (1,1).
-PSK_DEV int plane_a(int q) { return (0x120100 >> (4 * q)) & 15; }
-PSK_DEV int plane_b(int q) { return (0x102010 >> (4 * q)) & 15; }
+// Planes of the partial product q of two operands of two planes: hi·hi, hi·lo, lo·hi.
+PSK_DEV int plane_a(int q) { return q == 2; }
+PSK_DEV int plane_b(int q) { return q == 1; }
+
+// Powers of two that the operands are scaled by, in device memory: what k_head_scales makes of the maxima.
+struct Scales {
+    uint32_t max_x, max_w, max_ct; // bits of the greatest finite |element|
+    float x, w, g;                 // what they are multiplied by
+    float un_w, un_dx, un_dw;      // 1/w; 1/(g·w); 1/(g·x)
+};
 
 struct Params {
     int64_t m, n;                 // rows and columns of the product
     int64_t tiles_m, tiles_n, splits, panel;
-    int32_t kb_k, nprod;          // blocks of 64 along the summed axis; partial products a block (1, or 6 for f32 planes)
+    int32_t kb_k, nprod;          // blocks of 64 along the summed axis; partial products a block (1, or 3 of two planes)
     int32_t kb_split;             // blocks of the summed axis a split
     int32_t chunk;                // steps (block, partial product) in one accumulator before it is added into registers
     int32_t in_f16, a_m_major, b_n_major;
     uint32_t *status;
+    const Scales *scales;         // or null: every factor 1
+    int32_t logits_scaled;        // the operands of the logits are
     // MODE_STATS, MODE_GRAD
     float c;                      // log2 e / τ
-    int64_t rows;                 // rows with a target list (m may be larger: rows of zeros)
+    const float *un_x;            // a row's factor that undoes its scale; or null
+    int64_t rows;                 // rows with a target list
     int64_t col0;                 // the class of column 0: where the piece begins
     const int32_t *label;         // one class a row, or -1; or null, and then
     const int32_t *ids;           // rows x top classes in ascending order, absent entries last as 0x7fffffff
     const float *p;               // their weights
     int32_t top;
     // MODE_STATS
-    float2 *part;                 // [2·tile column][row]: (max·c, sum of 2^(l·c - max·c))
-    float *hit;                   // label: [row], the label's logit; list: [2·tile column][row], sum of p·l
-    int64_t part0;                // index of the piece's first half-tile column
+    float2 *part;                 // [128-column part][row]: (max, sum of 2^((l - max)·c))
+    float *hit;                   // label: [row], the label's logit; list: [part][row], sum of p·l
+    int64_t part0;                // index of the piece's first part
     // MODE_GRAD
     const float *lse2, *coef;     // a row's log-sum-exp in base 2, and ct/τ (0 where it has no target)
-    const uint32_t *scale;        // binary16: the exponent (biased, see k_head_scale) g is multiplied up by; or null
     uint16_t *g;
-    int64_t g_ld, g_plane;        // row stride; distance of the planes of an f32 operand's g (0: one plane)
-    int64_t g_lo;                 // rows further down where g - (g as stored) goes too (0: nowhere)
+    int32_t g_f16;                // g in binary16, times scales->g where there are scales; else bf16
+    int64_t g_ld, g_rest;         // row stride; how much further on what the rounding leaves is kept (0: nowhere)
     // MODE_OUT
-    float *out;                   // [split][m][out_ld]
+    void *out;                    // [split][m][out_ld]
     int64_t out_ld;
-    int32_t accumulate;           // add to what is there (a later piece of the summed axis)
+    int32_t out_dtype;            // f32, bf16 or binary16 (one split then)
+    int32_t out_vec;              // whole 16-byte units: aligned rows, n a multiple of a unit
+    int32_t accumulate;           // f32: add to what is there (a later piece of the summed axis)
+    int32_t un;                   // times scales->un_dx (1), scales->un_dw (2)
+    uint32_t *ovf;                // the overflow guard's flag; or null
 };
 
 PSK_DEV float ex2(float x)
@@ -95,9 +119,9 @@ PSK_DEV int lower_bound(const int32_t *ids, int n, int32_t c)
 
 // 128 bytes of each of this warp's 32 rows: from the threads' packed words through a staging tile (16-byte units
 // swizzled by the row), so that a store instruction writes whole lines (8 lanes a row, 4 rows an instruction).
-// `units`: how many of the 8 units of 16 bytes lie inside the matrix.
+// `bytes`: how many of the 128 lie inside the matrix, a multiple of 16.
 template <bool ADD>
-PSK_DEV void store_rows(uint4 *stage, int lane, const uint32_t (&w)[32], uint8_t *base, int64_t ld_bytes, int rows_live, int units)
+PSK_DEV void store_rows(uint4 *stage, int lane, const uint32_t (&w)[32], uint8_t *base, int64_t ld_bytes, int rows_live, int bytes)
 {
 #pragma unroll
     for (int q = 0; q < 8; ++q) stage[lane * 8 + (q ^ (lane & 7))] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
@@ -106,7 +130,7 @@ PSK_DEV void store_rows(uint4 *stage, int lane, const uint32_t (&w)[32], uint8_t
 #pragma unroll
     for (int it = 0; it < 8; ++it) {
         const int rr = it * 4 + (lane >> 3);
-        if (rr < rows_live && unit < units) {
+        if (rr < rows_live && unit * 16 < bytes) {
             uint4 v = stage[rr * 8 + (unit ^ (rr & 7))];
             uint4 *dst = reinterpret_cast<uint4 *>(base + rr * ld_bytes + unit * 16);
             if (ADD) {
@@ -120,11 +144,32 @@ PSK_DEV void store_rows(uint4 *stage, int lane, const uint32_t (&w)[32], uint8_t
     __syncwarp();
 }
 
+// The same where rows begin at any element: the lanes write neighbouring elements (T: 16 or 32 bits) of one row.
+template <class T>
+PSK_DEV void store_rows_any(uint4 *stage, int lane, const uint32_t (&w)[32], uint8_t *base, int64_t ld_bytes, int rows_live, int bytes)
+{
+#pragma unroll
+    for (int q = 0; q < 8; ++q) stage[lane * 8 + (q ^ (lane & 7))] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+    __syncwarp();
+    constexpr int PER = 16 / sizeof(T);
+#pragma unroll 4
+    for (int rr = 0; rr < rows_live; ++rr) {
+        T *dst = reinterpret_cast<T *>(base + rr * ld_bytes);
+        const T *src = reinterpret_cast<const T *>(stage + rr * 8);
+#pragma unroll
+        for (int e = lane; e < 128 / (int)sizeof(T); e += 32)
+            if (e * (int)sizeof(T) < bytes) dst[e] = src[((e / PER) ^ (rr & 7)) * PER + e % PER];
+    }
+    __syncwarp();
+}
+
 // The product of a persistent CTA's tiles, and what MODE makes of it. Bounds: the tensor pipe (2·m·n·k flops) for many
 // rows; for few, the bytes of the second operand.
-template <int MODE>
+template <int MODE, int MT = 1>
 __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ Params P)
 {
+    static_assert(MT == 1 || MODE == MODE_OUT, "two halves leave no second accumulator to sum in parts with");
+    constexpr int STAGES = Cfg<MT>::STAGES, A_BYTES = Cfg<MT>::A_BYTES, B_BYTES = Cfg<MT>::B_BYTES, TILE_BYTES = Cfg<MT>::TILE_BYTES;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint8_t *smem_a = smem, *smem_b = smem + STAGES * A_BYTES;
@@ -167,7 +212,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ CUt
             for (int64_t t = blockIdx.x; t < total && ok; t += gridDim.x) {
                 int64_t mt, nt;
                 tc::tile_of(t % per_split, P.tiles_m, P.tiles_n, P.panel, mt, nt);
-                const int m0 = (int)mt * BM, n0 = (int)nt * BN;
+                const int m0 = (int)mt * BM * MT, n0 = (int)nt * BN;
                 int kb0;
                 const int steps = steps_of(t / per_split, kb0);
                 int kb = kb0, q = 0;
@@ -181,7 +226,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ CUt
                     if (!P.a_m_major) tc::tma_load_4d(sa, &map_a, fb, k0, m0, pa, 0);
                     else
 #pragma unroll
-                        for (int c = 0; c < BM / 64; ++c) tc::tma_load_4d(sa + c * 8192, &map_a, fb, m0 + c * 64, k0, pa, 0);
+                        for (int c = 0; c < BM * MT / 64; ++c) tc::tma_load_4d(sa + c * 8192, &map_a, fb, m0 + c * 64, k0, pa, 0);
                     if (!P.b_n_major) tc::tma_load_4d(sb, &map_b, fb, k0, n0, pb, 0);
                     else
 #pragma unroll
@@ -200,7 +245,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ CUt
                 const int steps = steps_of(t / per_split, kb0);
                 int in_chunk = 0;
                 for (int s = 0; s < steps; ++s) {
-                    if (in_chunk == 0) {
+                    if (MT == 1 && in_chunk == 0) {
                         ok = tc::mbar_wait(tempty0 + 8 * acc, acc_phase ^ 1u, abort_flag, P.status, 2u);
                         if (!ok) break;
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -210,19 +255,30 @@ __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ CUt
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint32_t sa = tc::smem_u32(smem_a + stage * A_BYTES), sb = tc::smem_u32(smem_b + stage * B_BYTES);
 #pragma unroll
-                    for (int k = 0; k < BK / tc::UMMA_K; ++k) {
-                        const uint64_t ad = P.a_m_major ? tc::smem_desc(sa + k * 2048, 8192, 1024) : tc::smem_desc(sa + k * 32, 16, 1024);
-                        const uint64_t bd = P.b_n_major ? tc::smem_desc(sb + k * 2048, 8192, 1024) : tc::smem_desc(sb + k * 32, 16, 1024);
-                        tc::umma(tmem_base + acc * BN, ad, bd, idesc, (in_chunk | k) != 0 ? 1u : 0u);
+                    for (int h = 0; h < MT; ++h) {
+                        if (MT == 2 && s == 0) { // this half's accumulator has to be read out by the tile before
+                            ok = tc::mbar_wait(tempty0 + 8 * h, acc_phase ^ 1u, abort_flag, P.status, 2u);
+                            if (!ok) break;
+                            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        }
+#pragma unroll
+                        for (int k = 0; k < BK / tc::UMMA_K; ++k) {
+                            const uint64_t ad = P.a_m_major ? tc::smem_desc(sa + h * (BM * BK * 2) + k * 2048, 8192, 1024) : tc::smem_desc(sa + h * (BM * BK * 2) + k * 32, 16, 1024);
+                            const uint64_t bd = P.b_n_major ? tc::smem_desc(sb + k * 2048, 8192, 1024) : tc::smem_desc(sb + k * 32, 16, 1024);
+                            tc::umma(tmem_base + (MT == 1 ? acc : (uint32_t)h) * BN, ad, bd, idesc, (in_chunk | k) != 0 ? 1u : 0u);
+                        }
                     }
+                    if (!ok) break;
                     tc::umma_commit(empty0 + 8 * stage);
                     if (++stage == STAGES) { stage = 0; phase ^= 1u; }
-                    if (++in_chunk == P.chunk || s + 1 == steps) {
+                    ++in_chunk;
+                    if (MT == 1 && (in_chunk == P.chunk || s + 1 == steps)) {
                         tc::umma_commit(tfull0 + 8 * acc);
                         in_chunk = 0;
                         if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
                     }
                 }
+                if (MT == 2 && ok) { tc::umma_commit(tfull0); acc_phase ^= 1u; }
             }
         }
     } else {
@@ -234,16 +290,21 @@ __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ CUt
         for (int64_t t = blockIdx.x; t < total && ok; t += gridDim.x) {
             int64_t mt, nt;
             tc::tile_of(t % per_split, P.tiles_m, P.tiles_n, P.panel, mt, nt);
-            const int64_t sp = t / per_split, row0 = mt * BM + quad * 32, row = row0 + lane, cbase = nt * BN + half * COLS;
+            const int64_t sp = t / per_split, cbase = nt * BN + half * COLS;
             int kb0;
-            const int steps = steps_of(sp, kb0), chunks = (steps + P.chunk - 1) / P.chunk;
+            const int steps = steps_of(sp, kb0), chunks = MT == 1 ? (steps + P.chunk - 1) / P.chunk : 1;
+#pragma unroll 1
+            for (int mh = 0; mh < MT && ok; ++mh) {
+            const int64_t row0 = (mt * MT + mh) * BM + quad * 32, row = row0 + lane;
             float v[COLS];
             for (int ch = 0; ch < chunks; ++ch) {
-                ok = tc::mbar_wait(tfull0 + 8 * acc, acc_phase, abort_flag, P.status, 4u);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
+                if (MT == 1 || mh == 0) {
+                    ok = tc::mbar_wait(MT == 1 ? tfull0 + 8 * acc : tfull0, acc_phase, abort_flag, P.status, 4u);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t ta = tmem_base + ((uint32_t)(quad * 32) << 16) + acc * BN + half * COLS;
+                const uint32_t ta = tmem_base + ((uint32_t)(quad * 32) << 16) + (MT == 1 ? acc : (uint32_t)mh) * BN + half * COLS;
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
                     uint32_t r[32];
@@ -259,12 +320,12 @@ __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ CUt
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) tc::mbar_arrive(tempty0 + 8 * acc);
-                if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+                if (lane == 0) tc::mbar_arrive(tempty0 + 8 * (MT == 1 ? acc : (uint32_t)mh));
+                if (MT == 1 && ++acc == 2) { acc = 0; acc_phase ^= 1u; }
             }
             if (!ok) break;
             const int rows_live = P.m - row0 < 32 ? (int)(P.m - row0) : 32;
-            if (rows_live <= 0 || cbase >= P.n) continue; // the whole warp
+            if (rows_live <= 0 || cbase >= P.n) continue; // the whole warp: the next half, or the next tile
             const int live = P.n - cbase < COLS ? (int)(P.n - cbase) : COLS; // columns inside the matrix
             if constexpr (MODE == MODE_STATS || MODE == MODE_GRAD) {
                 if (live < COLS) {
@@ -275,12 +336,16 @@ __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ CUt
             }
             const int32_t first = (int32_t)(P.col0 + cbase); // the class of v[0]
             const bool own = row < P.rows;
+            // what undoes the operands' scales: a power of two a row
+            const float un = MODE == MODE_OUT || !P.logits_scaled ? 1.0f : __fmul_rn(P.scales->un_w, own && P.un_x ? P.un_x[row] : 1.0f);
+            const float c = MODE == MODE_OUT ? 0.0f : __fmul_rn(P.c, un);
             if constexpr (MODE == MODE_STATS) {
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                 for (int i = 0; i < COLS; ++i) mx[i & 3] = fmaxf(mx[i & 3], v[i]);
                 const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                const float mc = __fmul_rn(m, P.c), shift = m == -INFINITY ? 0.0f : mc;
+                // (one rounded product m·c instead of the differences would be an instruction less, and wrong by 2^-24 of m·c)
+                const float shift = m == -INFINITY ? 0.0f : m;
                 float hit = 0.0f;
                 const int64_t th = P.part0 + 2 * nt + half;
                 if (own) {
@@ -290,7 +355,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ CUt
 #pragma unroll
                             for (int i = 0; i < COLS; ++i)
                                 if (i == y) hit = v[i];
-                            P.hit[row] = hit;
+                            P.hit[row] = __fmul_rn(hit, un);
                         }
                     } else {
                         const int32_t *ids = P.ids + row * P.top;
@@ -304,20 +369,20 @@ __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ CUt
                                 if (i == y) l = v[i];
                             hit = __fmaf_rn(p[j], l, hit);
                         }
-                        P.hit[th * P.rows + row] = hit;
+                        P.hit[th * P.rows + row] = __fmul_rn(hit, un);
                     }
                 }
                 float z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int i = 0; i < COLS; ++i) z[i & 3] = __fadd_rn(z[i & 3], ex2(__fmaf_rn(v[i], P.c, -shift)));
-                if (own) P.part[th * P.rows + row] = make_float2(mc, __fadd_rn(__fadd_rn(z[0], z[1]), __fadd_rn(z[2], z[3])));
+                for (int i = 0; i < COLS; ++i) z[i & 3] = __fadd_rn(z[i & 3], ex2(__fmul_rn(__fsub_rn(v[i], shift), c)));
+                if (own) P.part[th * P.rows + row] = make_float2(__fmul_rn(m, un), __fadd_rn(__fadd_rn(z[0], z[1]), __fadd_rn(z[2], z[3])));
             } else if constexpr (MODE == MODE_GRAD) {
                 const float lse2 = own ? P.lse2[row] : 0.0f;
                 float coef = own ? P.coef[row] : 0.0f;
                 const bool none = !own || (P.label ? P.label[row] < 0 : P.ids[row * P.top] == 0x7fffffff); // no target: zeros, whatever the row holds
-                if (P.scale) coef = __fmul_rn(coef, __uint_as_float(*P.scale));
+                if (P.scales && P.g_f16) coef = __fmul_rn(coef, P.scales->g);
 #pragma unroll
-                for (int i = 0; i < COLS; ++i) v[i] = ex2(__fmaf_rn(v[i], P.c, -lse2));
+                for (int i = 0; i < COLS; ++i) v[i] = ex2(__fmaf_rn(v[i], c, -lse2));
                 if (!none) {
                     if (P.label) {
                         const int32_t y = P.label[row] - first;
@@ -341,46 +406,64 @@ __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ CUt
                 }
 #pragma unroll
                 for (int i = 0; i < COLS; ++i) v[i] = none ? 0.0f : __fmul_rn(v[i], coef);
-                // Rounded to the operand's type for the two products that read it (2^-9 an entry on average, of terms
-                // of both signs). Where the rest of a rounding is kept too (few rows; the planes of f32), it is the
-                // exact remainder rounded again.
+                // Rounded for the two products that read it; where the rest of a rounding is kept too (bf16 with few
+                // rows, f32), it is the exact remainder rounded again.
                 uint8_t *base = (uint8_t *)(P.g + row0 * P.g_ld + cbase);
-                const int planes = P.g_plane ? 3 : P.g_lo ? 2 : 1;
-                const int64_t step = (P.g_plane ? P.g_plane : P.g_lo * P.g_ld) * 2;
+                const int planes = P.g_rest ? 2 : 1;
+#pragma unroll 1
                 for (int pl = 0; pl < planes; ++pl) {
 #pragma unroll
                     for (int g = 0; g < 2; ++g) {
                         uint32_t w[32];
 #pragma unroll
                         for (int i = 0; i < 32; ++i) {
-                            float a = v[g * 64 + 2 * i], b = v[g * 64 + 2 * i + 1];
-                            w[i] = P.in_f16 ? pack_f16x2_hw(a, b) : pack_bf16x2_hw(a, b);
-                            if (planes > 1) {
-                                if (P.in_f16) {
-                                    v[g * 64 + 2 * i] = __fsub_rn(a, f16_to_f32((uint16_t)(w[i] & 0xffffu)));
-                                    v[g * 64 + 2 * i + 1] = __fsub_rn(b, f16_to_f32((uint16_t)(w[i] >> 16)));
-                                } else {
-                                    v[g * 64 + 2 * i] = __fsub_rn(a, bf16_up(w[i] & 0xffffu));
-                                    v[g * 64 + 2 * i + 1] = __fsub_rn(b, bf16_up(w[i] >> 16));
-                                }
-                            }
+                            const float a = v[g * 64 + 2 * i], b = v[g * 64 + 2 * i + 1];
+                            w[i] = P.g_f16 ? pack_f16x2_hw(a, b) : pack_bf16x2_hw(a, b);
+                            v[g * 64 + 2 * i] = __fsub_rn(a, P.g_f16 ? f16_to_f32((uint16_t)(w[i] & 0xffffu)) : bf16_up(w[i] & 0xffffu));
+                            v[g * 64 + 2 * i + 1] = __fsub_rn(b, P.g_f16 ? f16_to_f32((uint16_t)(w[i] >> 16)) : bf16_up(w[i] >> 16));
                         }
-                        const int64_t left = (P.g_ld - cbase - g * 64) / 8; // the rows are padded to whole lines, the padding zeros
-                        store_rows<false>(stage_out, lane, w, base + g * 128 + pl * step, P.g_ld * 2, rows_live, left < 8 ? (int)left : 8);
+                        // the rows are padded to whole lines, the padding zeros
+                        const int64_t left = (P.g_ld - cbase - g * 64) * 2;
+                        store_rows<false>(stage_out, lane, w, base + g * 128 + pl * P.g_rest * 2, P.g_ld * 2, rows_live, left < 128 ? (int)left : 128);
                     }
                 }
             } else {
-                float *base = P.out + sp * P.m * P.out_ld + row0 * P.out_ld + cbase;
+                const float f = !P.scales ? 1.0f : P.un == 1 ? P.scales->un_dx : P.un == 2 ? P.scales->un_dw : 1.0f;
+                if (P.out_dtype == PSK_F32) {
+                    uint8_t *base = (uint8_t *)((float *)P.out + (sp * P.m + row0) * P.out_ld + cbase);
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    uint32_t w[32];
+                    for (int g = 0; g < 4; ++g) {
+                        uint32_t w[32];
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(v[g * 32 + i]);
-                    const int64_t left = ((P.n + 3) / 4 * 4 - cbase - g * 32) / 4;
-                    if (P.accumulate) store_rows<true>(stage_out, lane, w, (uint8_t *)(base + g * 32), P.out_ld * 4, rows_live, left < 8 ? (int)left : 8);
-                    else store_rows<false>(stage_out, lane, w, (uint8_t *)(base + g * 32), P.out_ld * 4, rows_live, left < 8 ? (int)left : 8);
+                        for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(__fmul_rn(v[g * 32 + i], f));
+                        const int64_t left = (P.n - cbase - g * 32) * 4;
+                        const int bytes = left < 128 ? (int)(P.out_vec ? (left + 15) / 16 * 16 : left) : 128; // vec: n a multiple of 4, or rows padded to one
+                        if (P.accumulate) store_rows<true>(stage_out, lane, w, base + g * 128, P.out_ld * 4, rows_live, bytes);
+                        else if (P.out_vec) store_rows<false>(stage_out, lane, w, base + g * 128, P.out_ld * 4, rows_live, bytes);
+                        else store_rows_any<uint32_t>(stage_out, lane, w, base + g * 128, P.out_ld * 4, rows_live, bytes);
+                    }
+                } else {
+                    uint8_t *base = (uint8_t *)((uint16_t *)P.out + row0 * P.out_ld + cbase);
+                    uint32_t over = 0;
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+                        uint32_t w[32];
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            const float a = __fmul_rn(v[g * 64 + 2 * i], f), b = __fmul_rn(v[g * 64 + 2 * i + 1], f);
+                            if (P.out_dtype == PSK_F16) { over |= overflows(a, kF16Overflow) | overflows(b, kF16Overflow); w[i] = pack_f16x2_hw(a, b); }
+                            else w[i] = pack_bf16x2_hw(a, b);
+                        }
+                        const int64_t left = (P.n - cbase - g * 64) * 2;
+                        const int bytes = left < 128 ? (int)left : 128;
+                        if (P.out_vec) store_rows<false>(stage_out, lane, w, base + g * 128, P.out_ld * 2, rows_live, bytes);
+                        else store_rows_any<uint16_t>(stage_out, lane, w, base + g * 128, P.out_ld * 2, rows_live, bytes);
+                    }
+                    if (P.ovf && over) atomicOr(P.ovf, 1u);
                 }
             }
+            } // mh
+            if (MT == 2) acc_phase ^= 1u;
         }
     }
 
@@ -521,29 +604,92 @@ static __global__ void __launch_bounds__(1024) k_head_teacher(const __grid_const
     }
 }
 
-// The scale of binary16 g: the power of two that brings the largest |ct/τ| into [2^14, 2^15), written as an f32's
-// bits (and its reciprocal). A gradient spread over a vocabulary is far below binary16's least number otherwise; g
-// itself is at most that maximum, so nothing overflows.
-static __global__ void k_head_scale(const uint32_t *ctmax, uint32_t *scale)
+// The greatest finite |element| of a matrix, as f32 bits (non-negative floats order as their bits do, so the blocks'
+// order changes nothing): rows of `cols` elements `col_stride` apart; rows without a target are passed over.
+struct MaxParams {
+    RowSpace s;
+    RowOperand src;
+    int64_t col_stride, cols;
+    const int32_t *label, *ids;
+    int32_t top, vec; // vec: 16 bytes a load (contiguous, aligned, cols a multiple of a unit)
+    uint32_t *out;
+};
+
+PSK_DEV bool no_target(const int32_t *label, const int32_t *ids, int top, int64_t row) { return label ? label[row] < 0 : ids ? ids[row * top] == 0x7fffffff : false; }
+
+PSK_DEV uint32_t finite_bits(float x)
 {
-    const int e = (int)(*ctmax >> 23); // biased exponent of the maximum; 0 for zero and subnormals
-    int up = 14 + 127 - e;             // 2^up
-    if (e == 0 || up > 120) up = e == 0 ? 0 : 120;
-    if (up < -120) up = -120;
-    scale[0] = (uint32_t)(127 + up) << 23;
-    scale[1] = (uint32_t)(127 - up) << 23;
+    const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
+    return b < 0x7f800000u ? b : 0u;
+}
+
+static __global__ void __launch_bounds__(256) k_head_max(const __grid_constant__ MaxParams P)
+{
+    __shared__ uint32_t red[8];
+    const int lane = threadIdx.x & 31;
+    const int64_t warps = (int64_t)gridDim.x * 8;
+    uint32_t m = 0;
+    for (int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < P.s.rows; row += warps) {
+        if (no_target(P.label, P.ids, P.top, row)) continue;
+        const int64_t off = row_offset(P.s, P.src.stride, row);
+        if (P.vec) {
+            const uint4 *q = reinterpret_cast<const uint4 *>((const uint8_t *)P.src.p + off * (P.src.dtype == PSK_F32 ? 4 : 2));
+            const int64_t n = P.cols * (P.src.dtype == PSK_F32 ? 4 : 2) / 16;
+#pragma unroll 4
+            for (int64_t i = lane; i < n; i += 32) {
+                const uint4 u = q[i];
+                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    if (P.src.dtype == PSK_F32) m = max(m, finite_bits(__uint_as_float(w[k])));
+                    else m = max(m, max(finite_bits(bf16_up(w[k] & 0xffffu)), finite_bits(bf16_up(w[k] >> 16)))); // bf16: the only 16-bit type that is scaled
+                }
+            }
+        } else
+#pragma unroll 4
+            for (int64_t c = lane; c < P.cols; c += 32) m = max(m, finite_bits(load_real(P.src.p, P.src.dtype, off + c * P.col_stride)));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (lane == 0) red[threadIdx.x >> 5] = m;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 8; ++w) m = max(m, red[w]);
+        if (m) atomicMax(P.out, m);
+    }
+}
+
+// 2^e as an f32, e within its normal range.
+PSK_DEV float pow2(int e) { return __uint_as_float((uint32_t)(127 + (e < -126 ? -126 : e > 127 ? 127 : e)) << 23); }
+
+// The exponent of the power of two that brings a maximum into [2^14, 2^15); 0 for none.
+PSK_DEV int scale_of(uint32_t max_bits)
+{
+    const int e = (int)(max_bits >> 23);
+    if (max_bits == 0) return 0;
+    const int k = 14 + 127 - (e == 0 ? 1 : e);
+    return k > 60 ? 60 : k; // 1/(g·w) and 1/(g·x) are f32 numbers then
+}
+
+// `has`: bit 0 x, bit 1 w, bit 2 g.
+static __global__ void k_head_scales(Scales *s, int has)
+{
+    const int x = has & 1 ? scale_of(s->max_x) : 0, w = has & 2 ? scale_of(s->max_w) : 0, g = has & 4 ? scale_of(s->max_ct) : 0;
+    s->x = pow2(x); s->w = pow2(w); s->g = pow2(g);
+    s->un_w = pow2(-w); s->un_dx = pow2(-g - w); s->un_dw = pow2(-g - x);
 }
 
 // The tiles' (m, z) of a row put together, and its loss. 32 rows a block, the half-tile columns over the block's y.
 struct JoinParams {
     RowSpace s;
-    int64_t halves; // half-tile columns
+    int64_t halves; // parts of 128 columns
     const float2 *part;
     const float *hit;
     const int32_t *label, *ids;
     const float *plogp;
     int32_t top;
-    float inv_tau;
+    float c;      // log2 e / τ
+    double inv_tau;
     RowOperand loss, lse; // lse.p may be null
     uint32_t *ovf;
     int32_t guarded;
@@ -551,91 +697,129 @@ struct JoinParams {
 
 static __global__ void __launch_bounds__(256) k_head_join(const __grid_constant__ JoinParams P)
 {
-    __shared__ float sm[8][33], sz[8][33], sh[8][33];
-    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
-    const int64_t row = (int64_t)blockIdx.x * 32 + x;
+    // a row's parts over 32 threads: four lanes of each of the eight warps; eight neighbouring rows a warp's load
+    __shared__ float sm[8][8], sz[8][8], sh[8][8];
+    const int x = threadIdx.x & 7, y = threadIdx.x >> 3, warp = threadIdx.x >> 5;
+    const int64_t row = (int64_t)blockIdx.x * 8 + x;
     float m = -INFINITY, z = 0.0f, h = 0.0f;
-    if (row < P.s.rows)
-        for (int64_t th = y; th < P.halves; th += 8) {
-            const float2 a = P.part[th * P.s.rows + row];
-            if (!P.label) h = __fadd_rn(h, P.hit[th * P.s.rows + row]);
-            // (m, z) + (a.x, a.y) about the greater of the two; an empty part has m = -inf and z = 0
-            const float g = fmaxf(m, a.x);
-            if (!(g == -INFINITY)) z = __fadd_rn(__fmul_rn(z, exp2f(__fsub_rn(m, g))), __fmul_rn(a.y, exp2f(__fsub_rn(a.x, g))));
-            m = g;
-        }
-    sm[y][x] = m; sz[y][x] = z; sh[y][x] = h;
-    __syncthreads();
-    if (y != 0 || row >= P.s.rows) return;
-    for (int i = 1; i < 8; ++i) {
-        const float am = sm[i][x], g = fmaxf(m, am);
-        if (!(g == -INFINITY)) z = __fadd_rn(__fmul_rn(z, exp2f(__fsub_rn(m, g))), __fmul_rn(sz[i][x], exp2f(__fsub_rn(am, g))));
+    // (m, z) + (am, az) about the greater maximum; an empty part has m = -inf and z = 0
+    auto join = [&](float am, float az) {
+        const float g = fmaxf(m, am);
+        if (!(g == -INFINITY)) z = __fadd_rn(__fmul_rn(z, exp2f(__fmul_rn(__fsub_rn(m, g), P.c))), __fmul_rn(az, exp2f(__fmul_rn(__fsub_rn(am, g), P.c))));
         m = g;
+    };
+    if (row < P.s.rows)
+        for (int64_t th = y; th < P.halves; th += 32 * 8) {
+            float2 a[8];
+            float b[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const bool in = th + 32 * k < P.halves;
+                const int64_t at = (th + 32 * k) * P.s.rows + row;
+                a[k] = in ? P.part[at] : make_float2(-INFINITY, 0.0f);
+                b[k] = in && !P.label ? P.hit[at] : 0.0f;
+            }
+            float g = a[0].x;
+#pragma unroll
+            for (int k = 1; k < 8; ++k) g = fmaxf(g, a[k].x);
+            float s = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                if (!(g == -INFINITY)) s = __fadd_rn(s, __fmul_rn(a[k].y, exp2f(__fmul_rn(__fsub_rn(a[k].x, g), P.c))));
+                h = __fadd_rn(h, b[k]);
+            }
+            join(g, s);
+        }
+#pragma unroll
+    for (int o = 8; o <= 16; o <<= 1) {
+        const float am = __shfl_xor_sync(0xffffffffu, m, o), az = __shfl_xor_sync(0xffffffffu, z, o);
+        h = __fadd_rn(h, __shfl_xor_sync(0xffffffffu, h, o));
+        join(am, az);
+    }
+    if ((threadIdx.x & 31) < 8) { sm[warp][x] = m; sz[warp][x] = z; sh[warp][x] = h; }
+    __syncthreads();
+    if (threadIdx.x >= 8 || row >= P.s.rows) return;
+    for (int i = 1; i < 8; ++i) {
+        join(sm[i][x], sz[i][x]);
         h = __fadd_rn(h, sh[i][x]);
     }
-    const bool none = P.label ? P.label[row] < 0 : P.ids[row * P.top] == 0x7fffffff;
-    const double lse = ((double)m + log2((double)z)) * 0.6931471805599453;
+    const bool none = no_target(P.label, P.ids, P.top, row);
+    const double lse = (double)m * P.inv_tau + log((double)z);
     double loss;
     if (P.label) loss = lse - (double)P.hit[row];
-    else loss = (double)P.plogp[row] - (double)h * (double)P.inv_tau + lse;
-    uint32_t ovf = store_real(const_cast<void *>(P.loss.p), P.loss.dtype, row_offset(P.s, P.loss.stride, row), none ? 0.0f : (float)loss);
+    else loss = (double)P.plogp[row] - (double)h * P.inv_tau + lse;
+    const uint32_t ovf = store_real(const_cast<void *>(P.loss.p), P.loss.dtype, row_offset(P.s, P.loss.stride, row), none ? 0.0f : (float)loss);
     if (P.lse.p) store_real(const_cast<void *>(P.lse.p), P.lse.dtype, row_offset(P.s, P.lse.stride, row), none ? 0.0f : (float)lse);
     if (P.guarded && ovf) atomicOr(P.ovf, 1u);
 }
 
 // A matrix laid out for the tensor maps: rows of `cols` elements from any strides into rows of `ld` (a multiple of 8),
-// the padding zeros; f32 as three bf16 planes one after the other. Rows without a target (of x, backward) become
-// zeros, so that nothing they hold reaches dw. `copies`: the rows again below themselves (the second operand of a
-// product over g and its remainder).
+// the padding zeros, a warp a row and neighbouring lanes neighbouring elements (both sides whole lines whatever the
+// source's alignment). `to`: the same 16 bits; binary16 of bf16, scaled (exact); two binary16 planes of f32, scaled.
+// Rows without a target (of x) become zeros, so that nothing they hold reaches dw. `copies`: the rows again below
+// themselves (the second operand of a product over g and its remainder).
+enum { PACK_SAME = 0, PACK_F16 = 1, PACK_SPLIT = 2 };
+
 struct PackParams {
-    RowSpace s;       // the rows (for w: one axis)
+    RowSpace s; // the rows (for w: one axis)
     RowOperand src;
     int64_t col_stride, cols, ld, plane;
     uint16_t *dst;
-    int32_t f32, copies;
+    int32_t to, copies;
+    const float *scale; // of the whole matrix; or null
+    float *un;          // PACK_SPLIT: scale every row by its own greatest element instead, and put the factor that undoes it here
     const int32_t *label, *ids;
     int32_t top;
 };
 
 static __global__ void __launch_bounds__(256) k_head_pack(const __grid_constant__ PackParams P)
 {
-    const int64_t vecs = P.ld / 8, total = P.s.rows * vecs, step = (int64_t)gridDim.x * blockDim.x;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += step) {
-        const int64_t row = i / vecs, c0 = (i - row * vecs) * 8;
-        bool none = false;
-        if (P.label) none = P.label[row] < 0;
-        else if (P.ids) none = P.ids[row * P.top] == 0x7fffffff;
-        const int64_t off = row_offset(P.s, P.src.stride, row) + c0 * P.col_stride;
-        uint16_t w[3][8];
+    const int lane = threadIdx.x & 31;
+    const int64_t warps = (int64_t)gridDim.x * 8;
+    for (int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < P.s.rows; row += warps) {
+        const bool none = no_target(P.label, P.ids, P.top, row);
+        const int64_t off = row_offset(P.s, P.src.stride, row), cs = P.col_stride;
+        float f = P.scale ? *P.scale : 1.0f;
+        if (P.un) {
+            uint32_t m = 0;
+            if (!none)
+#pragma unroll 4
+                for (int64_t c = lane; c < P.cols; c += 32) m = max(m, finite_bits(((const float *)P.src.p)[off + c * cs]));
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const bool in = !none && c0 + j < P.cols;
-            if (P.f32) {
-                const float x = in ? ((const float *)P.src.p)[off + j * P.col_stride] : 0.0f;
-                const uint32_t hi = pack_bf16x2_hw(x, 0.0f) & 0xffffu;
-                const float r = __fsub_rn(x, bf16_up(hi));
-                const uint32_t mid = pack_bf16x2_hw(r, 0.0f) & 0xffffu;
-                const uint32_t lo = pack_bf16x2_hw(__fsub_rn(r, bf16_up(mid)), 0.0f) & 0xffffu;
-                const bool whole = fabsf(x) <= 3.38e38f; // an infinity or a NaN (or what rounds to one) stays in its first plane
-                w[0][j] = (uint16_t)hi; w[1][j] = whole ? (uint16_t)mid : 0; w[2][j] = whole ? (uint16_t)lo : 0;
-            } else w[0][j] = in ? ((const uint16_t *)P.src.p)[off + j * P.col_stride] : 0;
+            for (int o = 16; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+            const int e = scale_of(m);
+            f = pow2(e);
+            if (lane == 0) P.un[row] = pow2(-e);
         }
-        for (int k = 0; k < P.copies; ++k)
-#pragma unroll
-            for (int pl = 0; pl < 3; ++pl)
-                if (pl == 0 || P.f32)
-                    *reinterpret_cast<uint4 *>(P.dst + pl * P.plane + (k * P.s.rows + row) * P.ld + c0) =
-                        make_uint4(w[pl][0] | (uint32_t)w[pl][1] << 16, w[pl][2] | (uint32_t)w[pl][3] << 16, w[pl][4] | (uint32_t)w[pl][5] << 16, w[pl][6] | (uint32_t)w[pl][7] << 16);
+        uint16_t *dst = P.dst + row * P.ld;
+        const int64_t again = P.s.rows * P.ld;
+#pragma unroll 8
+        for (int64_t c = lane; c < P.ld; c += 32) {
+            const bool in = !none && c < P.cols;
+            if (P.to == PACK_SPLIT) {
+                const float x = in ? __fmul_rn(((const float *)P.src.p)[off + c * cs], f) : 0.0f;
+                const uint32_t hi = pack_f16x2_hw(x, 0.0f) & 0xffffu;
+                const float r = __fsub_rn(x, f16_to_f32((uint16_t)hi)); // an infinity or a NaN stays in its first plane
+                dst[c] = (uint16_t)hi;
+                dst[c + P.plane] = fabsf(r) < 65504.0f ? (uint16_t)(pack_f16x2_hw(r, 0.0f) & 0xffffu) : 0;
+            } else {
+                uint16_t w = in ? ((const uint16_t *)P.src.p)[off + c * cs] : 0;
+                if (P.to == PACK_F16) w = (uint16_t)(pack_f16x2_hw(__fmul_rn(bf16_up(w), f), 0.0f) & 0xffffu);
+                dst[c] = w;
+                if (P.copies > 1) dst[c + again] = w;
+            }
+        }
     }
 }
 
 // A gradient from its f32 partial sums into its place: the splits' sums in their order (and, of few rows, those of g's
-// remainder `fold` rows below), times the binary16 scale's reciprocal, rounded once.
+// remainder `fold` rows below), times what undoes the scales, rounded once. Four columns a thread.
 struct SumParams {
     RowSpace s;
     const float *part;
-    int64_t parts, part_rows, ld, fold, cols, col_stride;
-    const uint32_t *scale;
+    int64_t parts, part_rows, ld, fold, cols, col_stride; // ld: a multiple of 4
+    const Scales *scales;
+    int32_t un; // 1: scales->un_dx, 2: scales->un_dw
     RowOperand dst;
     uint32_t *ovf;
     int32_t guarded;
@@ -643,18 +827,28 @@ struct SumParams {
 
 static __global__ void __launch_bounds__(256) k_head_sum(const __grid_constant__ SumParams P)
 {
-    const int64_t total = P.s.rows * P.cols, step = (int64_t)gridDim.x * blockDim.x;
-    const float un = P.scale ? __uint_as_float(P.scale[1]) : 1.0f;
+    const int64_t quads = (P.cols + 3) / 4, warps = (int64_t)gridDim.x * 8, chunks = (quads + 31) / 32;
+    const int lane = threadIdx.x & 31;
+    const float un = !P.scales ? 1.0f : P.un == 1 ? P.scales->un_dx : P.scales->un_dw;
     uint32_t ovf = 0;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += step) {
-        const int64_t row = i / P.cols, c = i - row * P.cols;
+    for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < P.s.rows * chunks; i += warps) {
+        const int64_t row = i / chunks, c = ((i - row * chunks) * 32 + lane) * 4;
+        if (c >= P.cols) continue;
+        float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         const float *src = P.part + row * P.ld + c;
-        float a = 0.0f;
+#pragma unroll 4
         for (int64_t k = 0; k < P.parts; ++k) {
-            a = __fadd_rn(a, src[k * P.part_rows * P.ld]);
-            if (P.fold) a = __fadd_rn(a, src[(k * P.part_rows + P.fold) * P.ld]);
+            const float4 q = *reinterpret_cast<const float4 *>(src + k * P.part_rows * P.ld);
+            a[0] = __fadd_rn(a[0], q.x); a[1] = __fadd_rn(a[1], q.y); a[2] = __fadd_rn(a[2], q.z); a[3] = __fadd_rn(a[3], q.w);
+            if (P.fold) {
+                const float4 r = *reinterpret_cast<const float4 *>(src + (k * P.part_rows + P.fold) * P.ld);
+                a[0] = __fadd_rn(a[0], r.x); a[1] = __fadd_rn(a[1], r.y); a[2] = __fadd_rn(a[2], r.z); a[3] = __fadd_rn(a[3], r.w);
+            }
         }
-        ovf |= store_real(const_cast<void *>(P.dst.p), P.dst.dtype, row_offset(P.s, P.dst.stride, row) + c * P.col_stride, __fmul_rn(a, un));
+        const int64_t off = row_offset(P.s, P.dst.stride, row) + c * P.col_stride;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (c + j < P.cols) ovf |= store_real(const_cast<void *>(P.dst.p), P.dst.dtype, off + j * P.col_stride, __fmul_rn(a[j], un));
     }
     if (P.guarded && ovf) atomicOr(P.ovf, 1u);
 }

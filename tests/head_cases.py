@@ -79,12 +79,16 @@ def plain(s, lse_in=None):
     ct = torch.where(has, s["ct"].reshape(-1).double(), 0.0) / tau
     e = torch.where(has[:, None], torch.exp(z - lse[:, None]), 0.0)
     g = (e - q) * ct[:, None]
-    # A logit's error. An accumulator holds up to 256 products of the summed axis: 16 matrix instructions of 16
+    # A logit's error. An accumulator holds up to 512 products of the summed axis: 32 matrix instructions of 16
     # (24 for the planes of f32) that each add by truncation, below 2^-23 of a partial sum, itself at most
-    # the sum of |x w|; those partial sums are then added rounded to nearest. f32's planes leave out 3·2^-24 a product.
+    # the sum of |x w|; those partial sums are then added rounded to nearest.
     absum = x.abs() @ w.abs().t() / tau
     chunks = (s["model"] + 63) // 64
-    el = absum * (24 * 2.0**-23 + (chunks + 4) * 2.0**-24) + 1e-30
+    el = absum * (32 * 2.0**-23 + (chunks + 4) * 2.0**-24) + 1e-30
+    small = 2.0**-39  # of the greatest element: half binary16's least step, when the greatest is scaled to 2^14 or more
+    if dt == abi.F32 and x.numel():
+        # two binary16 planes: each operand to 2^-23 (its second plane's half step), lo·lo left out, below 2^-22
+        el = el + absum * 2.0**-21 + small * (x.abs().amax(1, keepdim=True) * w.abs().sum(1)[None] + w.abs().amax() * x.abs().sum(1, keepdim=True)) / tau
     el_row = el.amax(1) if rows and s["vocab"] else torch.zeros(rows, dtype=torch.float64, device=x.device)
     # the exponentials' sum: 2^-22 a term (the hardware's), 34 additions a thread and as many as there are parts; the
     # exponent's product and differences round once each
@@ -97,14 +101,19 @@ def plain(s, lse_in=None):
     # gradients: g's own error (e from a logit and a log-sum-exp that are off by b_lse and el; p), its rounding to the
     # operands' type, then a sum of products by truncation (as above, chunks of 256) and the result's rounding
     eg = ct.abs()[:, None] * (e * (el + b_lse[:, None] + ez[:, None]) + q * 2.0**-20) + g.abs() * (HALF[dt] + 2.0**-22)
-    if dt == abi.F16:  # stored times a power of two that brings the greatest ct near 2^15: steps of 2^-24 of that scale
-        eg = eg + torch.where(has[:, None], ct.abs().amax() * 2.0**-38, 0.0)
-    if dt == abi.F32:
-        eg = eg + 3 * 2.0**-24 * g.abs()
+    if dt != abi.F32 or not x.numel():
+        planes = 0.0
+    else:
+        planes = 2.0**-21  # of a product, as above
+    if x.numel():
+        eg = eg + torch.where(has[:, None], ct.abs().amax() * 2 * small, 0.0)  # g in binary16 is scaled by the greatest ct
     dx, dw = g @ w, g.t() @ x
-    acc = 24 * 2.0**-23 + (max(s["vocab"], rows) // 64 + 8) * 2.0**-24 + (3 * 2.0**-24 if dt == abi.F32 else 0.0)
-    b_dx = eg @ w.abs() + acc * (g.abs() @ w.abs()) + dx.abs() * HALF[dt] * 1.01 + LEAST[dt]
-    b_dw = eg.t() @ x.abs() + acc * (g.abs().t() @ x.abs()) + dw.abs() * HALF[dt] * 1.01 + LEAST[dt]
+    # one accumulator throughout: truncation below 2^-23 of a partial sum an instruction of 16
+    acc = (max(s["vocab"], 2 * rows) // 16 + 8) * 2.0**-23 + planes
+    low = small * (g.abs().sum(1, keepdim=True) * w.abs().amax() if x.numel() else 0.0)  # copies of w and x in binary16
+    low_w = small * (g.abs().sum(0)[:, None] * x.abs().amax() if x.numel() else 0.0)
+    b_dx = eg @ w.abs() + acc * (g.abs() @ w.abs()) + low + dx.abs() * HALF[dt] * 1.01 + LEAST[dt]
+    b_dw = eg.t() @ x.abs() + acc * (g.abs().t() @ x.abs()) + low_w + dw.abs() * HALF[dt] * 1.01 + LEAST[dt]
     if not s["vocab_major"]:
         dw, b_dw = dw.t(), b_dw.t()
     shape = s["ct"].shape

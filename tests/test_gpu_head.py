@@ -65,6 +65,12 @@ CASES = [
     dict(outer=(33,), vocab=384, model=136, dtype=abi.F32),
     dict(outer=(200,), vocab=777, model=257, dtype=abi.F32, vocab_major=True),
     dict(outer=(700,), vocab=130, model=40, dtype=abi.BF16),
+    # many rows (g in binary16, x and w copied into it), and enough tiles of dw for the products of 256 rows
+    dict(outer=(257,), vocab=640, model=320, dtype=abi.BF16),
+    dict(outer=(300,), vocab=10000, model=2048, dtype=abi.BF16),
+    dict(outer=(301,), vocab=10001, model=2052, dtype=abi.BF16, vocab_major=True),
+    dict(outer=(290,), vocab=9999, model=2051, dtype=abi.F16),
+    dict(outer=(5000,), vocab=520, model=4100, dtype=abi.BF16, top=5, tau=2.0),
     # every row without a target; none
     dict(outer=(17,), vocab=100, model=32, dtype=abi.BF16, ignored=1.1),
     dict(outer=(17,), vocab=100, model=32, dtype=abi.F32, ignored=1.1, top=3),
@@ -280,6 +286,35 @@ def test_precision_of_long_sums(cuda):
     got = run(cuda, s)
     compare(got, want, tol)
     assert float((got["lse"].double() - want["lse"]).norm() / want["lse"].norm()) < 2e-6
+
+
+@pytest.mark.parametrize("rows", [1, 3, 60, 200, 400])
+@pytest.mark.parametrize("top", [0, 4])
+def test_gradients_are_as_exact_as_their_type(cuda, rows, top):
+    """bf16 results: g's own rounding must not show beside the result's (its half step is 2^-8, 2^-9.2 on average)."""
+    s = hc.make((rows,), 3000, 256, abi.BF16, device="cuda", top=top, ignored=0.0, seed=rows)
+    want, _ = hc.plain(s)
+    got = run(cuda, s)
+    for k in ("dx", "dw"):
+        off = float((got[k].double() - want[k]).norm() / want[k].norm())
+        best = float((want[k].to(torch.bfloat16).double() - want[k]).norm() / want[k].norm())
+        assert off <= 1.1 * best, (k, off, best)
+
+
+def test_rows_of_other_magnitudes(cuda):
+    """f32 operands are split about a row's own greatest element: a row of 1e18 takes nothing from its neighbours' logits."""
+    s = hc.make((140,), 300, 64, abi.F32, device="cuda", ignored=0.0)
+    want, tol = hc.plain(s)
+    s["x"][7] *= 1e18
+    s["x"][9] *= 1e-18
+    got = run(cuda, s, step=False)
+    rest = torch.tensor([i not in (7, 9) for i in range(140)], device="cuda")
+    for k in ("loss", "lse"):
+        assert ((got[k][rest].double() - want[k][rest]).abs() <= tol[k][rest]).all(), k
+    w9, t9 = hc.plain(s)
+    assert (got["lse"][9].double() - w9["lse"][9]).abs() <= t9["lse"][9]
+    big = w9["lse"][7]
+    assert (got["lse"][7].double() - big).abs() <= t9["lse"][7]
 
 
 def test_a_class_the_vocabulary_does_not_have(cuda):
