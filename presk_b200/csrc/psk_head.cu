@@ -3,6 +3,7 @@
 #include "psk_head.h"
 #include "psk_head_shape.h"
 #include <algorithm>
+#include <atomic>
 #include <cstring>
 #include <vector>
 #include "psk_head.cuh"
@@ -12,7 +13,7 @@ namespace {
 
 using namespace head;
 
-constexpr int64_t kPieceBytes = 512ll << 20; // what a piece's g (and copy of the head, where one is needed) may take
+constexpr int64_t kPieceBytes = 768ll << 20; // what a piece's g and copies of the head may take: 8192 rows of the 7B head in one piece
 
 int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 
@@ -79,7 +80,7 @@ int fail(HeadContext &x, int code, const std::string &msg)
         if (err__ != cudaSuccess) return fail(x, PSK_E10001, std::string(#call) + ": " + cudaGetErrorString(err__)); \
     } while (0)
 
-template <int MODE, int MT = 1>
+template <int MODE, int MT = 1, bool REST = false>
 int product(HeadContext &x, Params P, const Operand &a, const Operand &b, int f16)
 {
     CUtensorMap ma, mb;
@@ -90,15 +91,21 @@ int product(HeadContext &x, Params P, const Operand &a, const Operand &b, int f1
     P.nprod = a.planes == 2 ? 3 : 1;
     if (MODE != MODE_OUT) { P.splits = 1; P.kb_split = P.kb_k; }
     // Steps an accumulator: 512 products of the summed axis (384 of f32's, three a block). Results of 16 bits, dx and dw, keep one
-    // accumulator throughout: what truncation loses there is far below their rounding.
-    P.chunk = MODE == MODE_OUT && P.out_dtype != PSK_F32 ? 1 << 28 : P.nprod == 3 ? 6 : 8;
+    // accumulator throughout, and g's logits 1024 products: what truncation loses there is far below their rounding.
+    P.chunk = MODE == MODE_OUT && P.out_dtype != PSK_F32 ? 1 << 28 : P.nprod == 3 ? 6 : MODE == MODE_GRAD ? 16 : 8;
     // a panel's columns of b stay in a quarter of the L2 while a's rows stream past them
     P.panel = std::min<int64_t>(P.tiles_n, std::max<int64_t>(8, (16ll << 20) / std::max<int64_t>(1, BN * a.k * 2 * a.planes)));
     P.in_f16 = f16; P.a_m_major = !a.k_contiguous; P.b_n_major = !b.k_contiguous;
     P.status = x.status;
-    HEAD_TRY(cudaFuncSetAttribute(k_head<MODE, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<MT>::SMEM_TOTAL));
+    static std::atomic<uint64_t> set{0}; // devices whose copy of this kernel has its shared memory allowed
+    int device = 0;
+    HEAD_TRY(cudaGetDevice(&device));
+    if (device >= 64 || !(set.load(std::memory_order_relaxed) >> device & 1)) {
+        HEAD_TRY(cudaFuncSetAttribute(k_head<MODE, MT, REST>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<MT>::SMEM_TOTAL));
+        if (device < 64) set.fetch_or(1ull << device, std::memory_order_relaxed);
+    }
     const int64_t tiles = P.tiles_m * P.tiles_n * P.splits;
-    k_head<MODE, MT><<<(unsigned)std::min<int64_t>(tiles, x.sms), THREADS, Cfg<MT>::SMEM_TOTAL, x.stream>>>(ma, mb, P);
+    k_head<MODE, MT, REST><<<(unsigned)std::min<int64_t>(tiles, x.sms), THREADS, Cfg<MT>::SMEM_TOTAL, x.stream>>>(ma, mb, P);
     x.kernels += 1;
     x.flops += 2.0 * (double)P.m * (double)P.n * (double)a.k;
     return PSK_OK;
@@ -106,6 +113,27 @@ int product(HeadContext &x, Params P, const Operand &a, const Operand &b, int f1
 
 // Blocks of eight warps for `work` warps' worth.
 int warps_of(const HeadContext &x, int64_t work) { return (int)std::max<int64_t>(1, std::min<int64_t>((work + 7) / 8, (int64_t)x.sms * 8)); }
+
+// The copy's kernel by what it makes and whether it may read and write 16 bytes at a time.
+void pack(HeadContext &x, const PackParams &k)
+{
+    bool vec = k.col_stride == 1 && k.cols == k.ld && ((uintptr_t)k.src.p & 15u) == 0;
+    const int64_t unit = k.to == PACK_SPLIT ? 4 : 8; // elements of 16 bytes
+    for (int a = 0; a < k.s.no; ++a) vec = vec && (k.s.dims[a] == 1 || k.src.stride[a] % unit == 0);
+    const int grid = warps_of(x, k.un ? k.s.rows : k.s.rows * ((k.ld + PIECE - 1) / PIECE));
+    if (k.to == PACK_SPLIT) { if (vec) k_head_pack<PACK_SPLIT, true><<<grid, 256, 0, x.stream>>>(k); else k_head_pack<PACK_SPLIT, false><<<grid, 256, 0, x.stream>>>(k); }
+    else if (k.to == PACK_F16) { if (vec) k_head_pack<PACK_F16, true><<<grid, 256, 0, x.stream>>>(k); else k_head_pack<PACK_F16, false><<<grid, 256, 0, x.stream>>>(k); }
+    else { if (vec) k_head_pack<PACK_SAME, true><<<grid, 256, 0, x.stream>>>(k); else k_head_pack<PACK_SAME, false><<<grid, 256, 0, x.stream>>>(k); }
+    x.kernels += 1;
+}
+
+void greatest(HeadContext &x, const MaxParams &m)
+{
+    const int grid = warps_of(x, m.s.rows * ((m.cols + PIECE - 1) / PIECE));
+    if (m.src.dtype == PSK_F32) k_head_max<true><<<grid, 256, 0, x.stream>>>(m);
+    else k_head_max<false><<<grid, 256, 0, x.stream>>>(m);
+    x.kernels += 1;
+}
 
 RowOperand row_operand(const psk_operand &o, void *base, int no)
 {
@@ -190,7 +218,7 @@ int head_run(HeadContext &x, const psk_launch *l, void *const *table)
         const int64_t kb = (k + BK - 1) / BK, tiles = ((m + BM - 1) / BM) * ((n + BN - 1) / BN);
         o.two = !f32 && m >= 2 * BM && tiles >= 2 * x.sms;
         // few tiles: cut the summed axis, so that every SM has some of it
-        const int64_t want = std::max<int64_t>(1, std::min<int64_t>(x.sms / tiles, kb / 4));
+        const int64_t want = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(x.sms / tiles, 32), kb / 4));
         o.kb_split = (int32_t)((kb + want - 1) / want);
         o.splits = (kb + o.kb_split - 1) / o.kb_split;
         if (o.splits > 1) o.straight = false;
@@ -202,21 +230,22 @@ int head_run(HeadContext &x, const psk_launch *l, void *const *table)
     if (vjp && N) dxo = plan(Ng, D, Vc, !rest && pieces == 1 && dx_ld && O.stride[ax_d] == 1);
     if (DW && N) dwo = plan(dw_v_inner ? D : Vc, dw_v_inner ? Vc : D, Ng, DW->stride[dw_v_inner ? ax_v : ax_d] == 1);
 
-    int32_t *label, *ids;
+    int32_t *ids;
+    uint16_t *start;
     float *p, *plogp, *coef, *lse2, *hit, *dxp, *dwp, *un_x;
     float2 *part;
     uint16_t *xl, *xd, *wl, *wd, *g;
     Scales *scales;
     Slab slab(x);
     const bool xl_is_xd = vjp && !f32 && !conv; // the copy of x that dw reads serves the logits too
-    slab.need(label, distill ? 0 : N);
-    slab.need(ids, distill ? N * K : 0);
+    slab.need(ids, N * K);
+    slab.need(start, distill ? N * (parts + 1) : 0);
     slab.need(p, distill ? N * K : 0);
     slab.need(plogp, distill ? N : 0);
     slab.need(coef, vjp ? N : 0);
     slab.need(lse2, vjp ? N : 0);
     slab.need(part, vjp ? 0 : parts * N);
-    slab.need(hit, vjp ? 0 : distill ? parts * N : N);
+    slab.need(hit, vjp ? 0 : N * K);
     slab.need(un_x, f32 ? N : 0);
     slab.need(xl, x_direct || xl_is_xd ? 0 : N * Dp * planes);
     slab.need(xd, DW || (xl_is_xd && !x_direct) ? Ng * Dp * planes : 0);
@@ -238,13 +267,13 @@ int head_run(HeadContext &x, const psk_launch *l, void *const *table)
             memset(&T, 0, sizeof T);
             T.s = s; T.ids = rids; T.t = row_operand(l->in[3], table[3], no); T.ct = rct; T.lse = rlse;
             T.ids_k = I.stride[ax_k]; T.t_k = l->in[3].stride[ax_k]; T.classes = V; T.top = (int32_t)K; T.inv_tau = inv_tau;
-            T.out_ids = ids; T.out_p = p; T.plogp = plogp; T.coef = coef; T.lse2 = lse2; T.status = x.status; T.ctmax = g_scaled ? &scales->max_ct : nullptr;
-            k_head_teacher<<<(unsigned)N, (unsigned)up(K, 32), (size_t)K * 4, x.stream>>>(T);
+            T.out_ids = ids; T.start = start; T.parts = parts; T.out_p = p; T.plogp = plogp; T.coef = coef; T.lse2 = lse2; T.status = x.status; T.ctmax = g_scaled ? &scales->max_ct : nullptr;
+            k_head_teacher<<<(unsigned)N, (unsigned)up(K, 32), (size_t)K * 8, x.stream>>>(T);
         } else {
             LabelParams T;
             memset(&T, 0, sizeof T);
             T.s = s; T.ids = rids; T.ct = rct; T.lse = rlse; T.classes = V; T.inv_tau = inv_tau;
-            T.label = label; T.coef = coef; T.lse2 = lse2; T.status = x.status; T.ctmax = g_scaled ? &scales->max_ct : nullptr;
+            T.ids_out = ids; T.coef = coef; T.lse2 = lse2; T.status = x.status; T.ctmax = g_scaled ? &scales->max_ct : nullptr;
             k_head_labels<<<(unsigned)((N + 255) / 256), 256, 0, x.stream>>>(T);
         }
         x.kernels += 1;
@@ -254,80 +283,73 @@ int head_run(HeadContext &x, const psk_launch *l, void *const *table)
             MaxParams M;
             if (of_x) {
                 memset(&M, 0, sizeof M);
-                M.s = s; M.src = rx; M.col_stride = X.stride[ax_d]; M.cols = D; M.label = label; M.ids = ids; M.top = (int32_t)K; M.out = &scales->max_x;
+                M.s = s; M.src = rx; M.col_stride = X.stride[ax_d]; M.cols = D; M.ids = ids; M.top = (int32_t)K; M.out = &scales->max_x;
                 M.vec = x_ld && M.col_stride == 1 && aligned(rx.p) && x_ld * eb % 16 == 0 && D * eb % 16 == 0;
-                k_head_max<<<warps_of(x, N), 256, 0, x.stream>>>(M);
-                x.kernels += 1;
+                greatest(x, M);
             }
             if (of_w) {
                 memset(&M, 0, sizeof M);
                 M.s.no = 1; M.s.rows = M.s.dims[0] = v_inner ? D : V; M.src.p = wp; M.src.dtype = dt; M.src.stride[0] = v_inner ? w_d : w_v;
                 M.col_stride = v_inner ? w_v : w_d; M.cols = v_inner ? V : D; M.out = &scales->max_w;
                 M.vec = M.col_stride == 1 && aligned(wp) && M.src.stride[0] * eb % 16 == 0 && M.cols * eb % 16 == 0;
-                k_head_max<<<warps_of(x, M.s.rows), 256, 0, x.stream>>>(M);
-                x.kernels += 1;
+                greatest(x, M);
             }
-            k_head_scales<<<1, 1, 0, x.stream>>>(scales, (of_x ? 1 : 0) | (of_w ? 2 : 0) | (g_scaled ? 4 : 0));
-            x.kernels += 1;
         }
     }
     // 3. x for the logits, and (rows without a target zeros) for dw
     PackParams kx;
     memset(&kx, 0, sizeof kx);
-    kx.s = s; kx.src = rx; kx.col_stride = X.stride[ax_d]; kx.cols = D; kx.ld = Dp; kx.label = label; kx.ids = ids; kx.top = (int32_t)K; kx.copies = 1;
+    kx.s = s; kx.src = rx; kx.col_stride = X.stride[ax_d]; kx.cols = D; kx.ld = Dp; kx.ids = ids; kx.top = (int32_t)K; kx.copies = 1;
     if (xl) {
         PackParams k = kx;
         k.dst = xl; k.plane = N * Dp; k.to = f32 ? PACK_SPLIT : PACK_SAME; k.un = un_x;
-        k_head_pack<<<warps_of(x, N), 256, 0, x.stream>>>(k);
-        x.kernels += 1;
+        pack(x, k);
     }
     if (xd && N) {
         PackParams k = kx;
         k.dst = xd; k.plane = N * Dp; k.to = f32 ? PACK_SPLIT : conv ? PACK_F16 : PACK_SAME; k.copies = (int32_t)(Ng / N);
-        k.scale = f32 || conv ? &scales->x : nullptr;
-        k_head_pack<<<warps_of(x, N), 256, 0, x.stream>>>(k);
-        x.kernels += 1;
+        k.max = f32 || conv ? &scales->max_x : nullptr;
+        pack(x, k);
     }
     const Operand a = x_direct ? Operand{rx.p, N, D, x_ld, true, 1, 0} : Operand{xl ? xl : xd, N, D, Dp, true, planes, N * Dp};
 
     for (int64_t piece = 0; piece < pieces && N > 0; ++piece) {
         const int64_t v0 = piece * Vc, vn = std::min(Vc, V - v0);
         // 4. the piece of the head
-        auto pack_w = [&](uint16_t *dst, int to, const float *scale) {
+        auto pack_w = [&](uint16_t *dst, int to, const uint32_t *max) {
             PackParams k;
             memset(&k, 0, sizeof k);
             k.s.no = 1; k.s.rows = k.s.dims[0] = v_inner ? D : vn;
             k.src.p = wp + v0 * w_v * eb; k.src.dtype = dt; k.src.stride[0] = v_inner ? w_d : w_v;
-            k.col_stride = v_inner ? w_v : w_d; k.cols = v_inner ? vn : D; k.ld = wc_ld; k.plane = wc_plane; k.dst = dst; k.to = to; k.scale = scale; k.copies = 1;
-            k_head_pack<<<warps_of(x, k.s.rows), 256, 0, x.stream>>>(k);
-            x.kernels += 1;
+            k.col_stride = v_inner ? w_v : w_d; k.cols = v_inner ? vn : D; k.ld = wc_ld; k.plane = wc_plane; k.dst = dst; k.to = to; k.max = max; k.copies = 1;
+            pack(x, k);
             return Operand{dst, vn, D, wc_ld, !v_inner, planes, wc_plane};
         };
-        const Operand b = w_direct ? Operand{wp + v0 * w_v * 2, vn, D, v_inner ? w_d : w_v, !v_inner, 1, 0} : pack_w(wl, f32 ? PACK_SPLIT : PACK_SAME, f32 ? &scales->w : nullptr);
+        const Operand b = w_direct ? Operand{wp + v0 * w_v * 2, vn, D, v_inner ? w_d : w_v, !v_inner, 1, 0} : pack_w(wl, f32 ? PACK_SPLIT : PACK_SAME, f32 ? &scales->max_w : nullptr);
         // 5. the logits' tiles
         Params P;
         memset(&P, 0, sizeof P);
         P.scales = scales; P.logits_scaled = f32; P.un_x = un_x;
         P.c = (float)(1.4426950408889634 / tau); P.rows = N; P.col0 = v0;
-        P.label = label; P.ids = ids; P.p = p; P.top = (int32_t)K;
+        P.ids = ids; P.p = p; P.start = start; P.top = (int32_t)K; P.parts = parts;
         if (!vjp) {
-            P.part = part; P.hit = hit; P.part0 = v0 / COLS;
+            P.part = part; P.hit = hit;
             const int r = product<MODE_STATS>(x, P, a, b, in_f16);
             if (r != PSK_OK) return r;
             continue;
         }
-        P.lse2 = lse2; P.coef = coef; P.g = g; P.g_f16 = g_f16; P.g_ld = g_ld; P.g_rest = rest || f32 ? N * g_ld : 0;
-        int r = product<MODE_GRAD>(x, P, a, b, in_f16);
+        P.lse2 = lse2; P.coef = coef; P.g = g; P.g_f16 = g_f16; P.g_ld = g_ld; P.g_rest = N * g_ld;
+        int r = rest || f32 ? product<MODE_GRAD, 1, true>(x, P, a, b, in_f16) : product<MODE_GRAD>(x, P, a, b, in_f16);
         if (r != PSK_OK) return r;
         // 6. dx = g·wᵀ summed over the pieces: both operands along the classes
-        const Operand bd = conv ? pack_w(wd, PACK_F16, &scales->w) : b;
+        const Operand bd = conv ? pack_w(wd, PACK_F16, &scales->max_w) : b;
         Params Q;
         memset(&Q, 0, sizeof Q);
         Q.scales = scales;
         Q.kb_split = dxo.kb_split;
         Q.splits = ((vn + BK - 1) / BK + dxo.kb_split - 1) / dxo.kb_split; // a shorter last piece may have fewer
         Q.out = dxo.straight ? const_cast<void *>(rout.p) : dxp; Q.out_ld = dxo.straight ? dx_ld : dxo.ld; Q.out_dtype = dxo.straight ? dt : PSK_F32;
-        Q.un = dxo.straight ? 1 : 0; Q.accumulate = piece > 0;
+        Q.un = dxo.straight ? UN_DX : UN_NONE; Q.accumulate = piece > 0;
         Q.out_vec = !dxo.straight || (aligned(rout.p) && dx_ld * eb % 16 == 0 && D * eb % 16 == 0);
         Q.ovf = x.guarded && dxo.straight ? x.ovf : nullptr;
         const Operand gk{g, Ng, vn, g_ld, true, planes, N * g_ld}, wk{bd.p, D, vn, bd.ld, v_inner, planes, bd.plane};
@@ -342,7 +364,7 @@ int head_run(HeadContext &x, const psk_launch *l, void *const *table)
             Q.scales = scales;
             Q.splits = dwo.splits; Q.kb_split = dwo.kb_split;
             Q.out = dwo.straight ? (void *)dst : dwp; Q.out_ld = dwo.straight ? dw_ld : dwo.ld; Q.out_dtype = dwo.straight ? dt : PSK_F32;
-            Q.un = dwo.straight ? 2 : 0;
+            Q.un = dwo.straight ? UN_DW : UN_NONE;
             Q.out_vec = !dwo.straight || (aligned(dst) && dw_ld * eb % 16 == 0 && cols * eb % 16 == 0);
             Q.ovf = x.guarded && dwo.straight ? x.ovf : nullptr;
             r = dwo.two ? product<MODE_OUT, 2>(x, Q, dw_v_inner ? xr : gr, dw_v_inner ? gr : xr, g_f16) : product<MODE_OUT>(x, Q, dw_v_inner ? xr : gr, dw_v_inner ? gr : xr, g_f16);
@@ -352,7 +374,7 @@ int head_run(HeadContext &x, const psk_launch *l, void *const *table)
                 memset(&S, 0, sizeof S);
                 S.s.no = 1; S.s.rows = S.s.dims[0] = dw_v_inner ? D : vn;
                 S.part = dwp; S.parts = dwo.splits; S.part_rows = S.s.rows; S.ld = dwo.ld; S.cols = cols; S.col_stride = DW->stride[dw_v_inner ? ax_v : ax_d];
-                S.scales = scales; S.un = 2; S.dst.p = dst; S.dst.dtype = dt; S.dst.stride[0] = dw_ld; S.ovf = x.ovf; S.guarded = x.guarded;
+                S.scales = scales; S.un = UN_DW; S.dst.p = dst; S.dst.dtype = dt; S.dst.stride[0] = dw_ld; S.ovf = x.ovf; S.guarded = x.guarded;
                 k_head_sum<<<warps_of(x, S.s.rows * ((S.cols + 127) / 128)), 256, 0, x.stream>>>(S);
                 x.kernels += 1;
             }
@@ -361,16 +383,17 @@ int head_run(HeadContext &x, const psk_launch *l, void *const *table)
     if (!vjp) {
         JoinParams J;
         memset(&J, 0, sizeof J);
-        J.s = s; J.halves = parts; J.part = part; J.hit = hit; J.label = label; J.ids = ids; J.plogp = plogp; J.top = (int32_t)K; J.c = (float)(1.4426950408889634 / tau); J.inv_tau = 1.0 / tau;
+        J.s = s; J.parts = parts; J.part = part; J.hit = hit; J.ids = ids; J.p = p; J.plogp = plogp; J.top = (int32_t)K; J.c = (float)(1.4426950408889634 / tau); J.inv_tau = 1.0 / tau;
         J.loss = rout; J.ovf = x.ovf; J.guarded = x.guarded;
         if (LSE) J.lse = row_operand(*LSE, table[h.lse], no);
-        k_head_join<<<(unsigned)((N + 7) / 8), 256, 0, x.stream>>>(J);
+        if (N >= 32 * x.sms) k_head_join<32><<<(unsigned)((N + 31) / 32), 256, 0, x.stream>>>(J);
+        else k_head_join<8><<<(unsigned)((N + 7) / 8), 256, 0, x.stream>>>(J);
         x.kernels += 1;
     } else if (N > 0 && !dxo.straight) {
         SumParams S;
         memset(&S, 0, sizeof S);
         S.s = s; S.part = dxp; S.parts = dxo.splits; S.part_rows = dxo.m; S.ld = dxo.ld; S.fold = rest ? N : 0; S.cols = D; S.col_stride = O.stride[ax_d];
-        S.scales = scales; S.un = 1; S.dst = rout; S.ovf = x.ovf; S.guarded = x.guarded;
+        S.scales = scales; S.un = UN_DX; S.dst = rout; S.ovf = x.ovf; S.guarded = x.guarded;
         k_head_sum<<<warps_of(x, N * ((D + 127) / 128)), 256, 0, x.stream>>>(S);
         x.kernels += 1;
     } else if (N == 0 && DW) { // no rows: a gradient of zeros

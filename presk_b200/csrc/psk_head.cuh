@@ -20,6 +20,7 @@
 // g itself is kept in binary16 for f32 and, for many rows, for bf16 operands too, x and w being copied into it (exactly:
 // eight bits into eleven): g in bf16 would cost its 2^-9 an entry, as much again as the result's own rounding.
 #pragma once
+#include <utility>
 #include "psk_dev.cuh"
 #include "psk_gemm_tc.cuh"
 
@@ -51,12 +52,29 @@ enum { MODE_STATS = 0, MODE_GRAD = 1, MODE_OUT = 2 };
 PSK_DEV int plane_a(int q) { return q == 2; }
 PSK_DEV int plane_b(int q) { return q == 1; }
 
-// Powers of two that the operands are scaled by, in device memory: what k_head_scales makes of the maxima.
+// The greatest finite |element| of the operands, as f32 bits (0: not scaled), and the powers of two made of them.
 struct Scales {
-    uint32_t max_x, max_w, max_ct; // bits of the greatest finite |element|
-    float x, w, g;                 // what they are multiplied by
-    float un_w, un_dx, un_dw;      // 1/w; 1/(g·w); 1/(g·x)
+    uint32_t max_x, max_w, max_ct, pad;
 };
+
+// 2^e as an f32, e within its normal range.
+PSK_DEV float pow2(int e) { return __uint_as_float((uint32_t)(127 + (e < -126 ? -126 : e > 127 ? 127 : e)) << 23); }
+
+// The exponent of the power of two that brings a maximum into [2^14, 2^15); 0 for none.
+PSK_DEV int scale_of(uint32_t max_bits)
+{
+    const int e = (int)(max_bits >> 23);
+    if (max_bits == 0) return 0;
+    const int k = 14 + 127 - (e == 0 ? 1 : e);
+    return k > 60 ? 60 : k; // 1/(g·w) and 1/(g·x) are f32 numbers then
+}
+
+enum { UN_NONE = 0, UN_DX = 1, UN_DW = 2 }; // what a product's sums are multiplied by: 1, 1/(g·w), 1/(g·x)
+PSK_DEV float undo(const Scales *s, int un)
+{
+    if (!s || un == UN_NONE) return 1.0f;
+    return pow2(-scale_of(s->max_ct) - scale_of(un == UN_DX ? s->max_w : s->max_x));
+}
 
 struct Params {
     int64_t m, n;                 // rows and columns of the product
@@ -73,26 +91,26 @@ struct Params {
     const float *un_x;            // a row's factor that undoes its scale; or null
     int64_t rows;                 // rows with a target list
     int64_t col0;                 // the class of column 0: where the piece begins
-    const int32_t *label;         // one class a row, or -1; or null, and then
     const int32_t *ids;           // rows x top classes in ascending order, absent entries last as 0x7fffffff
-    const float *p;               // their weights
+    const float *p;               // their weights; or null: 1 (labels)
+    const uint16_t *start;        // rows x (parts + 1): a row's first entry of each 128 classes; or null: one entry a row
     int32_t top;
+    int64_t parts;                // 128-class parts of the vocabulary
     // MODE_STATS
-    float2 *part;                 // [128-column part][row]: (max, sum of 2^((l - max)·c))
-    float *hit;                   // label: [row], the label's logit; list: [part][row], sum of p·l
-    int64_t part0;                // index of the piece's first part
+    float2 *part;                 // [part][row]: (max, sum of 2^((l - max)·c))
+    float *hit;                   // rows x top: the entries' logits
     // MODE_GRAD
     const float *lse2, *coef;     // a row's log-sum-exp in base 2, and ct/τ (0 where it has no target)
     uint16_t *g;
-    int32_t g_f16;                // g in binary16, times scales->g where there are scales; else bf16
-    int64_t g_ld, g_rest;         // row stride; how much further on what the rounding leaves is kept (0: nowhere)
+    int32_t g_f16;                // g in binary16, scaled by max_ct where there are scales; else bf16
+    int64_t g_ld, g_rest;         // row stride; REST: how much further on what the rounding leaves is kept
     // MODE_OUT
     void *out;                    // [split][m][out_ld]
     int64_t out_ld;
     int32_t out_dtype;            // f32, bf16 or binary16 (one split then)
     int32_t out_vec;              // whole 16-byte units: aligned rows, n a multiple of a unit
     int32_t accumulate;           // f32: add to what is there (a later piece of the summed axis)
-    int32_t un;                   // times scales->un_dx (1), scales->un_dw (2)
+    int32_t un;                   // UN_DX, UN_DW
     uint32_t *ovf;                // the overflow guard's flag; or null
 };
 
@@ -104,6 +122,32 @@ PSK_DEV float ex2(float x)
 }
 
 PSK_DEV float bf16_up(uint32_t h) { return __uint_as_float(h << 16); }
+
+// One of a thread's registers, chosen by a number that only the thread knows: a compare and a predicated operation a
+// register, sixteen at a time. The comparison's number is a constant of the instruction: written as an index, or with
+// numbers that could be merged, the array would be moved to local memory for every tile (1.5 times the time).
+template <int I>
+PSK_DEV void pick(float &l, int y, float v)
+{
+    asm("{\n\t.reg .pred p;\n\tsetp.eq.s32 p, %1, %2;\n\t@p mov.f32 %0, %3;\n\t}" : "+f"(l) : "r"(y), "n"(I), "f"(v));
+}
+template <int I>
+PSK_DEV void take(float &v, int y, float amount)
+{
+    asm("{\n\t.reg .pred p;\n\tsetp.eq.s32 p, %1, %2;\n\t@p sub.rn.f32 %0, %0, %3;\n\t}" : "+f"(v) : "r"(y), "n"(I), "f"(amount));
+}
+template <int G, int... I>
+PSK_DEV void pick_column(float &l, int y, const float (&v)[COLS], std::integer_sequence<int, I...> s)
+{
+    if (y >> 4 == G) (pick<G * 16 + I>(l, y, v[G * 16 + I]), ...);
+    if constexpr (G + 1 < COLS / 16) pick_column<G + 1>(l, y, v, s);
+}
+template <int G, int... I>
+PSK_DEV void take_column(float (&v)[COLS], int y, float amount, std::integer_sequence<int, I...> s)
+{
+    if (y >> 4 == G) (take<G * 16 + I>(v[G * 16 + I], y, amount), ...);
+    if constexpr (G + 1 < COLS / 16) take_column<G + 1>(v, y, amount, s);
+}
 
 // First entry of a row's ascending list that is at least `c`.
 PSK_DEV int lower_bound(const int32_t *ids, int n, int32_t c)
@@ -165,7 +209,7 @@ PSK_DEV void store_rows_any(uint4 *stage, int lane, const uint32_t (&w)[32], uin
 
 // The product of a persistent CTA's tiles, and what MODE makes of it. Bounds: the tensor pipe (2·m·n·k flops) for many
 // rows; for few, the bytes of the second operand.
-template <int MODE, int MT = 1>
+template <int MODE, int MT = 1, bool REST = false>
 __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ Params P)
 {
     static_assert(MT == 1 || MODE == MODE_OUT, "two halves leave no second accumulator to sum in parts with");
@@ -296,7 +340,37 @@ __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ CUt
 #pragma unroll 1
             for (int mh = 0; mh < MT && ok; ++mh) {
             const int64_t row0 = (mt * MT + mh) * BM + quad * 32, row = row0 + lane;
+            // what the row's epilogue reads, asked for while the products still run: its factors and its first target here
+            const bool own = MODE != MODE_OUT && row < P.rows && cbase < P.n;
+            const int32_t first = (int32_t)(P.col0 + cbase); // the class of v[0]
+            int32_t y = 0x7fffffff;                          // the target's column, if it has one here
+            float pw = 1.0f, un = 1.0f, lse2 = 0.0f, coef = 0.0f;
+            int32_t at = 0, end = 0; // its place in the row's list, and how far the part's entries go
+            bool none = true;
+            const int32_t *list = nullptr;
+            if (MODE != MODE_OUT && own) {
+                list = P.ids + row * P.top;
+                end = 1;
+                none = list[0] == 0x7fffffff; // ascending, absent entries last
+                if (P.start) {
+                    const uint16_t *sr = P.start + row * (P.parts + 1) + (first / COLS);
+                    end = sr[1];
+                    at = sr[0];
+                }
+                if (at < end) {
+                    y = list[at] - first;
+                    if (P.p) pw = P.p[row * P.top + at];
+                }
+                if (P.logits_scaled) un = __fmul_rn(pow2(-scale_of(P.scales->max_w)), P.un_x ? P.un_x[row] : 1.0f);
+                if (MODE == MODE_GRAD) {
+                    lse2 = P.lse2[row];
+                    coef = P.coef[row];
+                    if (P.scales && P.g_f16) coef = __fmul_rn(coef, pow2(scale_of(P.scales->max_ct)));
+                }
+            }
             float v[COLS];
+#pragma unroll
+            for (int i = 0; i < COLS; ++i) v[i] = 0.0f;
             for (int ch = 0; ch < chunks; ++ch) {
                 if (MT == 1 || mh == 0) {
                     ok = tc::mbar_wait(MT == 1 ? tfull0 + 8 * acc : tfull0, acc_phase, abort_flag, P.status, 4u);
@@ -305,18 +379,15 @@ __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ CUt
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t ta = tmem_base + ((uint32_t)(quad * 32) << 16) + (MT == 1 ? acc : (uint32_t)mh) * BN + half * COLS;
+                // 32 columns at a time, the next 32 on their way while these are added
+                uint32_t ra[32], rb[32];
+                tc::tmem_ld32(ta, ra);
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    uint32_t r[32];
-                    tc::tmem_ld32(ta + g * 32, r);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                    if (ch == 0) {
+                    if (g < 3) tc::tmem_ld32(ta + (g + 1) * 32, g & 1 ? ra : rb);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[g * 32 + i] = __uint_as_float(r[i]);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) v[g * 32 + i] = __fadd_rn(v[g * 32 + i], __uint_as_float(r[i]));
-                    }
+                    for (int i = 0; i < 32; ++i) v[g * 32 + i] = __fadd_rn(v[g * 32 + i], __uint_as_float(g & 1 ? rb[i] : ra[i]));
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
@@ -334,10 +405,6 @@ __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ CUt
                         if (i >= live) v[i] = -INFINITY;
                 }
             }
-            const int32_t first = (int32_t)(P.col0 + cbase); // the class of v[0]
-            const bool own = row < P.rows;
-            // what undoes the operands' scales: a power of two a row
-            const float un = MODE == MODE_OUT || !P.logits_scaled ? 1.0f : __fmul_rn(P.scales->un_w, own && P.un_x ? P.un_x[row] : 1.0f);
             const float c = MODE == MODE_OUT ? 0.0f : __fmul_rn(P.c, un);
             if constexpr (MODE == MODE_STATS) {
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -346,89 +413,59 @@ __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ CUt
                 const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                 // (one rounded product m·c instead of the differences would be an instruction less, and wrong by 2^-24 of m·c)
                 const float shift = m == -INFINITY ? 0.0f : m;
-                float hit = 0.0f;
-                const int64_t th = P.part0 + 2 * nt + half;
-                if (own) {
-                    if (P.label) {
-                        const int32_t y = P.label[row] - first;
-                        if (y >= 0 && y < live) {
-#pragma unroll
-                            for (int i = 0; i < COLS; ++i)
-                                if (i == y) hit = v[i];
-                            P.hit[row] = __fmul_rn(hit, un);
-                        }
-                    } else {
-                        const int32_t *ids = P.ids + row * P.top;
-                        const float *p = P.p + row * P.top;
-                        for (int j = lower_bound(ids, P.top, first); j < P.top; ++j) {
-                            const int32_t y = ids[j] - first;
-                            if (y >= live) break;
-                            float l = 0.0f;
-#pragma unroll
-                            for (int i = 0; i < COLS; ++i)
-                                if (i == y) l = v[i];
-                            hit = __fmaf_rn(p[j], l, hit);
-                        }
-                        P.hit[th * P.rows + row] = __fmul_rn(hit, un);
-                    }
+                // the targets' logits: a column that only its thread knows, found among registers sixteen at a time
+                while (y >= 0 && y < live) {
+                    float l = 0.0f;
+                    pick_column<0>(l, y, v, std::make_integer_sequence<int, 16>());
+                    P.hit[row * P.top + at] = __fmul_rn(l, un);
+                    y = ++at < end ? list[at] - first : -1;
                 }
                 float z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int i = 0; i < COLS; ++i) z[i & 3] = __fadd_rn(z[i & 3], ex2(__fmul_rn(__fsub_rn(v[i], shift), c)));
-                if (own) P.part[th * P.rows + row] = make_float2(__fmul_rn(m, un), __fadd_rn(__fadd_rn(z[0], z[1]), __fadd_rn(z[2], z[3])));
+                if (own) P.part[(int64_t)(first / COLS) * P.rows + row] = make_float2(__fmul_rn(m, un), __fadd_rn(__fadd_rn(z[0], z[1]), __fadd_rn(z[2], z[3])));
             } else if constexpr (MODE == MODE_GRAD) {
-                const float lse2 = own ? P.lse2[row] : 0.0f;
-                float coef = own ? P.coef[row] : 0.0f;
-                const bool none = !own || (P.label ? P.label[row] < 0 : P.ids[row * P.top] == 0x7fffffff); // no target: zeros, whatever the row holds
-                if (P.scales && P.g_f16) coef = __fmul_rn(coef, P.scales->g);
 #pragma unroll
                 for (int i = 0; i < COLS; ++i) v[i] = ex2(__fmaf_rn(v[i], c, -lse2));
-                if (!none) {
-                    if (P.label) {
-                        const int32_t y = P.label[row] - first;
-                        if (y >= 0 && y < live) {
-#pragma unroll
-                            for (int i = 0; i < COLS; ++i)
-                                if (i == y) v[i] = __fadd_rn(v[i], -1.0f);
-                        }
-                    } else {
-                        const int32_t *ids = P.ids + row * P.top;
-                        const float *p = P.p + row * P.top;
-                        for (int j = lower_bound(ids, P.top, first); j < P.top; ++j) {
-                            const int32_t y = ids[j] - first;
-                            if (y >= live) break;
-                            const float pj = p[j];
-#pragma unroll
-                            for (int i = 0; i < COLS; ++i)
-                                if (i == y) v[i] = __fsub_rn(v[i], pj);
-                        }
-                    }
+                while (y >= 0 && y < live) {
+                    take_column<0>(v, y, pw, std::make_integer_sequence<int, 16>());
+                    y = -1;
+                    if (++at < end) { y = list[at] - first; pw = P.p[row * P.top + at]; }
                 }
+                // a row without a target: zeros, whatever it holds
 #pragma unroll
                 for (int i = 0; i < COLS; ++i) v[i] = none ? 0.0f : __fmul_rn(v[i], coef);
-                // Rounded for the two products that read it; where the rest of a rounding is kept too (bf16 with few
-                // rows, f32), it is the exact remainder rounded again.
+                // Rounded for the two products that read it; where the rest of a rounding is kept too (REST: few rows,
+                // f32), it is the exact remainder rounded again. Rows are padded to whole lines, the padding zeros.
                 uint8_t *base = (uint8_t *)(P.g + row0 * P.g_ld + cbase);
-                const int planes = P.g_rest ? 2 : 1;
-#pragma unroll 1
-                for (int pl = 0; pl < planes; ++pl) {
 #pragma unroll
-                    for (int g = 0; g < 2; ++g) {
-                        uint32_t w[32];
+                for (int g = 0; g < 2; ++g) {
+                    const int64_t left = (P.g_ld - cbase - g * 64) * 2;
+                    const int bytes = left < 128 ? (int)left : 128;
+                    uint32_t w[32];
+                    if (P.g_f16) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const float a = v[g * 64 + 2 * i], b = v[g * 64 + 2 * i + 1];
-                            w[i] = P.g_f16 ? pack_f16x2_hw(a, b) : pack_bf16x2_hw(a, b);
-                            v[g * 64 + 2 * i] = __fsub_rn(a, P.g_f16 ? f16_to_f32((uint16_t)(w[i] & 0xffffu)) : bf16_up(w[i] & 0xffffu));
-                            v[g * 64 + 2 * i + 1] = __fsub_rn(b, P.g_f16 ? f16_to_f32((uint16_t)(w[i] >> 16)) : bf16_up(w[i] >> 16));
+                        for (int i = 0; i < 32; ++i) w[i] = pack_f16x2_hw(v[g * 64 + 2 * i], v[g * 64 + 2 * i + 1]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) w[i] = pack_bf16x2_hw(v[g * 64 + 2 * i], v[g * 64 + 2 * i + 1]);
+                    }
+                    store_rows<false>(stage_out, lane, w, base + g * 128, P.g_ld * 2, rows_live, bytes);
+                    if constexpr (REST) {
+                        if (P.g_f16) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                w[i] = pack_f16x2_hw(__fsub_rn(v[g * 64 + 2 * i], f16_to_f32((uint16_t)(w[i] & 0xffffu))), __fsub_rn(v[g * 64 + 2 * i + 1], f16_to_f32((uint16_t)(w[i] >> 16))));
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                w[i] = pack_bf16x2_hw(__fsub_rn(v[g * 64 + 2 * i], bf16_up(w[i] & 0xffffu)), __fsub_rn(v[g * 64 + 2 * i + 1], bf16_up(w[i] >> 16)));
                         }
-                        // the rows are padded to whole lines, the padding zeros
-                        const int64_t left = (P.g_ld - cbase - g * 64) * 2;
-                        store_rows<false>(stage_out, lane, w, base + g * 128 + pl * P.g_rest * 2, P.g_ld * 2, rows_live, left < 128 ? (int)left : 128);
+                        store_rows<false>(stage_out, lane, w, base + g * 128 + P.g_rest * 2, P.g_ld * 2, rows_live, bytes);
                     }
                 }
             } else {
-                const float f = !P.scales ? 1.0f : P.un == 1 ? P.scales->un_dx : P.un == 2 ? P.scales->un_dw : 1.0f;
+                const float f = undo(P.scales, P.un);
                 if (P.out_dtype == PSK_F32) {
                     uint8_t *base = (uint8_t *)((float *)P.out + (sp * P.m + row0) * P.out_ld + cbase);
 #pragma unroll
@@ -500,14 +537,14 @@ PSK_DEV int64_t row_offset(const RowSpace &s, const int64_t *stride, int64_t row
     return off;
 }
 
-// Labels as classes (32 bits; -1 where a row has none) and, backward, a row's factor ct/τ and its log-sum-exp in
+// Labels as lists of one class (0x7fffffff where a row has none) and, backward, a row's factor ct/τ and its log-sum-exp in
 // base 2. A class that the vocabulary does not have is reported and counts as no target.
 struct LabelParams {
     RowSpace s;
     RowOperand ids, ct, lse;
     int64_t classes;
     float inv_tau;
-    int32_t *label;
+    int32_t *ids_out;
     float *coef, *lse2;
     uint32_t *status, *ctmax;
 };
@@ -529,7 +566,7 @@ static __global__ void __launch_bounds__(256) k_head_labels(const __grid_constan
     const int64_t y = ((const int64_t *)P.ids.p)[row_offset(P.s, P.ids.stride, row)];
     if (y >= P.classes) atomicOr(P.status, 2u);
     const bool none = y < 0 || y >= P.classes;
-    P.label[row] = none ? -1 : (int32_t)y;
+    P.ids_out[row] = none ? 0x7fffffff : (int32_t)y;
     row_factors(P.s, P.ct, P.lse, row, none, P.inv_tau, P.coef, P.lse2, P.ctmax);
 }
 
@@ -544,6 +581,8 @@ struct TeacherParams {
     int32_t top;
     float inv_tau;
     int32_t *out_ids;
+    uint16_t *start; // rows x (parts + 1)
+    int64_t parts;
     float *out_p, *plogp;
     float *coef, *lse2;
     uint32_t *status, *ctmax;
@@ -567,7 +606,7 @@ PSK_DEV float block_all(float x, float *red)
 
 static __global__ void __launch_bounds__(1024) k_head_teacher(const __grid_constant__ TeacherParams P)
 {
-    extern __shared__ int32_t list[]; // top ids
+    extern __shared__ int32_t list[]; // top ids as they come, then in order
     __shared__ float red[32];
     const int64_t row = blockIdx.x;
     const int j = threadIdx.x;
@@ -597,7 +636,10 @@ static __global__ void __launch_bounds__(1024) k_head_teacher(const __grid_const
         for (int i = 0; i < P.top; ++i) at += list[i] < id || (list[i] == id && i < j);
         P.out_ids[row * P.top + at] = id;
         P.out_p[row * P.top + at] = p;
+        list[P.top + at] = id;
     }
+    __syncthreads();
+    for (int64_t c = j; c <= P.parts; c += blockDim.x) P.start[row * (P.parts + 1) + c] = (uint16_t)lower_bound(list + P.top, P.top, c * COLS < 0x7fffffff ? (int32_t)(c * COLS) : 0x7fffffff);
     if (j == 0) {
         P.plogp[row] = sum;
         row_factors(P.s, P.ct, P.lse, row, none, P.inv_tau, P.coef, P.lse2, P.ctmax);
@@ -610,12 +652,12 @@ struct MaxParams {
     RowSpace s;
     RowOperand src;
     int64_t col_stride, cols;
-    const int32_t *label, *ids;
+    const int32_t *ids;
     int32_t top, vec; // vec: 16 bytes a load (contiguous, aligned, cols a multiple of a unit)
     uint32_t *out;
 };
 
-PSK_DEV bool no_target(const int32_t *label, const int32_t *ids, int top, int64_t row) { return label ? label[row] < 0 : ids ? ids[row * top] == 0x7fffffff : false; }
+PSK_DEV bool no_target(const int32_t *ids, int top, int64_t row) { return ids && ids[row * top] == 0x7fffffff; }
 
 PSK_DEV uint32_t finite_bits(float x)
 {
@@ -623,31 +665,39 @@ PSK_DEV uint32_t finite_bits(float x)
     return b < 0x7f800000u ? b : 0u;
 }
 
-static __global__ void __launch_bounds__(256) k_head_max(const __grid_constant__ MaxParams P)
+constexpr int PIECE = 1024; // columns of a row that a warp takes at a time
+
+template <bool F32>
+__global__ void __launch_bounds__(256) k_head_max(const __grid_constant__ MaxParams P)
 {
     __shared__ uint32_t red[8];
     const int lane = threadIdx.x & 31;
-    const int64_t warps = (int64_t)gridDim.x * 8;
+    const int64_t warps = (int64_t)gridDim.x * 8, pieces = (P.cols + PIECE - 1) / PIECE;
     uint32_t m = 0;
-    for (int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < P.s.rows; row += warps) {
-        if (no_target(P.label, P.ids, P.top, row)) continue;
+    for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < P.s.rows * pieces; i += warps) {
+        const int64_t row = i / pieces, c0 = (i - row * pieces) * PIECE, c1 = c0 + PIECE < P.cols ? c0 + PIECE : P.cols;
+        if (no_target(P.ids, P.top, row)) continue;
         const int64_t off = row_offset(P.s, P.src.stride, row);
         if (P.vec) {
-            const uint4 *q = reinterpret_cast<const uint4 *>((const uint8_t *)P.src.p + off * (P.src.dtype == PSK_F32 ? 4 : 2));
-            const int64_t n = P.cols * (P.src.dtype == PSK_F32 ? 4 : 2) / 16;
+            const uint4 *q = reinterpret_cast<const uint4 *>((const uint8_t *)P.src.p + (off + c0) * (F32 ? 4 : 2));
+            const int n = (int)(c1 - c0) / (F32 ? 4 : 8);
 #pragma unroll 4
-            for (int64_t i = lane; i < n; i += 32) {
-                const uint4 u = q[i];
+            for (int k = lane; k < n; k += 32) {
+                const uint4 u = q[k];
                 const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    if (P.src.dtype == PSK_F32) m = max(m, finite_bits(__uint_as_float(w[k])));
-                    else m = max(m, max(finite_bits(bf16_up(w[k] & 0xffffu)), finite_bits(bf16_up(w[k] >> 16)))); // bf16: the only 16-bit type that is scaled
+                for (int k2 = 0; k2 < 4; ++k2) {
+                    if (F32) m = max(m, finite_bits(__uint_as_float(w[k2])));
+                    else m = max(m, max(finite_bits(bf16_up(w[k2] & 0xffffu)), finite_bits(bf16_up(w[k2] >> 16)))); // bf16: the only 16-bit type that is scaled
                 }
             }
-        } else
-#pragma unroll 4
-            for (int64_t c = lane; c < P.cols; c += 32) m = max(m, finite_bits(load_real(P.src.p, P.src.dtype, off + c * P.col_stride)));
+        } else {
+            const int n = (int)(c1 - c0);
+            const int64_t cs = P.col_stride;
+            const void *src = (const uint8_t *)P.src.p + (off + c0 * cs) * (F32 ? 4 : 2);
+#pragma unroll 8
+            for (int c = lane; c < n; c += 32) m = max(m, finite_bits(F32 ? ((const float *)src)[c * cs] : bf16_up(((const uint16_t *)src)[c * cs])));
+        }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -659,33 +709,14 @@ static __global__ void __launch_bounds__(256) k_head_max(const __grid_constant__
     }
 }
 
-// 2^e as an f32, e within its normal range.
-PSK_DEV float pow2(int e) { return __uint_as_float((uint32_t)(127 + (e < -126 ? -126 : e > 127 ? 127 : e)) << 23); }
-
-// The exponent of the power of two that brings a maximum into [2^14, 2^15); 0 for none.
-PSK_DEV int scale_of(uint32_t max_bits)
-{
-    const int e = (int)(max_bits >> 23);
-    if (max_bits == 0) return 0;
-    const int k = 14 + 127 - (e == 0 ? 1 : e);
-    return k > 60 ? 60 : k; // 1/(g·w) and 1/(g·x) are f32 numbers then
-}
-
-// `has`: bit 0 x, bit 1 w, bit 2 g.
-static __global__ void k_head_scales(Scales *s, int has)
-{
-    const int x = has & 1 ? scale_of(s->max_x) : 0, w = has & 2 ? scale_of(s->max_w) : 0, g = has & 4 ? scale_of(s->max_ct) : 0;
-    s->x = pow2(x); s->w = pow2(w); s->g = pow2(g);
-    s->un_w = pow2(-w); s->un_dx = pow2(-g - w); s->un_dw = pow2(-g - x);
-}
-
-// The tiles' (m, z) of a row put together, and its loss. 32 rows a block, the half-tile columns over the block's y.
+// The parts' (m, z) of a row put together, and its loss. X neighbouring rows a block, 256 / X threads a row.
 struct JoinParams {
     RowSpace s;
-    int64_t halves; // parts of 128 columns
+    int64_t parts;
     const float2 *part;
-    const float *hit;
-    const int32_t *label, *ids;
+    const float *hit;   // rows x top
+    const int32_t *ids; // rows x top
+    const float *p;     // or null: labels
     const float *plogp;
     int32_t top;
     float c;      // log2 e / τ
@@ -695,66 +726,68 @@ struct JoinParams {
     int32_t guarded;
 };
 
-static __global__ void __launch_bounds__(256) k_head_join(const __grid_constant__ JoinParams P)
+template <int X>
+__global__ void __launch_bounds__(256) k_head_join(const __grid_constant__ JoinParams P)
 {
-    // a row's parts over 32 threads: four lanes of each of the eight warps; eight neighbouring rows a warp's load
-    __shared__ float sm[8][8], sz[8][8], sh[8][8];
-    const int x = threadIdx.x & 7, y = threadIdx.x >> 3, warp = threadIdx.x >> 5;
-    const int64_t row = (int64_t)blockIdx.x * 8 + x;
-    float m = -INFINITY, z = 0.0f, h = 0.0f;
+    constexpr int Y = 256 / X, AHEAD = 8;
+    __shared__ float sm[8][X], sz[8][X];
+    __shared__ double sh[8][X];
+    const int x = threadIdx.x % X, y = threadIdx.x / X, warp = threadIdx.x >> 5;
+    const int64_t row = (int64_t)blockIdx.x * X + x;
+    float m = -INFINITY, z = 0.0f;
+    double h = 0.0; // sum of p·l
     // (m, z) + (am, az) about the greater maximum; an empty part has m = -inf and z = 0
     auto join = [&](float am, float az) {
         const float g = fmaxf(m, am);
         if (!(g == -INFINITY)) z = __fadd_rn(__fmul_rn(z, exp2f(__fmul_rn(__fsub_rn(m, g), P.c))), __fmul_rn(az, exp2f(__fmul_rn(__fsub_rn(am, g), P.c))));
         m = g;
     };
-    if (row < P.s.rows)
-        for (int64_t th = y; th < P.halves; th += 32 * 8) {
-            float2 a[8];
-            float b[8];
+    if (row < P.s.rows) {
+        for (int64_t th = y; th < P.parts; th += Y * AHEAD) {
+            float2 a[AHEAD];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const bool in = th + 32 * k < P.halves;
-                const int64_t at = (th + 32 * k) * P.s.rows + row;
-                a[k] = in ? P.part[at] : make_float2(-INFINITY, 0.0f);
-                b[k] = in && !P.label ? P.hit[at] : 0.0f;
-            }
-            float g = a[0].x;
+            for (int k = 0; k < AHEAD; ++k) a[k] = th + Y * k < P.parts ? P.part[(th + Y * k) * P.s.rows + row] : make_float2(-INFINITY, 0.0f);
+            float g = a[0].x, s = 0.0f;
 #pragma unroll
-            for (int k = 1; k < 8; ++k) g = fmaxf(g, a[k].x);
-            float s = 0.0f;
+            for (int k = 1; k < AHEAD; ++k) g = fmaxf(g, a[k].x);
+            if (!(g == -INFINITY)) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                if (!(g == -INFINITY)) s = __fadd_rn(s, __fmul_rn(a[k].y, exp2f(__fmul_rn(__fsub_rn(a[k].x, g), P.c))));
-                h = __fadd_rn(h, b[k]);
+                for (int k = 0; k < AHEAD; ++k) s = __fadd_rn(s, __fmul_rn(a[k].y, exp2f(__fmul_rn(__fsub_rn(a[k].x, g), P.c))));
             }
             join(g, s);
         }
-#pragma unroll
-    for (int o = 8; o <= 16; o <<= 1) {
-        const float am = __shfl_xor_sync(0xffffffffu, m, o), az = __shfl_xor_sync(0xffffffffu, z, o);
-        h = __fadd_rn(h, __shfl_xor_sync(0xffffffffu, h, o));
-        join(am, az);
+        if (P.p)
+            for (int j = y; j < P.top; j += Y) {
+                const int64_t at = row * P.top + j;
+                if (P.ids[at] != 0x7fffffff) h += (double)P.p[at] * (double)P.hit[at];
+            }
     }
-    if ((threadIdx.x & 31) < 8) { sm[warp][x] = m; sz[warp][x] = z; sh[warp][x] = h; }
+    if (X < 32) {
+#pragma unroll
+        for (int o = X; o < 32; o <<= 1) {
+            const float am = __shfl_xor_sync(0xffffffffu, m, o), az = __shfl_xor_sync(0xffffffffu, z, o);
+            h += __shfl_xor_sync(0xffffffffu, h, o);
+            join(am, az);
+        }
+    }
+    if ((threadIdx.x & 31) < X) { sm[warp][x] = m; sz[warp][x] = z; sh[warp][x] = h; }
     __syncthreads();
-    if (threadIdx.x >= 8 || row >= P.s.rows) return;
+    if (threadIdx.x >= X || row >= P.s.rows) return;
+#pragma unroll
     for (int i = 1; i < 8; ++i) {
         join(sm[i][x], sz[i][x]);
-        h = __fadd_rn(h, sh[i][x]);
+        h += sh[i][x];
     }
-    const bool none = no_target(P.label, P.ids, P.top, row);
+    const bool none = no_target(P.ids, P.top, row);
     const double lse = (double)m * P.inv_tau + log((double)z);
-    double loss;
-    if (P.label) loss = lse - (double)P.hit[row];
-    else loss = (double)P.plogp[row] - (double)h * P.inv_tau + lse;
+    const double loss = P.p ? (double)P.plogp[row] - h * P.inv_tau + lse : lse - (double)P.hit[row];
     const uint32_t ovf = store_real(const_cast<void *>(P.loss.p), P.loss.dtype, row_offset(P.s, P.loss.stride, row), none ? 0.0f : (float)loss);
     if (P.lse.p) store_real(const_cast<void *>(P.lse.p), P.lse.dtype, row_offset(P.s, P.lse.stride, row), none ? 0.0f : (float)lse);
     if (P.guarded && ovf) atomicOr(P.ovf, 1u);
 }
 
 // A matrix laid out for the tensor maps: rows of `cols` elements from any strides into rows of `ld` (a multiple of 8),
-// the padding zeros, a warp a row and neighbouring lanes neighbouring elements (both sides whole lines whatever the
+// the padding zeros, a warp 1024 columns of a row and neighbouring lanes neighbouring elements (both sides whole lines whatever the
 // source's alignment). `to`: the same 16 bits; binary16 of bf16, scaled (exact); two binary16 planes of f32, scaled.
 // Rows without a target (of x) become zeros, so that nothing they hold reaches dw. `copies`: the rows again below
 // themselves (the second operand of a product over g and its remainder).
@@ -766,47 +799,115 @@ struct PackParams {
     int64_t col_stride, cols, ld, plane;
     uint16_t *dst;
     int32_t to, copies;
-    const float *scale; // of the whole matrix; or null
+    const uint32_t *max; // of the whole matrix, for its scale; or null
     float *un;          // PACK_SPLIT: scale every row by its own greatest element instead, and put the factor that undoes it here
-    const int32_t *label, *ids;
+    const int32_t *ids;
     int32_t top;
 };
 
-static __global__ void __launch_bounds__(256) k_head_pack(const __grid_constant__ PackParams P)
+template <int TO>
+PSK_DEV uint16_t packed(uint16_t w, float f)
+{
+    return TO == PACK_F16 ? (uint16_t)(pack_f16x2_hw(__fmul_rn(bf16_up(w), f), 0.0f) & 0xffffu) : w;
+}
+
+// An f32 number's two planes; an infinity or a NaN stays in the first.
+PSK_DEV uint32_t split_f16(float x)
+{
+    const uint32_t hi = pack_f16x2_hw(x, 0.0f) & 0xffffu;
+    const float r = __fsub_rn(x, f16_to_f32((uint16_t)hi));
+    return hi | (fabsf(r) < 65504.0f ? pack_f16x2_hw(r, 0.0f) << 16 : 0u);
+}
+
+// VEC: the source's rows contiguous and on 16-byte boundaries, cols = ld: eight elements a lane.
+template <int TO, bool VEC>
+__global__ void __launch_bounds__(256) k_head_pack(const __grid_constant__ PackParams P)
 {
     const int lane = threadIdx.x & 31;
-    const int64_t warps = (int64_t)gridDim.x * 8;
-    for (int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < P.s.rows; row += warps) {
-        const bool none = no_target(P.label, P.ids, P.top, row);
-        const int64_t off = row_offset(P.s, P.src.stride, row), cs = P.col_stride;
-        float f = P.scale ? *P.scale : 1.0f;
-        if (P.un) {
-            uint32_t m = 0;
-            if (!none)
-#pragma unroll 4
-                for (int64_t c = lane; c < P.cols; c += 32) m = max(m, finite_bits(((const float *)P.src.p)[off + c * cs]));
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-            const int e = scale_of(m);
-            f = pow2(e);
-            if (lane == 0) P.un[row] = pow2(-e);
-        }
-        uint16_t *dst = P.dst + row * P.ld;
-        const int64_t again = P.s.rows * P.ld;
+    const int64_t warps = (int64_t)gridDim.x * 8, width = P.un ? P.ld : PIECE, pieces = (P.ld + width - 1) / width, again = P.s.rows * P.ld;
+    const float whole = P.max ? pow2(scale_of(*P.max)) : 1.0f;
+    for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < P.s.rows * pieces; i += warps) {
+        const int64_t row = i / pieces, c0 = (i - row * pieces) * width;
+        const int n = (int)((P.ld - c0) < width ? P.ld - c0 : width);                                        // columns to write
+        const int live = no_target(P.ids, P.top, row) ? 0 : (int)((P.cols - c0) < n ? P.cols - c0 : n); // of which the matrix has
+        const int64_t cs = P.col_stride, off = row_offset(P.s, P.src.stride, row) + c0 * cs;
+        uint16_t *dst = P.dst + row * P.ld + c0;
+        if constexpr (TO == PACK_SPLIT) {
+            const float *src = (const float *)P.src.p + off;
+            float f = whole;
+            if (P.un) {
+                uint32_t m = 0;
 #pragma unroll 8
-        for (int64_t c = lane; c < P.ld; c += 32) {
-            const bool in = !none && c < P.cols;
-            if (P.to == PACK_SPLIT) {
-                const float x = in ? __fmul_rn(((const float *)P.src.p)[off + c * cs], f) : 0.0f;
-                const uint32_t hi = pack_f16x2_hw(x, 0.0f) & 0xffffu;
-                const float r = __fsub_rn(x, f16_to_f32((uint16_t)hi)); // an infinity or a NaN stays in its first plane
-                dst[c] = (uint16_t)hi;
-                dst[c + P.plane] = fabsf(r) < 65504.0f ? (uint16_t)(pack_f16x2_hw(r, 0.0f) & 0xffffu) : 0;
+                for (int c = lane; c < live; c += 32) m = max(m, finite_bits(src[c * cs]));
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+                const int e = scale_of(m);
+                f = pow2(e);
+                if (lane == 0) P.un[row] = pow2(-e);
+            }
+            if constexpr (VEC) {
+                for (int cb = lane * 4; cb < n; cb += 4 * 128) {
+                    float4 in[4]; // (all loads of a batch before its stores: the compiler cannot tell the buffers apart)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) in[k] = live && cb + k * 128 < n ? *reinterpret_cast<const float4 *>(src + cb + k * 128) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                    const int c = cb + k * 128;
+                    if (c >= n) break;
+                    const float4 x = in[k];
+                    const uint32_t w0 = split_f16(__fmul_rn(x.x, f)), w1 = split_f16(__fmul_rn(x.y, f)), w2 = split_f16(__fmul_rn(x.z, f)), w3 = split_f16(__fmul_rn(x.w, f));
+                    *reinterpret_cast<uint2 *>(dst + c) = make_uint2((w0 & 0xffffu) | w1 << 16, (w2 & 0xffffu) | w3 << 16);
+                    *reinterpret_cast<uint2 *>(dst + P.plane + c) = make_uint2(w0 >> 16 | (w1 & 0xffff0000u), w2 >> 16 | (w3 & 0xffff0000u));
+                    }
+                }
             } else {
-                uint16_t w = in ? ((const uint16_t *)P.src.p)[off + c * cs] : 0;
-                if (P.to == PACK_F16) w = (uint16_t)(pack_f16x2_hw(__fmul_rn(bf16_up(w), f), 0.0f) & 0xffffu);
-                dst[c] = w;
-                if (P.copies > 1) dst[c + again] = w;
+                for (int cb = lane; cb < n; cb += 8 * 32) {
+                    float in[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) in[k] = cb + k * 32 < live ? src[(cb + k * 32) * cs] : 0.0f;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int c = cb + k * 32;
+                        if (c >= n) break;
+                        const uint32_t w = split_f16(__fmul_rn(in[k], f));
+                        dst[c] = (uint16_t)w;
+                        dst[c + P.plane] = (uint16_t)(w >> 16);
+                    }
+                }
+            }
+        } else {
+            const uint16_t *src = (const uint16_t *)P.src.p + off;
+            if constexpr (VEC) {
+                uint4 in[PIECE / 256];
+#pragma unroll
+                for (int k = 0; k < PIECE / 256; ++k) in[k] = live && lane * 8 + k * 256 < n ? *reinterpret_cast<const uint4 *>(src + lane * 8 + k * 256) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+                for (int k4 = 0; k4 < PIECE / 256; ++k4) {
+                    const int c = lane * 8 + k4 * 256;
+                    if (c >= n) break;
+                    uint4 u = in[k4];
+                    if constexpr (TO == PACK_F16) {
+                        uint32_t *w = &u.x;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) w[k] = pack_f16x2_hw(__fmul_rn(bf16_up(w[k] & 0xffffu), whole), __fmul_rn(bf16_up(w[k] >> 16), whole));
+                    }
+                    *reinterpret_cast<uint4 *>(dst + c) = u;
+                    if (P.copies > 1) *reinterpret_cast<uint4 *>(dst + c + again) = u;
+                }
+            } else {
+                for (int cb = lane; cb < n; cb += 16 * 32) {
+                    uint16_t in[16];
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) in[k] = cb + k * 32 < live ? src[(cb + k * 32) * cs] : (uint16_t)0;
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        const int c = cb + k * 32;
+                        if (c >= n) break;
+                        const uint16_t w = packed<TO>(in[k], whole);
+                        dst[c] = w;
+                        if (P.copies > 1) dst[c + again] = w;
+                    }
+                }
             }
         }
     }
@@ -819,7 +920,7 @@ struct SumParams {
     const float *part;
     int64_t parts, part_rows, ld, fold, cols, col_stride; // ld: a multiple of 4
     const Scales *scales;
-    int32_t un; // 1: scales->un_dx, 2: scales->un_dw
+    int32_t un; // UN_DX, UN_DW
     RowOperand dst;
     uint32_t *ovf;
     int32_t guarded;
@@ -829,7 +930,7 @@ static __global__ void __launch_bounds__(256) k_head_sum(const __grid_constant__
 {
     const int64_t quads = (P.cols + 3) / 4, warps = (int64_t)gridDim.x * 8, chunks = (quads + 31) / 32;
     const int lane = threadIdx.x & 31;
-    const float un = !P.scales ? 1.0f : P.un == 1 ? P.scales->un_dx : P.scales->un_dw;
+    const float un = undo(P.scales, P.un);
     uint32_t ovf = 0;
     for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < P.s.rows * chunks; i += warps) {
         const int64_t row = i / chunks, c = ((i - row * chunks) * 32 + lane) * 4;
