@@ -53,17 +53,23 @@ struct Operand {
     int64_t plane;
 };
 
-bool map_of(HeadContext &x, CUtensorMap *map, const Operand &o, int f16, int box_rows)
+// The operand's tensor map for tiles of `box_rows` rows by 64 of the summed axis. Rows contiguous: 64 x 64 boxes, or
+// (`*blocks`) the rows in blocks of 64 as an axis of their own, so that a tile is one load; that takes a whole number of
+// blocks, since what lies in a last one beyond the rows would be read.
+bool map_of(HeadContext &x, CUtensorMap *map, const Operand &o, int f16, int box_rows, int32_t *blocks)
 {
-    const uint64_t inner = (uint64_t)(o.k_contiguous ? o.k : o.rows), outer = (uint64_t)(o.k_contiguous ? o.rows : o.k);
-    const uint64_t ld = (uint64_t)(outer == 1 ? up((int64_t)inner, 8) : o.ld); // one row: its stride is never walked
-    cuuint64_t dims[4] = {inner, outer, (cuuint64_t)o.planes, 1};
-    cuuint64_t strides[3] = {ld * 2, (cuuint64_t)(o.planes > 1 ? o.plane * 2 : ld * 2 * outer), 0};
-    strides[2] = strides[1] * (cuuint64_t)o.planes;
+    const int64_t outer = o.k_contiguous ? o.rows : o.k, inner = o.k_contiguous ? o.k : o.rows;
+    const int64_t ld = outer == 1 ? up(inner, 8) : o.ld, plane = o.planes > 1 ? o.plane : ld * outer; // one row: its stride is never walked
+    *blocks = !o.k_contiguous && o.rows % 64 == 0;
+    cuuint64_t dims[4] = {(cuuint64_t)inner, (cuuint64_t)outer, (cuuint64_t)o.planes, 1}, strides[3] = {(cuuint64_t)ld * 2, (cuuint64_t)plane * 2, (cuuint64_t)plane * 2 * o.planes};
+    cuuint32_t box[4] = {(cuuint32_t)BK, (cuuint32_t)(o.k_contiguous ? box_rows : BK), 1, 1}, estr[4] = {1, 1, 1, 1};
+    if (*blocks) {
+        dims[0] = 64; dims[2] = (cuuint64_t)(o.rows / 64); dims[3] = (cuuint64_t)o.planes;
+        strides[1] = 128; strides[2] = (cuuint64_t)plane * 2;
+        box[2] = (cuuint32_t)(box_rows / 64);
+    }
     for (int i = 0; i < 3; ++i)
         if (strides[i] % 16 != 0 || strides[i] == 0) return false;
-    cuuint32_t box[4] = {(cuuint32_t)BK, (cuuint32_t)(o.k_contiguous ? box_rows : BK), 1, 1};
-    cuuint32_t estr[4] = {1, 1, 1, 1};
     return x.encode(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(o.p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -80,35 +86,77 @@ int fail(HeadContext &x, int code, const std::string &msg)
         if (err__ != cudaSuccess) return fail(x, PSK_E10001, std::string(#call) + ": " + cudaGetErrorString(err__)); \
     } while (0)
 
-template <int MODE, int MT = 1, bool REST = false>
+// How many clusters of two CTAs of a kernel the device holds at a time (SMs that no pair fits stay idle); 0: none.
+template <class K>
+int pairs_of(K kernel, const HeadContext &x)
+{
+    cudaLaunchConfig_t c;
+    memset(&c, 0, sizeof c);
+    c.gridDim = dim3((unsigned)(x.sms / 2 * 2)); c.blockDim = dim3(THREADS); c.dynamicSmemBytes = Cfg::SMEM_TOTAL;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = 2; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    c.attrs = at; c.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &c) != cudaSuccess) { cudaGetLastError(); n = 0; }
+    return n;
+}
+
+template <int MODE, bool REST, bool PAIR>
+int launch(HeadContext &x, const CUtensorMap &ma, const CUtensorMap &mb, const Params &P)
+{
+    // once a device: the kernel's shared memory, and how many pairs fit (bits 0: set; the rest the number)
+    static std::atomic<int> known[64];
+    int device = 0;
+    HEAD_TRY(cudaGetDevice(&device));
+    int k = device < 64 ? known[device].load(std::memory_order_relaxed) : 0;
+    if (!k) {
+        HEAD_TRY(cudaFuncSetAttribute(k_head<MODE, PAIR, REST>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_TOTAL));
+        k = 1 + 2 * (PAIR ? pairs_of(k_head<MODE, PAIR, REST>, x) : 0);
+        if (device < 64) known[device].store(k, std::memory_order_relaxed);
+    }
+    const int64_t tiles = P.tiles_m * P.tiles_n * P.splits;
+    if (PAIR) {
+        if (k >> 1 < 1) return fail(x, PSK_E10001, "head: no pair of SMs for a cluster");
+        cudaLaunchConfig_t c;
+        memset(&c, 0, sizeof c);
+        c.gridDim = dim3((unsigned)(2 * std::min<int64_t>(tiles, k >> 1))); c.blockDim = dim3(THREADS); c.dynamicSmemBytes = Cfg::SMEM_TOTAL; c.stream = x.stream;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = 2; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+        c.attrs = at; c.numAttrs = 1;
+        HEAD_TRY(cudaLaunchKernelEx(&c, k_head<MODE, PAIR, REST>, ma, mb, P));
+    } else k_head<MODE, PAIR, REST><<<(unsigned)std::min<int64_t>(tiles, x.sms), THREADS, Cfg::SMEM_TOTAL, x.stream>>>(ma, mb, P);
+    x.kernels += 1;
+    return PSK_OK;
+}
+
+// One product a·bᵀ and what MODE makes of it.
+template <int MODE, bool REST = false>
 int product(HeadContext &x, Params P, const Operand &a, const Operand &b, int f16)
 {
-    CUtensorMap ma, mb;
-    if (!map_of(x, &ma, a, f16, BM * MT) || !map_of(x, &mb, b, f16, BN)) return fail(x, PSK_E10001, "head: an operand's layout does not make a tensor map");
     P.m = a.rows; P.n = b.rows;
-    P.tiles_m = (P.m + BM * MT - 1) / (BM * MT); P.tiles_n = (P.n + BN - 1) / BN;
+    const int64_t tiles = ((P.m + BM - 1) / BM) * ((P.n + BN - 1) / BN);
+    // pairs of CTAs where there are rows for two and tiles for everybody (see Cfg)
+    const bool pair = P.m > BM && tiles >= x.sms;
+    P.tiles_m = (P.m + (pair ? 2 : 1) * BM - 1) / ((pair ? 2 : 1) * BM); P.tiles_n = (P.n + BN - 1) / BN;
+    const int a_rows = !pair && a.k_contiguous ? (int)std::min<int64_t>(BM, up(P.m, 8)) : BM;
+    P.a_stage = a_rows * BK * 2;
+    P.stages = Cfg::stages(P.a_stage, (pair ? BN / 2 : BN) * BK * 2, MODE != MODE_STATS);
+    CUtensorMap ma, mb;
+    if (!map_of(x, &ma, a, f16, a_rows, &P.a_blocks) || !map_of(x, &mb, b, f16, pair ? BN / 2 : BN, &P.b_blocks)) return fail(x, PSK_E10001, "head: an operand's layout does not make a tensor map");
     P.kb_k = (int32_t)((a.k + BK - 1) / BK);
     P.nprod = a.planes == 2 ? 3 : 1;
     if (MODE != MODE_OUT) { P.splits = 1; P.kb_split = P.kb_k; }
     // Steps an accumulator: 512 products of the summed axis (384 of f32's, three a block). Results of 16 bits, dx and dw, keep one
     // accumulator throughout, and g's logits 1024 products: what truncation loses there is far below their rounding.
-    P.chunk = MODE == MODE_OUT && P.out_dtype != PSK_F32 ? 1 << 28 : P.nprod == 3 ? 6 : MODE == MODE_GRAD ? 16 : 8;
-    // a panel's columns of b stay in a quarter of the L2 while a's rows stream past them
+    P.chunk = MODE == MODE_OUT && a.planes == 1 ? 1 << 28 : P.nprod == 3 ? 6 : MODE == MODE_GRAD ? 16 : 8;
+    // a panel's columns of b stay in a part of the L2 while a's rows stream past them
     P.panel = std::min<int64_t>(P.tiles_n, std::max<int64_t>(8, (16ll << 20) / std::max<int64_t>(1, BN * a.k * 2 * a.planes)));
     P.in_f16 = f16; P.a_m_major = !a.k_contiguous; P.b_n_major = !b.k_contiguous;
     P.status = x.status;
-    static std::atomic<uint64_t> set{0}; // devices whose copy of this kernel has its shared memory allowed
-    int device = 0;
-    HEAD_TRY(cudaGetDevice(&device));
-    if (device >= 64 || !(set.load(std::memory_order_relaxed) >> device & 1)) {
-        HEAD_TRY(cudaFuncSetAttribute(k_head<MODE, MT, REST>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<MT>::SMEM_TOTAL));
-        if (device < 64) set.fetch_or(1ull << device, std::memory_order_relaxed);
-    }
-    const int64_t tiles = P.tiles_m * P.tiles_n * P.splits;
-    k_head<MODE, MT, REST><<<(unsigned)std::min<int64_t>(tiles, x.sms), THREADS, Cfg<MT>::SMEM_TOTAL, x.stream>>>(ma, mb, P);
-    x.kernels += 1;
     x.flops += 2.0 * (double)P.m * (double)P.n * (double)a.k;
-    return PSK_OK;
+    return pair ? launch<MODE, REST, true>(x, ma, mb, P) : launch<MODE, REST, false>(x, ma, mb, P);
 }
 
 // Blocks of eight warps for `work` warps' worth.
@@ -212,11 +260,10 @@ int head_run(HeadContext &x, const psk_launch *l, void *const *table)
 
     // Where dx and dw are stored from: straight from the products where one launch has the whole sum and the result's
     // rows are one level; otherwise through f32 sums (k_head_sum).
-    struct Out { int64_t m, n, ld, splits; int32_t kb_split; bool straight, two; };
+    struct Out { int64_t m, n, ld, splits; int32_t kb_split; bool straight; };
     auto plan = [&](int64_t m, int64_t n, int64_t k, bool may_be_straight) {
-        Out o{m, n, up(n, 4), 1, 0, may_be_straight, false};
+        Out o{m, n, up(n, 4), 1, 0, may_be_straight};
         const int64_t kb = (k + BK - 1) / BK, tiles = ((m + BM - 1) / BM) * ((n + BN - 1) / BN);
-        o.two = !f32 && m >= 2 * BM && tiles >= 2 * x.sms;
         // few tiles: cut the summed axis, so that every SM has some of it
         const int64_t want = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(x.sms / tiles, 32), kb / 4));
         o.kb_split = (int32_t)((kb + want - 1) / want);
@@ -339,7 +386,7 @@ int head_run(HeadContext &x, const psk_launch *l, void *const *table)
             continue;
         }
         P.lse2 = lse2; P.coef = coef; P.g = g; P.g_f16 = g_f16; P.g_ld = g_ld; P.g_rest = N * g_ld;
-        int r = rest || f32 ? product<MODE_GRAD, 1, true>(x, P, a, b, in_f16) : product<MODE_GRAD>(x, P, a, b, in_f16);
+        int r = rest || f32 ? product<MODE_GRAD, true>(x, P, a, b, in_f16) : product<MODE_GRAD>(x, P, a, b, in_f16);
         if (r != PSK_OK) return r;
         // 6. dx = g·wᵀ summed over the pieces: both operands along the classes
         const Operand bd = conv ? pack_w(wd, PACK_F16, &scales->max_w) : b;
@@ -353,7 +400,7 @@ int head_run(HeadContext &x, const psk_launch *l, void *const *table)
         Q.out_vec = !dxo.straight || (aligned(rout.p) && dx_ld * eb % 16 == 0 && D * eb % 16 == 0);
         Q.ovf = x.guarded && dxo.straight ? x.ovf : nullptr;
         const Operand gk{g, Ng, vn, g_ld, true, planes, N * g_ld}, wk{bd.p, D, vn, bd.ld, v_inner, planes, bd.plane};
-        r = dxo.two ? product<MODE_OUT, 2>(x, Q, gk, wk, g_f16) : product<MODE_OUT>(x, Q, gk, wk, g_f16);
+        r = product<MODE_OUT>(x, Q, gk, wk, g_f16);
         if (r != PSK_OK) return r;
         // 7. dw of the piece = xᵀ·g: both operands along the rows
         if (DW) {
@@ -367,7 +414,7 @@ int head_run(HeadContext &x, const psk_launch *l, void *const *table)
             Q.un = dwo.straight ? UN_DW : UN_NONE;
             Q.out_vec = !dwo.straight || (aligned(dst) && dw_ld * eb % 16 == 0 && cols * eb % 16 == 0);
             Q.ovf = x.guarded && dwo.straight ? x.ovf : nullptr;
-            r = dwo.two ? product<MODE_OUT, 2>(x, Q, dw_v_inner ? xr : gr, dw_v_inner ? gr : xr, g_f16) : product<MODE_OUT>(x, Q, dw_v_inner ? xr : gr, dw_v_inner ? gr : xr, g_f16);
+            r = product<MODE_OUT>(x, Q, dw_v_inner ? xr : gr, dw_v_inner ? gr : xr, g_f16);
             if (r != PSK_OK) return r;
             if (!dwo.straight) {
                 SumParams S;

@@ -2,7 +2,7 @@
 // PSK_OP_HEAD_DISTILL and their _VJP): the logits l = x·w exist only as accumulators in tensor memory and registers.
 //
 // Forward. One pass over the vocabulary: a tile of 128 rows by 256 classes is multiplied on the tensor cores, and its
-// epilogue reduces each row's 128 columns a thread to a maximum m and z = sum of 2^((l - m)·c), c = log2 e / τ, which
+// epilogue reduces each row's 64 columns a thread to a maximum m and z = sum of 2^((l - m)·c), c = log2 e / τ, which
 // k_head_join puts together over the tiles: ln sum exp(l / τ) = M / τ + ln sum z·2^((m - M)·c).
 // The targets' logits are picked out of the same registers. Backward. The tile is multiplied again, the epilogue
 // writes g = ct/τ (2^(l·c - lse) - p) of a piece of the vocabulary, and two more products give dx and dw from it.
@@ -22,29 +22,37 @@
 #pragma once
 #include <utility>
 #include "psk_dev.cuh"
-#include "psk_gemm_tc.cuh"
+#include "psk_pair.cuh"
 
 namespace psk {
 namespace head {
 
 constexpr int BM = 128, BN = 256, BK = 64;
-// Three warpgroups: warp 0 issues the TMA loads, warp 1 the products (2 and 3 idle); warps 4 to 11 are the epilogue, two
-// a quadrant of tensor memory, 128 columns each. An epilogue thread keeps its 128 sums in registers, so the first
-// warpgroup gives most of its share up: 128·40 + 256·232 = 384·168, what the block is launched with.
-constexpr int THREADS = 384;
-constexpr int REGS_FEW = 40, REGS_MANY = 232, REGS_LAUNCH = 168;
-static_assert(128 * REGS_FEW + 256 * REGS_MANY <= THREADS * REGS_LAUNCH, "setmaxnreg waits for registers that the block does not have");
-// MT: 128-row halves of a CTA's tile. One, with the two accumulators taking turns, for sums kept in registers; two,
-// both multiplying the same tile of b (a third fewer bytes from the L2 a product), for the plain products dx and dw.
-template <int MT>
+// Five warpgroups: warps 0 and 2 issue the TMA loads, warp 1 the products (3 is idle); warps 4 to 19 are the epilogue, four
+// a quadrant of tensor memory, 64 columns each. Eight warps of 128 columns had too little to issue from (an instruction
+// every six cycles a warp, half the rate of the tiles of a model of 216). An epilogue thread keeps its 64 sums in
+// registers, so the first warpgroup gives up most of its share: 128·32 + 512·112 = 640·96, what the block is launched with.
+constexpr int EPILOGUE = 16, THREADS = 128 + 32 * EPILOGUE;
+constexpr int REGS_FEW = 32, REGS_MANY = 112, REGS_LAUNCH = 96;
+static_assert(128 * REGS_FEW + 32 * EPILOGUE * REGS_MANY <= THREADS * REGS_LAUNCH, "setmaxnreg waits for registers that the block does not have");
+// A tile is 128 rows by 256 columns a CTA. Two forms:
+//   PAIR   two CTAs of a cluster compute 256 x 256: each loads its own 128 rows of a and one half of b's columns, and
+//          the products (cta_group::2) read either half from either SM. What a CTA takes from the L2 a block of 64 of
+//          the summed axis is 32 KB where it is 48 alone; at 16 to 17 TB/s the L2 is what bounds the single form.
+//   single for few rows (up to 128: there b's bytes from memory are the bound) and few tiles.
 struct Cfg {
-    static constexpr int STAGES = MT == 1 ? 4 : 3;
-    static constexpr int A_BYTES = MT * BM * BK * 2, B_BYTES = BN * BK * 2;
-    static constexpr int TILE_BYTES = STAGES * (A_BYTES + B_BYTES);
-    static constexpr int STAGE_OUT = 8 * 32 * 128;
-    static constexpr int SMEM_TOTAL = TILE_BYTES + 256 + STAGE_OUT + 1024;
+    static constexpr int A_BYTES = BM * BK * 2, BARS = 256, MOST_STAGES = 8;
+    static constexpr int SMEM_TOTAL = 227 * 1024;
+    // Stages of the ring. With few rows the copy of a's tile takes as many rows as there are (a multiple of 8, a swizzle
+    // atom): the products read 128 all the same, of whatever lies behind, which makes rows of the result that
+    // nobody reads, and the room goes to more stages of b, whose bytes are then what bounds the kernel.
+    static int stages(int a_stage, int b_stage, bool staged)
+    {
+        const int n = (SMEM_TOTAL - 1024 - BARS - (staged ? EPILOGUE * 32 * 64 : 0)) / (a_stage + b_stage);
+        return n < MOST_STAGES ? n : MOST_STAGES;
+    }
 };
-constexpr int COLS = 128; // columns of a tile an epilogue thread holds
+constexpr int COLS = 64; // columns of a tile an epilogue thread holds: a part of the vocabulary
 
 enum { MODE_STATS = 0, MODE_GRAD = 1, MODE_OUT = 2 };
 
@@ -83,6 +91,8 @@ struct Params {
     int32_t kb_split;             // blocks of the summed axis a split
     int32_t chunk;                // steps (block, partial product) in one accumulator before it is added into registers
     int32_t in_f16, a_m_major, b_n_major;
+    int32_t stages, a_stage;      // of the ring; bytes of a's tile in one
+    int32_t a_blocks, b_blocks;   // a map over (64, k, rows / 64, plane): a tile of an operand with contiguous rows is one load
     uint32_t *status;
     const Scales *scales;         // or null: every factor 1
     int32_t logits_scaled;        // the operands of the logits are
@@ -93,9 +103,9 @@ struct Params {
     int64_t col0;                 // the class of column 0: where the piece begins
     const int32_t *ids;           // rows x top classes in ascending order, absent entries last as 0x7fffffff
     const float *p;               // their weights; or null: 1 (labels)
-    const uint16_t *start;        // rows x (parts + 1): a row's first entry of each 128 classes; or null: one entry a row
+    const uint16_t *start;        // rows x (parts + 1): a row's first entry of each part; or null: one entry a row
     int32_t top;
-    int64_t parts;                // 128-class parts of the vocabulary
+    int64_t parts;                // of the vocabulary, 64 classes each
     // MODE_STATS
     float2 *part;                 // [part][row]: (max, sum of 2^((l - max)·c))
     float *hit;                   // rows x top: the entries' logits
@@ -136,17 +146,59 @@ PSK_DEV void take(float &v, int y, float amount)
 {
     asm("{\n\t.reg .pred p;\n\tsetp.eq.s32 p, %1, %2;\n\t@p sub.rn.f32 %0, %0, %3;\n\t}" : "+f"(v) : "r"(y), "n"(I), "f"(amount));
 }
-template <int G, int... I>
-PSK_DEV void pick_column(float &l, int y, const float (&v)[COLS], std::integer_sequence<int, I...> s)
+template <int G, int N, int... I>
+PSK_DEV void pick_column(float &l, int y, const float (&v)[N], std::integer_sequence<int, I...> s)
 {
     if (y >> 4 == G) (pick<G * 16 + I>(l, y, v[G * 16 + I]), ...);
-    if constexpr (G + 1 < COLS / 16) pick_column<G + 1>(l, y, v, s);
+    if constexpr (G + 1 < N / 16) pick_column<G + 1>(l, y, v, s);
 }
-template <int G, int... I>
-PSK_DEV void take_column(float (&v)[COLS], int y, float amount, std::integer_sequence<int, I...> s)
+template <int G, int N, int... I>
+PSK_DEV void take_column(float (&v)[N], int y, float amount, std::integer_sequence<int, I...> s)
 {
     if (y >> 4 == G) (take<G * 16 + I>(v[G * 16 + I], y, amount), ...);
-    if constexpr (G + 1 < COLS / 16) take_column<G + 1>(v, y, amount, s);
+    if constexpr (G + 1 < N / 16) take_column<G + 1>(v, y, amount, s);
+}
+using Sixteen = std::make_integer_sequence<int, 16>;
+
+// Sixteen words of g, two numbers each, and what their rounding leaves.
+template <bool REST, int FROM>
+PSK_DEV void pack_g(bool f16, uint32_t (&w)[16], uint32_t (&rest)[16], const float (&u)[COLS])
+{
+    if (f16) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w[i] = pack_f16x2_hw(u[FROM + 2 * i], u[FROM + 2 * i + 1]);
+        if constexpr (REST) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) rest[i] = pack_f16x2_hw(__fsub_rn(u[FROM + 2 * i], f16_to_f32((uint16_t)(w[i] & 0xffffu))), __fsub_rn(u[FROM + 2 * i + 1], f16_to_f32((uint16_t)(w[i] >> 16))));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w[i] = pack_bf16x2_hw(u[FROM + 2 * i], u[FROM + 2 * i + 1]);
+        if constexpr (REST) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) rest[i] = pack_bf16x2_hw(__fsub_rn(u[FROM + 2 * i], bf16_up(w[i] & 0xffffu)), __fsub_rn(u[FROM + 2 * i + 1], bf16_up(w[i] >> 16)));
+        }
+    }
+}
+
+// A wait that is over at once costs a test; only another reads the clock (tc::mbar_wait, bounded).
+PSK_DEV bool wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, uint32_t *status, uint32_t where)
+{
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok || tc::mbar_wait(bar, parity, abort_flag, status, where);
+}
+
+// One matrix instruction, its descriptors as low words (the address, which alone changes from step to step) and high ones.
+template <bool PAIR>
+PSK_DEV void umma(uint32_t acc, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t add)
+{
+    if (PAIR)
+        asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\tsetp.ne.b32 p, %6, 0;\n\t"
+                     "tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %5, p;\n\t}" ::"r"(acc), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(add) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\tsetp.ne.b32 p, %6, 0;\n\t"
+                     "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n\t}" ::"r"(acc), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(add) : "memory");
 }
 
 // First entry of a row's ascending list that is at least `c`.
@@ -161,21 +213,21 @@ PSK_DEV int lower_bound(const int32_t *ids, int n, int32_t c)
     return lo;
 }
 
-// 128 bytes of each of this warp's 32 rows: from the threads' packed words through a staging tile (16-byte units
-// swizzled by the row), so that a store instruction writes whole lines (8 lanes a row, 4 rows an instruction).
-// `bytes`: how many of the 128 lie inside the matrix, a multiple of 16.
+// 64 bytes of each of this warp's 32 rows: from the threads' packed words through a staging tile (16-byte units
+// swizzled by the row), so that a store instruction writes whole sectors (4 lanes a row, 8 rows an instruction).
+// `bytes`: how many of the 64 lie inside the matrix, a multiple of 16.
 template <bool ADD>
-PSK_DEV void store_rows(uint4 *stage, int lane, const uint32_t (&w)[32], uint8_t *base, int64_t ld_bytes, int rows_live, int bytes)
+PSK_DEV void store_rows(uint4 *stage, int lane, const uint32_t (&w)[16], uint8_t *base, int64_t ld_bytes, int rows_live, int bytes)
 {
 #pragma unroll
-    for (int q = 0; q < 8; ++q) stage[lane * 8 + (q ^ (lane & 7))] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+    for (int q = 0; q < 4; ++q) stage[lane * 4 + (q ^ ((lane >> 1) & 3))] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
     __syncwarp();
-    const int unit = lane & 7;
+    const int unit = lane & 3;
 #pragma unroll
-    for (int it = 0; it < 8; ++it) {
-        const int rr = it * 4 + (lane >> 3);
+    for (int it = 0; it < 4; ++it) {
+        const int rr = it * 8 + (lane >> 2);
         if (rr < rows_live && unit * 16 < bytes) {
-            uint4 v = stage[rr * 8 + (unit ^ (rr & 7))];
+            uint4 v = stage[rr * 4 + (unit ^ ((rr >> 1) & 3))];
             uint4 *dst = reinterpret_cast<uint4 *>(base + rr * ld_bytes + unit * 16);
             if (ADD) {
                 const uint4 o = *dst;
@@ -190,57 +242,67 @@ PSK_DEV void store_rows(uint4 *stage, int lane, const uint32_t (&w)[32], uint8_t
 
 // The same where rows begin at any element: the lanes write neighbouring elements (T: 16 or 32 bits) of one row.
 template <class T>
-PSK_DEV void store_rows_any(uint4 *stage, int lane, const uint32_t (&w)[32], uint8_t *base, int64_t ld_bytes, int rows_live, int bytes)
+PSK_DEV void store_rows_any(uint4 *stage, int lane, const uint32_t (&w)[16], uint8_t *base, int64_t ld_bytes, int rows_live, int bytes)
 {
 #pragma unroll
-    for (int q = 0; q < 8; ++q) stage[lane * 8 + (q ^ (lane & 7))] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+    for (int q = 0; q < 4; ++q) stage[lane * 4 + (q ^ ((lane >> 1) & 3))] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
     __syncwarp();
-    constexpr int PER = 16 / sizeof(T);
+    constexpr int PER = 16 / sizeof(T), EACH = 64 / sizeof(T), ROWS = 32 / EACH; // elements a unit, a row; rows an instruction
+    const int e = lane % EACH;
 #pragma unroll 4
-    for (int rr = 0; rr < rows_live; ++rr) {
-        T *dst = reinterpret_cast<T *>(base + rr * ld_bytes);
-        const T *src = reinterpret_cast<const T *>(stage + rr * 8);
-#pragma unroll
-        for (int e = lane; e < 128 / (int)sizeof(T); e += 32)
-            if (e * (int)sizeof(T) < bytes) dst[e] = src[((e / PER) ^ (rr & 7)) * PER + e % PER];
+    for (int r = lane / EACH; r < rows_live; r += ROWS) {
+        const T *src = reinterpret_cast<const T *>(stage + r * 4);
+        if (e * (int)sizeof(T) < bytes) reinterpret_cast<T *>(base + r * ld_bytes)[e] = src[((e / PER) ^ ((r >> 1) & 3)) * PER + e % PER];
     }
     __syncwarp();
 }
 
 // The product of a persistent CTA's tiles, and what MODE makes of it. Bounds: the tensor pipe (2·m·n·k flops) for many
 // rows; for few, the bytes of the second operand.
-template <int MODE, int MT = 1, bool REST = false>
+template <int MODE, bool PAIR, bool REST = false>
 __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ Params P)
 {
-    static_assert(MT == 1 || MODE == MODE_OUT, "two halves leave no second accumulator to sum in parts with");
-    constexpr int STAGES = Cfg<MT>::STAGES, A_BYTES = Cfg<MT>::A_BYTES, B_BYTES = Cfg<MT>::B_BYTES, TILE_BYTES = Cfg<MT>::TILE_BYTES;
+    constexpr int B_BYTES = (PAIR ? BN / 2 : BN) * BK * 2, MOST = Cfg::MOST_STAGES, STAGE_OUT = MODE == MODE_STATS ? 0 : EPILOGUE * 32 * 64;
+    const int STAGES = P.stages, A_BYTES = P.a_stage;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    uint8_t *smem_a = smem, *smem_b = smem + STAGES * A_BYTES;
-    uint64_t *bars = (uint64_t *)(smem + TILE_BYTES);
-    // full[STAGES], empty[STAGES], accumulator full[2], accumulator empty[2]
-    uint32_t *tmem_slot = (uint32_t *)(bars + 2 * STAGES + 4);
+    // a's ring before b's: a short tile of a is read past its end, into what lies behind
+    uint8_t *smem_a = smem + STAGE_OUT, *smem_b = smem_a + STAGES * A_BYTES;
+    uint64_t *bars = (uint64_t *)(smem_b + STAGES * B_BYTES);
+    // full[MOST] (of a pair: the leader's, which counts both CTAs' loads), empty[MOST], accumulator full[2], empty[2]
+    // (of a pair: the leader's, which issues the products)
+    uint32_t *tmem_slot = (uint32_t *)(bars + 2 * MOST + 4);
     volatile int *abort_flag = (volatile int *)(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t full0 = tc::smem_u32(bars), empty0 = tc::smem_u32(bars + STAGES);
-    const uint32_t tfull0 = tc::smem_u32(bars + 2 * STAGES), tempty0 = tc::smem_u32(bars + 2 * STAGES + 2);
+    const uint32_t full0 = tc::smem_u32(bars), empty0 = tc::smem_u32(bars + MOST);
+    const uint32_t tfull0 = tc::smem_u32(bars + 2 * MOST), tempty0 = tc::smem_u32(bars + 2 * MOST + 2);
+    const uint32_t rank = PAIR ? tc2::cluster_rank() : 0u;
 
     if (threadIdx.x == 0) {
         *abort_flag = 0;
         for (int s = 0; s < STAGES; ++s) { tc::mbar_init(full0 + 8 * s, 1); tc::mbar_init(empty0 + 8 * s, 1); }
-        for (int s = 0; s < 2; ++s) { tc::mbar_init(tfull0 + 8 * s, 1); tc::mbar_init(tempty0 + 8 * s, 8); }
+        for (int s = 0; s < 2; ++s) { tc::mbar_init(tfull0 + 8 * s, 1); tc::mbar_init(tempty0 + 8 * s, PAIR ? 2 * EPILOGUE : EPILOGUE); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (PAIR) __syncthreads();
+    if (PAIR) tc2::cluster_sync(); // the peer is there, its barriers initialised
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(tmem_slot)), "r"(2 * BN) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(tmem_slot)), "r"(2 * BN) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(tmem_slot)), "r"(2 * BN) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if (PAIR) tc2::cluster_sync(); // both have their tensor memory before a product writes either
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem_base = *tmem_slot;
 
     const int64_t per_split = P.tiles_m * P.tiles_n, total = per_split * P.splits;
+    const int64_t tile0 = PAIR ? blockIdx.x >> 1 : blockIdx.x, tile_step = PAIR ? gridDim.x >> 1 : gridDim.x;
     // the steps of a split: blocks kb_first .. of the summed axis, nprod partial products each
     auto steps_of = [&](int64_t sp, int &kb_first) {
         kb_first = (int)sp * P.kb_split;
@@ -250,96 +312,100 @@ __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ CUt
 
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_FEW));
-        if (warp == 0 && lane == 0) {
+        // These three threads are what the tensor cores wait for: a stage's four products take 512 cycles, and a thread
+        // alone issues an instruction every five or so. So all that can be is kept out of the loops over the steps (with a
+        // descriptor put together for every product the pipe stood still 40 % of the time).
+        if ((warp == 0 || warp == 2) && lane == 0) { // warp 0 a's tiles, warp 2 b's
+            const bool of_a = warp == 0;
             uint32_t stage = 0, phase = 0;
             bool ok = true;
-            for (int64_t t = blockIdx.x; t < total && ok; t += gridDim.x) {
+            const CUtensorMap *map = of_a ? &map_a : &map_b;
+            const uint32_t dst0 = tc::smem_u32(of_a ? smem_a : smem_b), dst_step = of_a ? (uint32_t)A_BYTES : (uint32_t)B_BYTES;
+            const uint32_t full_at = PAIR ? tc2::map_to_rank(full0, 0) : full0, bytes = (PAIR ? 2 : 1) * (A_BYTES + B_BYTES), nprod = P.nprod;
+            const bool counts = of_a && (!PAIR || rank == 0), blocks = (of_a ? P.a_blocks : P.b_blocks) != 0;
+            const int boxes = (of_a ? P.a_m_major : P.b_n_major) && !blocks ? (int)(dst_step / 8192) : 0; // 64 x 64 each; 0: one load
+            const bool k_first = !(of_a ? P.a_m_major : P.b_n_major);
+            auto load = [&](uint32_t dst, uint32_t bar, int c0, int c1, int c2, int c3) {
+                if (PAIR) tc2::tma_load_4d_pair(dst, map, bar, c0, c1, c2, c3);
+                else tc::tma_load_4d(dst, map, bar, c0, c1, c2, c3);
+            };
+            for (int64_t t = tile0; t < total && ok; t += tile_step) {
                 int64_t mt, nt;
                 tc::tile_of(t % per_split, P.tiles_m, P.tiles_n, P.panel, mt, nt);
-                const int m0 = (int)mt * BM * MT, n0 = (int)nt * BN;
+                const int r0 = of_a ? (int)(PAIR ? mt * 2 + rank : mt) * BM : (int)nt * BN + (PAIR ? (int)rank * (BN / 2) : 0);
                 int kb0;
                 const int steps = steps_of(t / per_split, kb0);
-                int kb = kb0, q = 0;
+                int k0 = kb0 * BK, plane = 0;
+                uint32_t q = 0;
                 for (int s = 0; s < steps; ++s) {
-                    ok = tc::mbar_wait(empty0 + 8 * stage, phase ^ 1u, abort_flag, P.status, 1u);
+                    ok = wait(empty0 + 8 * stage, phase ^ 1u, abort_flag, P.status, 1u);
                     if (!ok) break;
-                    const uint32_t fb = full0 + 8 * stage;
-                    tc::mbar_expect_tx(fb, A_BYTES + B_BYTES);
-                    const int k0 = kb * BK, pa = P.nprod == 1 ? 0 : plane_a(q), pb = P.nprod == 1 ? 0 : plane_b(q);
-                    const uint32_t sa = tc::smem_u32(smem_a + stage * A_BYTES), sb = tc::smem_u32(smem_b + stage * B_BYTES);
-                    if (!P.a_m_major) tc::tma_load_4d(sa, &map_a, fb, k0, m0, pa, 0);
+                    const uint32_t dst = dst0 + stage * dst_step, fb = full_at + 8 * stage;
+                    if (counts) tc::mbar_expect_tx(full0 + 8 * stage, bytes);
+                    if (k_first) load(dst, fb, k0, r0, plane, 0);
+                    else if (blocks) load(dst, fb, 0, k0, r0 >> 6, plane);
                     else
-#pragma unroll
-                        for (int c = 0; c < BM * MT / 64; ++c) tc::tma_load_4d(sa + c * 8192, &map_a, fb, m0 + c * 64, k0, pa, 0);
-                    if (!P.b_n_major) tc::tma_load_4d(sb, &map_b, fb, k0, n0, pb, 0);
-                    else
-#pragma unroll
-                        for (int c = 0; c < BN / 64; ++c) tc::tma_load_4d(sb + c * 8192, &map_b, fb, n0 + c * 64, k0, pb, 0);
-                    if (++stage == STAGES) { stage = 0; phase ^= 1u; }
-                    if (++q == P.nprod) { q = 0; ++kb; }
+                        for (int c = 0; c < boxes; ++c) load(dst + c * 8192, fb, r0 + c * 64, k0, plane, 0);
+                    if (++stage == (uint32_t)STAGES) { stage = 0; phase ^= 1u; }
+                    if (nprod == 1) k0 += BK;
+                    else {
+                        if (++q == nprod) { q = 0; k0 += BK; }
+                        plane = of_a ? plane_a(q) : plane_b(q);
+                    }
                 }
             }
         }
-        if (warp == 1 && lane == 0) {
-            const uint32_t idesc = tc::instr_desc(P.in_f16, P.b_n_major, BN, P.a_m_major);
-            uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
+        if (warp == 1 && lane == 0 && rank == 0) {
+            const uint32_t idesc = PAIR ? tc2::instr_desc_pair(P.in_f16, P.b_n_major) | (P.a_m_major ? 1u << 15 : 0u) : tc::instr_desc(P.in_f16, P.b_n_major, BN, P.a_m_major);
+            const uint64_t ad = P.a_m_major ? tc::smem_desc(tc::smem_u32(smem_a), 8192, 1024) : tc::smem_desc(tc::smem_u32(smem_a), 16, 1024);
+            const uint64_t bd = P.b_n_major ? tc::smem_desc(tc::smem_u32(smem_b), 8192, 1024) : tc::smem_desc(tc::smem_u32(smem_b), 16, 1024);
+            const uint32_t a_hi = (uint32_t)(ad >> 32), b_hi = (uint32_t)(bd >> 32), a_lo0 = (uint32_t)ad, b_lo0 = (uint32_t)bd; // (shared memory ends below 2^18: the address never carries out of its 14 bits)
+            const uint32_t ak = P.a_m_major ? 2048 >> 4 : 32 >> 4, bk = P.b_n_major ? 2048 >> 4 : 32 >> 4; // 16 further along the summed axis
+            const uint32_t a_step = (uint32_t)A_BYTES >> 4, chunk = (uint32_t)P.chunk;
+            uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0, a_lo = a_lo0, b_lo = b_lo0;
             bool ok = true;
-            for (int64_t t = blockIdx.x; t < total && ok; t += gridDim.x) {
+            for (int64_t t = tile0; t < total && ok; t += tile_step) {
                 int kb0;
-                const int steps = steps_of(t / per_split, kb0);
-                int in_chunk = 0;
-                for (int s = 0; s < steps; ++s) {
-                    if (MT == 1 && in_chunk == 0) {
-                        ok = tc::mbar_wait(tempty0 + 8 * acc, acc_phase ^ 1u, abort_flag, P.status, 2u);
+                int left = steps_of(t / per_split, kb0);
+                while (left > 0 && ok) { // a chunk
+                    const uint32_t n = (uint32_t)left < chunk ? (uint32_t)left : chunk;
+                    left -= (int)n;
+                    ok = wait(tempty0 + 8 * acc, acc_phase ^ 1u, abort_flag, P.status, 2u);
+                    if (!ok) break;
+                    const uint32_t tacc = tmem_base + acc * BN;
+                    for (uint32_t s = 0; s < n; ++s) {
+                        ok = wait(full0 + 8 * stage, phase, abort_flag, P.status, 3u);
                         if (!ok) break;
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    }
-                    ok = tc::mbar_wait(full0 + 8 * stage, phase, abort_flag, P.status, 3u);
-                    if (!ok) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t sa = tc::smem_u32(smem_a + stage * A_BYTES), sb = tc::smem_u32(smem_b + stage * B_BYTES);
+                        umma<PAIR>(tacc, a_lo, a_hi, b_lo, b_hi, idesc, s);
 #pragma unroll
-                    for (int h = 0; h < MT; ++h) {
-                        if (MT == 2 && s == 0) { // this half's accumulator has to be read out by the tile before
-                            ok = tc::mbar_wait(tempty0 + 8 * h, acc_phase ^ 1u, abort_flag, P.status, 2u);
-                            if (!ok) break;
-                            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        }
-#pragma unroll
-                        for (int k = 0; k < BK / tc::UMMA_K; ++k) {
-                            const uint64_t ad = P.a_m_major ? tc::smem_desc(sa + h * (BM * BK * 2) + k * 2048, 8192, 1024) : tc::smem_desc(sa + h * (BM * BK * 2) + k * 32, 16, 1024);
-                            const uint64_t bd = P.b_n_major ? tc::smem_desc(sb + k * 2048, 8192, 1024) : tc::smem_desc(sb + k * 32, 16, 1024);
-                            tc::umma(tmem_base + (MT == 1 ? acc : (uint32_t)h) * BN, ad, bd, idesc, (in_chunk | k) != 0 ? 1u : 0u);
-                        }
+                        for (int k = 1; k < BK / tc::UMMA_K; ++k) umma<PAIR>(tacc, a_lo + k * ak, a_hi, b_lo + k * bk, b_hi, idesc, 1u);
+                        if (PAIR) tc2::umma_commit_pair(empty0 + 8 * stage);
+                        else tc::umma_commit(empty0 + 8 * stage);
+                        a_lo += a_step; b_lo += B_BYTES >> 4;
+                        if (++stage == (uint32_t)STAGES) { stage = 0; phase ^= 1u; a_lo = a_lo0; b_lo = b_lo0; }
                     }
                     if (!ok) break;
-                    tc::umma_commit(empty0 + 8 * stage);
-                    if (++stage == STAGES) { stage = 0; phase ^= 1u; }
-                    ++in_chunk;
-                    if (MT == 1 && (in_chunk == P.chunk || s + 1 == steps)) {
-                        tc::umma_commit(tfull0 + 8 * acc);
-                        in_chunk = 0;
-                        if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
-                    }
+                    if (PAIR) tc2::umma_commit_pair(tfull0 + 8 * acc);
+                    else tc::umma_commit(tfull0 + 8 * acc);
+                    if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
                 }
-                if (MT == 2 && ok) { tc::umma_commit(tfull0); acc_phase ^= 1u; }
             }
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_MANY));
-        const int quad = warp & 3, half = (warp - 4) >> 2;
-        uint4 *stage_out = reinterpret_cast<uint4 *>(smem + TILE_BYTES + 256) + (warp - 4) * 32 * 8;
+        const int quad = warp & 3, part = (warp - 4) >> 2; // which rows of the accumulator, which 64 columns
+        uint4 *stage_out = reinterpret_cast<uint4 *>(smem) + (warp - 4) * 32 * 4;
+        const uint32_t tempty_to = PAIR ? tc2::map_to_rank(tempty0, 0) : tempty0;
         uint32_t acc = 0, acc_phase = 0;
         bool ok = true;
-        for (int64_t t = blockIdx.x; t < total && ok; t += gridDim.x) {
+        for (int64_t t = tile0; t < total && ok; t += tile_step) {
             int64_t mt, nt;
             tc::tile_of(t % per_split, P.tiles_m, P.tiles_n, P.panel, mt, nt);
-            const int64_t sp = t / per_split, cbase = nt * BN + half * COLS;
+            const int64_t sp = t / per_split, cbase = nt * BN + part * COLS;
             int kb0;
-            const int steps = steps_of(sp, kb0), chunks = MT == 1 ? (steps + P.chunk - 1) / P.chunk : 1;
-#pragma unroll 1
-            for (int mh = 0; mh < MT && ok; ++mh) {
-            const int64_t row0 = (mt * MT + mh) * BM + quad * 32, row = row0 + lane;
+            const int steps = steps_of(sp, kb0), chunks = (steps + P.chunk - 1) / P.chunk;
+            const int64_t row0 = (PAIR ? mt * 2 + rank : mt) * BM + quad * 32, row = row0 + lane;
             // what the row's epilogue reads, asked for while the products still run: its factors and its first target here
             const bool own = MODE != MODE_OUT && row < P.rows && cbase < P.n;
             const int32_t first = (int32_t)(P.col0 + cbase); // the class of v[0]
@@ -369,43 +435,49 @@ __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ CUt
                 }
             }
             float v[COLS];
-#pragma unroll
-            for (int i = 0; i < COLS; ++i) v[i] = 0.0f;
             for (int ch = 0; ch < chunks; ++ch) {
-                if (MT == 1 || mh == 0) {
-                    ok = tc::mbar_wait(MT == 1 ? tfull0 + 8 * acc : tfull0, acc_phase, abort_flag, P.status, 4u);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                }
+                ok = tc::mbar_wait(tfull0 + 8 * acc, acc_phase, abort_flag, P.status, 4u);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t ta = tmem_base + ((uint32_t)(quad * 32) << 16) + (MT == 1 ? acc : (uint32_t)mh) * BN + half * COLS;
-                // 32 columns at a time, the next 32 on their way while these are added
-                uint32_t ra[32], rb[32];
-                tc::tmem_ld32(ta, ra);
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
+                const uint32_t ta = tmem_base + ((uint32_t)(quad * 32) << 16) + acc * BN + part * COLS;
+                if (ch == 0) {
+                    uint32_t ra[32], rb[32];
+                    tc::tmem_ld32(ta, ra);
+                    tc::tmem_ld32(ta + 32, rb);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                    if (g < 3) tc::tmem_ld32(ta + (g + 1) * 32, g & 1 ? ra : rb);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) v[g * 32 + i] = __fadd_rn(v[g * 32 + i], __uint_as_float(g & 1 ? rb[i] : ra[i]));
+                    for (int i = 0; i < 32; ++i) { v[i] = __uint_as_float(ra[i]); v[32 + i] = __uint_as_float(rb[i]); }
+                } else {
+#pragma unroll
+                    for (int g = 0; g < COLS; g += 16) {
+                        uint32_t r[16];
+                        tc::tmem_ld16(ta + g, r);
+                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) v[g + i] = __fadd_rn(v[g + i], __uint_as_float(r[i]));
+                    }
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) tc::mbar_arrive(tempty0 + 8 * (MT == 1 ? acc : (uint32_t)mh));
-                if (MT == 1 && ++acc == 2) { acc = 0; acc_phase ^= 1u; }
+                if (lane == 0) {
+                    if (PAIR) tc2::mbar_arrive_cluster(tempty_to + 8 * acc);
+                    else tc::mbar_arrive(tempty_to + 8 * acc);
+                }
+                if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
             }
             if (!ok) break;
             const int rows_live = P.m - row0 < 32 ? (int)(P.m - row0) : 32;
-            if (rows_live <= 0 || cbase >= P.n) continue; // the whole warp: the next half, or the next tile
+            if (rows_live <= 0 || cbase >= P.n) continue; // the whole warp: the next tile
             const int live = P.n - cbase < COLS ? (int)(P.n - cbase) : COLS; // columns inside the matrix
-            if constexpr (MODE == MODE_STATS || MODE == MODE_GRAD) {
+            const float c = MODE == MODE_OUT ? 0.0f : __fmul_rn(P.c, un);
+            if constexpr (MODE != MODE_OUT) {
                 if (live < COLS) {
 #pragma unroll
                     for (int i = 0; i < COLS; ++i)
                         if (i >= live) v[i] = -INFINITY;
                 }
             }
-            const float c = MODE == MODE_OUT ? 0.0f : __fmul_rn(P.c, un);
             if constexpr (MODE == MODE_STATS) {
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -413,10 +485,9 @@ __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ CUt
                 const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                 // (one rounded product m·c instead of the differences would be an instruction less, and wrong by 2^-24 of m·c)
                 const float shift = m == -INFINITY ? 0.0f : m;
-                // the targets' logits: a column that only its thread knows, found among registers sixteen at a time
-                while (y >= 0 && y < live) {
+                while (y >= 0 && y < live) { // the targets' logits
                     float l = 0.0f;
-                    pick_column<0>(l, y, v, std::make_integer_sequence<int, 16>());
+                    pick_column<0>(l, y, v, Sixteen());
                     P.hit[row * P.top + at] = __fmul_rn(l, un);
                     y = ++at < end ? list[at] - first : -1;
                 }
@@ -428,7 +499,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ CUt
 #pragma unroll
                 for (int i = 0; i < COLS; ++i) v[i] = ex2(__fmaf_rn(v[i], c, -lse2));
                 while (y >= 0 && y < live) {
-                    take_column<0>(v, y, pw, std::make_integer_sequence<int, 16>());
+                    take_column<0>(v, y, pw, Sixteen());
                     y = -1;
                     if (++at < end) { y = list[at] - first; pw = P.p[row * P.top + at]; }
                 }
@@ -439,76 +510,71 @@ __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ CUt
                 // f32), it is the exact remainder rounded again. Rows are padded to whole lines, the padding zeros.
                 uint8_t *base = (uint8_t *)(P.g + row0 * P.g_ld + cbase);
 #pragma unroll
-                for (int g = 0; g < 2; ++g) {
-                    const int64_t left = (P.g_ld - cbase - g * 64) * 2;
-                    const int bytes = left < 128 ? (int)left : 128;
-                    uint32_t w[32];
-                    if (P.g_f16) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) w[i] = pack_f16x2_hw(v[g * 64 + 2 * i], v[g * 64 + 2 * i + 1]);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) w[i] = pack_bf16x2_hw(v[g * 64 + 2 * i], v[g * 64 + 2 * i + 1]);
-                    }
-                    store_rows<false>(stage_out, lane, w, base + g * 128, P.g_ld * 2, rows_live, bytes);
-                    if constexpr (REST) {
-                        if (P.g_f16) {
-#pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                w[i] = pack_f16x2_hw(__fsub_rn(v[g * 64 + 2 * i], f16_to_f32((uint16_t)(w[i] & 0xffffu))), __fsub_rn(v[g * 64 + 2 * i + 1], f16_to_f32((uint16_t)(w[i] >> 16))));
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                w[i] = pack_bf16x2_hw(__fsub_rn(v[g * 64 + 2 * i], bf16_up(w[i] & 0xffffu)), __fsub_rn(v[g * 64 + 2 * i + 1], bf16_up(w[i] >> 16)));
-                        }
-                        store_rows<false>(stage_out, lane, w, base + g * 128 + P.g_rest * 2, P.g_ld * 2, rows_live, bytes);
-                    }
+                for (int g = 0; g < COLS; g += 32) {
+                    const int64_t left = (P.g_ld - cbase - g) * 2;
+                    const int bytes = left < 64 ? (int)left : 64;
+                    uint32_t w[16], rest[16];
+                    if (g == 0) pack_g<REST, 0>(P.g_f16, w, rest, v);
+                    else pack_g<REST, 32>(P.g_f16, w, rest, v);
+                    store_rows<false>(stage_out, lane, w, base + g * 2, P.g_ld * 2, rows_live, bytes);
+                    if constexpr (REST) store_rows<false>(stage_out, lane, rest, base + (g + P.g_rest) * 2, P.g_ld * 2, rows_live, bytes);
                 }
             } else {
                 const float f = undo(P.scales, P.un);
+#pragma unroll
+                for (int i = 0; i < COLS; ++i) v[i] = __fmul_rn(v[i], f);
+                const int eb = P.out_dtype == PSK_F32 ? 4 : 2;
+                uint8_t *base = (uint8_t *)P.out + ((sp * P.m + row0) * P.out_ld + cbase) * eb;
+                auto store = [&](const uint32_t (&w)[16], int g) { // columns g .. of the part, 64 bytes
+                    const int64_t left = (P.n - cbase - g) * eb;
+                    const int bytes = left < 64 ? (int)(P.out_vec ? (left + 15) / 16 * 16 : left) : 64; // vec: n in whole units, or rows padded to one
+                    uint8_t *to = base + g * eb;
+                    if (P.accumulate) store_rows<true>(stage_out, lane, w, to, P.out_ld * eb, rows_live, bytes);
+                    else if (P.out_vec) store_rows<false>(stage_out, lane, w, to, P.out_ld * eb, rows_live, bytes);
+                    else if (eb == 4) store_rows_any<uint32_t>(stage_out, lane, w, to, P.out_ld * eb, rows_live, bytes);
+                    else store_rows_any<uint16_t>(stage_out, lane, w, to, P.out_ld * eb, rows_live, bytes);
+                };
+                // (the type is asked for outside the loops: a test an element made this the longest part of short sums)
+                uint32_t w[16];
                 if (P.out_dtype == PSK_F32) {
-                    uint8_t *base = (uint8_t *)((float *)P.out + (sp * P.m + row0) * P.out_ld + cbase);
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        uint32_t w[32];
+                    for (int g = 0; g < COLS; g += 16) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(__fmul_rn(v[g * 32 + i], f));
-                        const int64_t left = (P.n - cbase - g * 32) * 4;
-                        const int bytes = left < 128 ? (int)(P.out_vec ? (left + 15) / 16 * 16 : left) : 128; // vec: n a multiple of 4, or rows padded to one
-                        if (P.accumulate) store_rows<true>(stage_out, lane, w, base + g * 128, P.out_ld * 4, rows_live, bytes);
-                        else if (P.out_vec) store_rows<false>(stage_out, lane, w, base + g * 128, P.out_ld * 4, rows_live, bytes);
-                        else store_rows_any<uint32_t>(stage_out, lane, w, base + g * 128, P.out_ld * 4, rows_live, bytes);
+                        for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(v[g + i]);
+                        store(w, g);
+                    }
+                } else if (P.out_dtype == PSK_BF16) {
+#pragma unroll
+                    for (int g = 0; g < COLS; g += 32) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) w[i] = pack_bf16x2_hw(v[g + 2 * i], v[g + 2 * i + 1]);
+                        store(w, g);
                     }
                 } else {
-                    uint8_t *base = (uint8_t *)((uint16_t *)P.out + row0 * P.out_ld + cbase);
-                    uint32_t over = 0;
+                    if (P.ovf) {
+                        uint32_t over = 0;
 #pragma unroll
-                    for (int g = 0; g < 2; ++g) {
-                        uint32_t w[32];
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const float a = __fmul_rn(v[g * 64 + 2 * i], f), b = __fmul_rn(v[g * 64 + 2 * i + 1], f);
-                            if (P.out_dtype == PSK_F16) { over |= overflows(a, kF16Overflow) | overflows(b, kF16Overflow); w[i] = pack_f16x2_hw(a, b); }
-                            else w[i] = pack_bf16x2_hw(a, b);
-                        }
-                        const int64_t left = (P.n - cbase - g * 64) * 2;
-                        const int bytes = left < 128 ? (int)left : 128;
-                        if (P.out_vec) store_rows<false>(stage_out, lane, w, base + g * 128, P.out_ld * 2, rows_live, bytes);
-                        else store_rows_any<uint16_t>(stage_out, lane, w, base + g * 128, P.out_ld * 2, rows_live, bytes);
+                        for (int i = 0; i < COLS; ++i) over |= overflows(v[i], kF16Overflow);
+                        if (over) atomicOr(P.ovf, 1u);
                     }
-                    if (P.ovf && over) atomicOr(P.ovf, 1u);
+#pragma unroll
+                    for (int g = 0; g < COLS; g += 32) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) w[i] = pack_f16x2_hw(v[g + 2 * i], v[g + 2 * i + 1]);
+                        store(w, g);
+                    }
                 }
             }
-            } // mh
-            if (MT == 2) acc_phase ^= 1u;
         }
     }
 
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if (PAIR) tc2::cluster_sync(); // nobody leaves, or frees tensor memory the pair's products write, while the other works
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(2 * BN) : "memory");
+        if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(2 * BN) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(2 * BN) : "memory");
     }
 }
 
