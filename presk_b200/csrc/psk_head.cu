@@ -115,7 +115,7 @@ int launch(HeadContext &x, const CUtensorMap &ma, const CUtensorMap &mb, const P
         k = 1 + 2 * (PAIR ? pairs_of(k_head<MODE, PAIR, REST>, x) : 0);
         if (device < 64) known[device].store(k, std::memory_order_relaxed);
     }
-    const int64_t tiles = P.tiles_m * P.tiles_n * P.splits;
+    const int64_t tiles = (int64_t)P.tiles_m * P.tiles_n * P.splits;
     if (PAIR) {
         if (k >> 1 < 1) return fail(x, PSK_E10001, "head: no pair of SMs for a cluster");
         cudaLaunchConfig_t c;
@@ -136,10 +136,12 @@ template <int MODE, bool REST = false>
 int product(HeadContext &x, Params P, const Operand &a, const Operand &b, int f16)
 {
     P.m = a.rows; P.n = b.rows;
+    if (MODE != MODE_OUT) P.splits = 1;
     const int64_t tiles = ((P.m + BM - 1) / BM) * ((P.n + BN - 1) / BN);
     // pairs of CTAs where there are rows for two and tiles for everybody (see Cfg)
     const bool pair = P.m > BM && tiles >= x.sms;
-    P.tiles_m = (P.m + (pair ? 2 : 1) * BM - 1) / ((pair ? 2 : 1) * BM); P.tiles_n = (P.n + BN - 1) / BN;
+    P.tiles_m = (uint32_t)((P.m + (pair ? 2 : 1) * BM - 1) / ((pair ? 2 : 1) * BM)); P.tiles_n = (uint32_t)((P.n + BN - 1) / BN);
+    if (tiles > 0x7fffffff / std::max<int64_t>(1, P.splits)) return fail(x, PSK_E7005, "head: more tiles than one launch counts");
     const int a_rows = !pair && a.k_contiguous ? (int)std::min<int64_t>(BM, up(P.m, 8)) : BM;
     P.a_stage = a_rows * BK * 2;
     P.stages = Cfg::stages(P.a_stage, (pair ? BN / 2 : BN) * BK * 2, MODE != MODE_STATS);
@@ -147,12 +149,12 @@ int product(HeadContext &x, Params P, const Operand &a, const Operand &b, int f1
     if (!map_of(x, &ma, a, f16, a_rows, &P.a_blocks) || !map_of(x, &mb, b, f16, pair ? BN / 2 : BN, &P.b_blocks)) return fail(x, PSK_E10001, "head: an operand's layout does not make a tensor map");
     P.kb_k = (int32_t)((a.k + BK - 1) / BK);
     P.nprod = a.planes == 2 ? 3 : 1;
-    if (MODE != MODE_OUT) { P.splits = 1; P.kb_split = P.kb_k; }
+    if (MODE != MODE_OUT) P.kb_split = P.kb_k;
     // Steps an accumulator: 512 products of the summed axis (384 of f32's, three a block). Results of 16 bits, dx and dw, keep one
     // accumulator throughout, and g's logits 1024 products: what truncation loses there is far below their rounding.
     P.chunk = MODE == MODE_OUT && a.planes == 1 ? 1 << 28 : P.nprod == 3 ? 6 : MODE == MODE_GRAD ? 16 : 8;
     // a panel's columns of b stay in a part of the L2 while a's rows stream past them
-    P.panel = std::min<int64_t>(P.tiles_n, std::max<int64_t>(8, (16ll << 20) / std::max<int64_t>(1, BN * a.k * 2 * a.planes)));
+    P.panel = (uint32_t)std::min<int64_t>(P.tiles_n, std::max<int64_t>(8, (16ll << 20) / std::max<int64_t>(1, BN * a.k * 2 * a.planes)));
     P.in_f16 = f16; P.a_m_major = !a.k_contiguous; P.b_n_major = !b.k_contiguous;
     P.status = x.status;
     x.flops += 2.0 * (double)P.m * (double)P.n * (double)a.k;
@@ -394,7 +396,7 @@ int head_run(HeadContext &x, const psk_launch *l, void *const *table)
         memset(&Q, 0, sizeof Q);
         Q.scales = scales;
         Q.kb_split = dxo.kb_split;
-        Q.splits = ((vn + BK - 1) / BK + dxo.kb_split - 1) / dxo.kb_split; // a shorter last piece may have fewer
+        Q.splits = (uint32_t)(((vn + BK - 1) / BK + dxo.kb_split - 1) / dxo.kb_split); // a shorter last piece may have fewer
         Q.out = dxo.straight ? const_cast<void *>(rout.p) : dxp; Q.out_ld = dxo.straight ? dx_ld : dxo.ld; Q.out_dtype = dxo.straight ? dt : PSK_F32;
         Q.un = dxo.straight ? UN_DX : UN_NONE; Q.accumulate = piece > 0;
         Q.out_vec = !dxo.straight || (aligned(rout.p) && dx_ld * eb % 16 == 0 && D * eb % 16 == 0);
@@ -409,7 +411,7 @@ int head_run(HeadContext &x, const psk_launch *l, void *const *table)
             const int64_t cols = dw_v_inner ? vn : D;
             memset(&Q, 0, sizeof Q);
             Q.scales = scales;
-            Q.splits = dwo.splits; Q.kb_split = dwo.kb_split;
+            Q.splits = (uint32_t)dwo.splits; Q.kb_split = dwo.kb_split;
             Q.out = dwo.straight ? (void *)dst : dwp; Q.out_ld = dwo.straight ? dw_ld : dwo.ld; Q.out_dtype = dwo.straight ? dt : PSK_F32;
             Q.un = dwo.straight ? UN_DW : UN_NONE;
             Q.out_vec = !dwo.straight || (aligned(dst) && dw_ld * eb % 16 == 0 && cols * eb % 16 == 0);

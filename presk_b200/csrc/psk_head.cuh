@@ -86,7 +86,7 @@ PSK_DEV float undo(const Scales *s, int un)
 
 struct Params {
     int64_t m, n;                 // rows and columns of the product
-    int64_t tiles_m, tiles_n, splits, panel;
+    uint32_t tiles_m, tiles_n, splits, panel; // their product below 2^31
     int32_t kb_k, nprod;          // blocks of 64 along the summed axis; partial products a block (1, or 3 of two planes)
     int32_t kb_split;             // blocks of the summed axis a split
     int32_t chunk;                // steps (block, partial product) in one accumulator before it is added into registers
@@ -201,6 +201,15 @@ PSK_DEV void umma(uint32_t acc, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uin
                      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n\t}" ::"r"(acc), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(add) : "memory");
 }
 
+// Where tile `t` of a split lies: panels of `panel` tile-columns, down every tile-row of one before the next, so that
+// the tiles in flight share columns of b that stay in the L2 (32-bit divisions: every warp does this for every tile).
+PSK_DEV void tile_at(uint32_t t, uint32_t tiles_m, uint32_t tiles_n, uint32_t panel, uint32_t &mt, uint32_t &nt)
+{
+    const uint32_t per = panel * tiles_m, p = t / per, in = t - p * per, width = tiles_n - p * panel < panel ? tiles_n - p * panel : panel;
+    mt = in / width;
+    nt = p * panel + (in - mt * width);
+}
+
 // First entry of a row's ascending list that is at least `c`.
 PSK_DEV int lower_bound(const int32_t *ids, int n, int32_t c)
 {
@@ -301,10 +310,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ CUt
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem_base = *tmem_slot;
 
-    const int64_t per_split = P.tiles_m * P.tiles_n, total = per_split * P.splits;
-    const int64_t tile0 = PAIR ? blockIdx.x >> 1 : blockIdx.x, tile_step = PAIR ? gridDim.x >> 1 : gridDim.x;
+    const uint32_t per_split = P.tiles_m * P.tiles_n, total = per_split * P.splits;
+    const uint32_t tile0 = PAIR ? blockIdx.x >> 1 : blockIdx.x, tile_step = PAIR ? gridDim.x >> 1 : gridDim.x;
     // the steps of a split: blocks kb_first .. of the summed axis, nprod partial products each
-    auto steps_of = [&](int64_t sp, int &kb_first) {
+    auto steps_of = [&](uint32_t sp, int &kb_first) {
         kb_first = (int)sp * P.kb_split;
         const int left = P.kb_k - kb_first;
         return (left < P.kb_split ? left : P.kb_split) * P.nprod;
@@ -329,12 +338,13 @@ __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ CUt
                 if (PAIR) tc2::tma_load_4d_pair(dst, map, bar, c0, c1, c2, c3);
                 else tc::tma_load_4d(dst, map, bar, c0, c1, c2, c3);
             };
-            for (int64_t t = tile0; t < total && ok; t += tile_step) {
-                int64_t mt, nt;
-                tc::tile_of(t % per_split, P.tiles_m, P.tiles_n, P.panel, mt, nt);
+            for (uint32_t t = tile0; t < total && ok; t += tile_step) {
+                uint32_t mt, nt;
+                const uint32_t sp = t / per_split;
+                tile_at(t - sp * per_split, P.tiles_m, P.tiles_n, P.panel, mt, nt);
                 const int r0 = of_a ? (int)(PAIR ? mt * 2 + rank : mt) * BM : (int)nt * BN + (PAIR ? (int)rank * (BN / 2) : 0);
                 int kb0;
-                const int steps = steps_of(t / per_split, kb0);
+                const int steps = steps_of(sp, kb0);
                 int k0 = kb0 * BK, plane = 0;
                 uint32_t q = 0;
                 for (int s = 0; s < steps; ++s) {
@@ -364,7 +374,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ CUt
             const uint32_t a_step = (uint32_t)A_BYTES >> 4, chunk = (uint32_t)P.chunk;
             uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0, a_lo = a_lo0, b_lo = b_lo0;
             bool ok = true;
-            for (int64_t t = tile0; t < total && ok; t += tile_step) {
+            for (uint32_t t = tile0; t < total && ok; t += tile_step) {
                 int kb0;
                 int left = steps_of(t / per_split, kb0);
                 while (left > 0 && ok) { // a chunk
@@ -399,13 +409,14 @@ __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ CUt
         const uint32_t tempty_to = PAIR ? tc2::map_to_rank(tempty0, 0) : tempty0;
         uint32_t acc = 0, acc_phase = 0;
         bool ok = true;
-        for (int64_t t = tile0; t < total && ok; t += tile_step) {
-            int64_t mt, nt;
-            tc::tile_of(t % per_split, P.tiles_m, P.tiles_n, P.panel, mt, nt);
-            const int64_t sp = t / per_split, cbase = nt * BN + part * COLS;
+        for (uint32_t t = tile0; t < total && ok; t += tile_step) {
+            uint32_t mt, nt;
+            const uint32_t sp = t / per_split;
+            tile_at(t - sp * per_split, P.tiles_m, P.tiles_n, P.panel, mt, nt);
+            const int64_t cbase = (int64_t)nt * BN + part * COLS;
             int kb0;
             const int steps = steps_of(sp, kb0), chunks = (steps + P.chunk - 1) / P.chunk;
-            const int64_t row0 = (PAIR ? mt * 2 + rank : mt) * BM + quad * 32, row = row0 + lane;
+            const int64_t row0 = (int64_t)(PAIR ? mt * 2 + rank : mt) * BM + quad * 32, row = row0 + lane;
             // what the row's epilogue reads, asked for while the products still run: its factors and its first target here
             const bool own = MODE != MODE_OUT && row < P.rows && cbase < P.n;
             const int32_t first = (int32_t)(P.col0 + cbase); // the class of v[0]
@@ -461,7 +472,9 @@ __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ CUt
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) {
-                    if (PAIR) tc2::mbar_arrive_cluster(tempty_to + 8 * acc);
+                    // (release at the scope of the CTA, the default: what is handed back is tensor memory, ordered by the fence above;
+                    // at the cluster's scope the arrival waits for the global stores of the tile before)
+                    if (PAIR) asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(tempty_to + 8 * acc) : "memory");
                     else tc::mbar_arrive(tempty_to + 8 * acc);
                 }
                 if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
@@ -524,7 +537,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ CUt
 #pragma unroll
                 for (int i = 0; i < COLS; ++i) v[i] = __fmul_rn(v[i], f);
                 const int eb = P.out_dtype == PSK_F32 ? 4 : 2;
-                uint8_t *base = (uint8_t *)P.out + ((sp * P.m + row0) * P.out_ld + cbase) * eb;
+                uint8_t *base = (uint8_t *)P.out + (((int64_t)sp * P.m + row0) * P.out_ld + cbase) * eb;
                 auto store = [&](const uint32_t (&w)[16], int g) { // columns g .. of the part, 64 bytes
                     const int64_t left = (P.n - cbase - g) * eb;
                     const int bytes = left < 64 ? (int)(P.out_vec ? (left + 15) / 16 * 16 : left) : 64; // vec: n in whole units, or rows padded to one
