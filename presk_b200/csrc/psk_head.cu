@@ -86,6 +86,29 @@ int fail(HeadContext &x, int code, const std::string &msg)
         if (err__ != cudaSuccess) return fail(x, PSK_E10001, std::string(#call) + ": " + cudaGetErrorString(err__)); \
     } while (0)
 
+// Queues a kernel that may begin while the one before it on the stream ends (each waits for that by itself, `follow`).
+template <class K, class... A>
+int enqueue(HeadContext &x, K kernel, int64_t grid, unsigned grid_y, unsigned block, size_t shared, unsigned cluster, const A &...args)
+{
+    cudaLaunchConfig_t c;
+    memset(&c, 0, sizeof c);
+    c.gridDim = dim3((unsigned)grid, grid_y); c.blockDim = dim3(block); c.dynamicSmemBytes = shared; c.stream = x.stream;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cluster; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
+    c.attrs = at; c.numAttrs = cluster > 1 ? 2 : 1;
+    HEAD_TRY(cudaLaunchKernelEx(&c, kernel, args...));
+    x.kernels += 1;
+    return PSK_OK;
+}
+#define HEAD_START(...)                                    \
+    do {                                                   \
+        const int rc__ = enqueue(x, __VA_ARGS__);            \
+        if (rc__ != PSK_OK) return rc__;                   \
+    } while (0)
+
 // How many clusters of two CTAs of a kernel the device holds at a time (SMs that no pair fits stay idle); 0: none.
 template <class K>
 int pairs_of(K kernel, const HeadContext &x)
@@ -116,19 +139,8 @@ int launch(HeadContext &x, const CUtensorMap &ma, const CUtensorMap &mb, const P
         if (device < 64) known[device].store(k, std::memory_order_relaxed);
     }
     const int64_t tiles = (int64_t)P.tiles_m * P.tiles_n * P.splits;
-    if (PAIR) {
-        if (k >> 1 < 1) return fail(x, PSK_E10001, "head: no pair of SMs for a cluster");
-        cudaLaunchConfig_t c;
-        memset(&c, 0, sizeof c);
-        c.gridDim = dim3((unsigned)(2 * std::min<int64_t>(tiles, k >> 1))); c.blockDim = dim3(THREADS); c.dynamicSmemBytes = Cfg::SMEM_TOTAL; c.stream = x.stream;
-        cudaLaunchAttribute at[1];
-        at[0].id = cudaLaunchAttributeClusterDimension;
-        at[0].val.clusterDim.x = 2; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
-        c.attrs = at; c.numAttrs = 1;
-        HEAD_TRY(cudaLaunchKernelEx(&c, k_head<MODE, PAIR, REST>, ma, mb, P));
-    } else k_head<MODE, PAIR, REST><<<(unsigned)std::min<int64_t>(tiles, x.sms), THREADS, Cfg::SMEM_TOTAL, x.stream>>>(ma, mb, P);
-    x.kernels += 1;
-    return PSK_OK;
+    if (PAIR && k >> 1 < 1) return fail(x, PSK_E10001, "head: no pair of SMs for a cluster");
+    return enqueue(x, k_head<MODE, PAIR, REST>, PAIR ? 2 * std::min<int64_t>(tiles, k >> 1) : std::min<int64_t>(tiles, x.sms), 1, THREADS, Cfg::SMEM_TOTAL, PAIR ? 2 : 1, ma, mb, P);
 }
 
 // One product a·bᵀ and what MODE makes of it.
@@ -164,26 +176,28 @@ int product(HeadContext &x, Params P, const Operand &a, const Operand &b, int f1
 // Blocks of eight warps for `work` warps' worth.
 int warps_of(const HeadContext &x, int64_t work) { return (int)std::max<int64_t>(1, std::min<int64_t>((work + 7) / 8, (int64_t)x.sms * 8)); }
 
-// The copy's kernel by what it makes and whether it may read and write 16 bytes at a time.
-void pack(HeadContext &x, const PackParams &k)
-{
-    bool vec = k.col_stride == 1 && k.cols == k.ld && ((uintptr_t)k.src.p & 15u) == 0;
-    const int64_t unit = k.to == PACK_SPLIT ? 4 : 8; // elements of 16 bytes
-    for (int a = 0; a < k.s.no; ++a) vec = vec && (k.s.dims[a] == 1 || k.src.stride[a] % unit == 0);
-    const int grid = warps_of(x, k.un ? k.s.rows : k.s.rows * ((k.ld + PIECE - 1) / PIECE));
-    if (k.to == PACK_SPLIT) { if (vec) k_head_pack<PACK_SPLIT, true><<<grid, 256, 0, x.stream>>>(k); else k_head_pack<PACK_SPLIT, false><<<grid, 256, 0, x.stream>>>(k); }
-    else if (k.to == PACK_F16) { if (vec) k_head_pack<PACK_F16, true><<<grid, 256, 0, x.stream>>>(k); else k_head_pack<PACK_F16, false><<<grid, 256, 0, x.stream>>>(k); }
-    else { if (vec) k_head_pack<PACK_SAME, true><<<grid, 256, 0, x.stream>>>(k); else k_head_pack<PACK_SAME, false><<<grid, 256, 0, x.stream>>>(k); }
-    x.kernels += 1;
-}
-
-void greatest(HeadContext &x, const MaxParams &m)
-{
-    const int grid = warps_of(x, m.s.rows * ((m.cols + PIECE - 1) / PIECE));
-    if (m.src.dtype == PSK_F32) k_head_max<true><<<grid, 256, 0, x.stream>>>(m);
-    else k_head_max<false><<<grid, 256, 0, x.stream>>>(m);
-    x.kernels += 1;
-}
+// Copies collected and made by one launch.
+struct Copies {
+    Packs all;
+    unsigned n = 0;
+    int64_t grid = 1;
+    Copies() { memset(&all, 0, sizeof all); }
+    void add(const HeadContext &x, PackParams k)
+    {
+        const int64_t unit = k.to == PACK_SPLIT ? 4 : 8; // elements of 16 bytes
+        k.vec = k.col_stride == 1 && k.cols == k.ld && ((uintptr_t)k.src.p & 15u) == 0;
+        for (int a = 0; a < k.s.no; ++a) k.vec = k.vec && (k.s.dims[a] == 1 || k.src.stride[a] % unit == 0);
+        grid = std::max<int64_t>(grid, warps_of(x, k.un ? k.s.rows : k.s.rows * ((k.ld + PIECE - 1) / PIECE)));
+        all.of[n++] = k;
+    }
+    int make(HeadContext &x)
+    {
+        if (!n) return PSK_OK;
+        HEAD_START(k_head_pack, grid, n, 256, 0, 1, all);
+        n = 0; grid = 1;
+        return PSK_OK;
+    }
+};
 
 RowOperand row_operand(const psk_operand &o, void *base, int no)
 {
@@ -317,48 +331,53 @@ int head_run(HeadContext &x, const psk_launch *l, void *const *table)
             T.s = s; T.ids = rids; T.t = row_operand(l->in[3], table[3], no); T.ct = rct; T.lse = rlse;
             T.ids_k = I.stride[ax_k]; T.t_k = l->in[3].stride[ax_k]; T.classes = V; T.top = (int32_t)K; T.inv_tau = inv_tau;
             T.out_ids = ids; T.start = start; T.parts = parts; T.out_p = p; T.plogp = plogp; T.coef = coef; T.lse2 = lse2; T.status = x.status; T.ctmax = g_scaled ? &scales->max_ct : nullptr;
-            k_head_teacher<<<(unsigned)N, (unsigned)up(K, 32), (size_t)K * 8, x.stream>>>(T);
+            HEAD_START(k_head_teacher, N, 1, (unsigned)up(K, 32), (size_t)K * 8, 1, T);
         } else {
             LabelParams T;
             memset(&T, 0, sizeof T);
             T.s = s; T.ids = rids; T.ct = rct; T.lse = rlse; T.classes = V; T.inv_tau = inv_tau;
             T.ids_out = ids; T.coef = coef; T.lse2 = lse2; T.status = x.status; T.ctmax = g_scaled ? &scales->max_ct : nullptr;
-            k_head_labels<<<(unsigned)((N + 255) / 256), 256, 0, x.stream>>>(T);
+            HEAD_START(k_head_labels, (N + 255) / 256, 1, 256, 0, 1, T);
         }
-        x.kernels += 1;
         // 2. the powers of two
         if (any_scale) {
             const bool of_x = DW && (f32 || conv), of_w = f32 || conv;
-            MaxParams M;
+            MaxOfTwo both;
+            memset(&both, 0, sizeof both);
+            unsigned n = 0;
+            int64_t grid = 1;
             if (of_x) {
-                memset(&M, 0, sizeof M);
+                MaxParams &M = both.of[n++];
                 M.s = s; M.src = rx; M.col_stride = X.stride[ax_d]; M.cols = D; M.ids = ids; M.top = (int32_t)K; M.out = &scales->max_x;
                 M.vec = x_ld && M.col_stride == 1 && aligned(rx.p) && x_ld * eb % 16 == 0 && D * eb % 16 == 0;
-                greatest(x, M);
+                grid = warps_of(x, N * ((D + PIECE - 1) / PIECE));
             }
             if (of_w) {
-                memset(&M, 0, sizeof M);
+                MaxParams &M = both.of[n++];
                 M.s.no = 1; M.s.rows = M.s.dims[0] = v_inner ? D : V; M.src.p = wp; M.src.dtype = dt; M.src.stride[0] = v_inner ? w_d : w_v;
                 M.col_stride = v_inner ? w_v : w_d; M.cols = v_inner ? V : D; M.out = &scales->max_w;
                 M.vec = M.col_stride == 1 && aligned(wp) && M.src.stride[0] * eb % 16 == 0 && M.cols * eb % 16 == 0;
-                greatest(x, M);
+                grid = std::max<int64_t>(grid, warps_of(x, M.s.rows * ((M.cols + PIECE - 1) / PIECE)));
             }
+            if (n && f32) HEAD_START(k_head_max<true>, grid, n, 256, 0, 1, both);
+            else if (n) HEAD_START(k_head_max<false>, grid, n, 256, 0, 1, both);
         }
     }
-    // 3. x for the logits, and (rows without a target zeros) for dw
+    // 3. x for the logits, and (rows without a target zeros) for dw: made together with the first piece's copies of the head
+    Copies copies;
     PackParams kx;
     memset(&kx, 0, sizeof kx);
     kx.s = s; kx.src = rx; kx.col_stride = X.stride[ax_d]; kx.cols = D; kx.ld = Dp; kx.ids = ids; kx.top = (int32_t)K; kx.copies = 1;
     if (xl) {
         PackParams k = kx;
         k.dst = xl; k.plane = N * Dp; k.to = f32 ? PACK_SPLIT : PACK_SAME; k.un = un_x;
-        pack(x, k);
+        copies.add(x, k);
     }
     if (xd && N) {
         PackParams k = kx;
         k.dst = xd; k.plane = N * Dp; k.to = f32 ? PACK_SPLIT : conv ? PACK_F16 : PACK_SAME; k.copies = (int32_t)(Ng / N);
         k.max = f32 || conv ? &scales->max_x : nullptr;
-        pack(x, k);
+        copies.add(x, k);
     }
     const Operand a = x_direct ? Operand{rx.p, N, D, x_ld, true, 1, 0} : Operand{xl ? xl : xd, N, D, Dp, true, planes, N * Dp};
 
@@ -371,10 +390,13 @@ int head_run(HeadContext &x, const psk_launch *l, void *const *table)
             k.s.no = 1; k.s.rows = k.s.dims[0] = v_inner ? D : vn;
             k.src.p = wp + v0 * w_v * eb; k.src.dtype = dt; k.src.stride[0] = v_inner ? w_d : w_v;
             k.col_stride = v_inner ? w_v : w_d; k.cols = v_inner ? vn : D; k.ld = wc_ld; k.plane = wc_plane; k.dst = dst; k.to = to; k.max = max; k.copies = 1;
-            pack(x, k);
+            copies.add(x, k);
             return Operand{dst, vn, D, wc_ld, !v_inner, planes, wc_plane};
         };
         const Operand b = w_direct ? Operand{wp + v0 * w_v * 2, vn, D, v_inner ? w_d : w_v, !v_inner, 1, 0} : pack_w(wl, f32 ? PACK_SPLIT : PACK_SAME, f32 ? &scales->max_w : nullptr);
+        const Operand bd = conv ? pack_w(wd, PACK_F16, &scales->max_w) : b;
+        int r = copies.make(x);
+        if (r != PSK_OK) return r;
         // 5. the logits' tiles
         Params P;
         memset(&P, 0, sizeof P);
@@ -383,15 +405,14 @@ int head_run(HeadContext &x, const psk_launch *l, void *const *table)
         P.ids = ids; P.p = p; P.start = start; P.top = (int32_t)K; P.parts = parts;
         if (!vjp) {
             P.part = part; P.hit = hit;
-            const int r = product<MODE_STATS>(x, P, a, b, in_f16);
+            r = product<MODE_STATS>(x, P, a, b, in_f16);
             if (r != PSK_OK) return r;
             continue;
         }
         P.lse2 = lse2; P.coef = coef; P.g = g; P.g_f16 = g_f16; P.g_ld = g_ld; P.g_rest = N * g_ld;
-        int r = rest || f32 ? product<MODE_GRAD, true>(x, P, a, b, in_f16) : product<MODE_GRAD>(x, P, a, b, in_f16);
+        r = rest || f32 ? product<MODE_GRAD, true>(x, P, a, b, in_f16) : product<MODE_GRAD>(x, P, a, b, in_f16);
         if (r != PSK_OK) return r;
         // 6. dx = g·wᵀ summed over the pieces: both operands along the classes
-        const Operand bd = conv ? pack_w(wd, PACK_F16, &scales->max_w) : b;
         Params Q;
         memset(&Q, 0, sizeof Q);
         Q.scales = scales;
@@ -424,8 +445,7 @@ int head_run(HeadContext &x, const psk_launch *l, void *const *table)
                 S.s.no = 1; S.s.rows = S.s.dims[0] = dw_v_inner ? D : vn;
                 S.part = dwp; S.parts = dwo.splits; S.part_rows = S.s.rows; S.ld = dwo.ld; S.cols = cols; S.col_stride = DW->stride[dw_v_inner ? ax_v : ax_d];
                 S.scales = scales; S.un = UN_DW; S.dst.p = dst; S.dst.dtype = dt; S.dst.stride[0] = dw_ld; S.ovf = x.ovf; S.guarded = x.guarded;
-                k_head_sum<<<warps_of(x, S.s.rows * ((S.cols + 127) / 128)), 256, 0, x.stream>>>(S);
-                x.kernels += 1;
+                HEAD_START(k_head_sum, warps_of(x, S.s.rows * ((S.cols + 127) / 128)), 1, 256, 0, 1, S);
             }
         }
     }
@@ -435,23 +455,20 @@ int head_run(HeadContext &x, const psk_launch *l, void *const *table)
         J.s = s; J.parts = parts; J.part = part; J.hit = hit; J.ids = ids; J.p = p; J.plogp = plogp; J.top = (int32_t)K; J.c = (float)(1.4426950408889634 / tau); J.inv_tau = 1.0 / tau;
         J.loss = rout; J.ovf = x.ovf; J.guarded = x.guarded;
         if (LSE) J.lse = row_operand(*LSE, table[h.lse], no);
-        if (N >= 32 * x.sms) k_head_join<32><<<(unsigned)((N + 31) / 32), 256, 0, x.stream>>>(J);
-        else k_head_join<8><<<(unsigned)((N + 7) / 8), 256, 0, x.stream>>>(J);
-        x.kernels += 1;
+        if (N >= 32 * x.sms) HEAD_START(k_head_join<32>, (N + 31) / 32, 1, 256, 0, 1, J);
+        else HEAD_START(k_head_join<8>, (N + 7) / 8, 1, 256, 0, 1, J);
     } else if (N > 0 && !dxo.straight) {
         SumParams S;
         memset(&S, 0, sizeof S);
         S.s = s; S.part = dxp; S.parts = dxo.splits; S.part_rows = dxo.m; S.ld = dxo.ld; S.fold = rest ? N : 0; S.cols = D; S.col_stride = O.stride[ax_d];
         S.scales = scales; S.un = UN_DX; S.dst = rout; S.ovf = x.ovf; S.guarded = x.guarded;
-        k_head_sum<<<warps_of(x, N * ((D + 127) / 128)), 256, 0, x.stream>>>(S);
-        x.kernels += 1;
+        HEAD_START(k_head_sum, warps_of(x, N * ((D + 127) / 128)), 1, 256, 0, 1, S);
     } else if (N == 0 && DW) { // no rows: a gradient of zeros
         SumParams S;
         memset(&S, 0, sizeof S);
         S.s.no = 1; S.s.rows = S.s.dims[0] = dw_v_inner ? D : V; S.cols = dw_v_inner ? V : D; S.col_stride = DW->stride[dw_v_inner ? ax_v : ax_d];
         S.dst.p = (const uint8_t *)table[h.dw] + DW->offset * eb; S.dst.dtype = dt; S.dst.stride[0] = dw_ld;
-        k_head_sum<<<warps_of(x, S.s.rows * ((S.cols + 127) / 128)), 256, 0, x.stream>>>(S);
-        x.kernels += 1;
+        HEAD_START(k_head_sum, warps_of(x, S.s.rows * ((S.cols + 127) / 128)), 1, 256, 0, 1, S);
     }
     HEAD_TRY(cudaGetLastError());
     return PSK_OK;

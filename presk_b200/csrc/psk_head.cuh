@@ -124,6 +124,14 @@ struct Params {
     uint32_t *ovf;                // the overflow guard's flag; or null
 };
 
+// Every kernel here is launched to begin while the one before it ends (programmatic stream serialization): it lets
+// the next one in at once and waits, before its first access to memory, until the one before is complete.
+PSK_DEV void follow()
+{
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 PSK_DEV float ex2(float x)
 {
     float y;
@@ -309,6 +317,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ CUt
     if (PAIR) tc2::cluster_sync(); // both have their tensor memory before a product writes either
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem_base = *tmem_slot;
+    follow();
 
     const uint32_t per_split = P.tiles_m * P.tiles_n, total = per_split * P.splits;
     const uint32_t tile0 = PAIR ? blockIdx.x >> 1 : blockIdx.x, tile_step = PAIR ? gridDim.x >> 1 : gridDim.x;
@@ -640,6 +649,7 @@ PSK_DEV void row_factors(const RowSpace &s, const RowOperand &ct, const RowOpera
 
 static __global__ void __launch_bounds__(256) k_head_labels(const __grid_constant__ LabelParams P)
 {
+    follow();
     const int64_t row = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (row >= P.s.rows) return;
     const int64_t y = ((const int64_t *)P.ids.p)[row_offset(P.s, P.ids.stride, row)];
@@ -687,6 +697,7 @@ static __global__ void __launch_bounds__(1024) k_head_teacher(const __grid_const
 {
     extern __shared__ int32_t list[]; // top ids as they come, then in order
     __shared__ float red[32];
+    follow();
     const int64_t row = blockIdx.x;
     const int j = threadIdx.x;
     int32_t id = 0x7fffffff;
@@ -746,10 +757,14 @@ PSK_DEV uint32_t finite_bits(float x)
 
 constexpr int PIECE = 1024; // columns of a row that a warp takes at a time
 
+struct MaxOfTwo { MaxParams of[2]; };
+
 template <bool F32>
-__global__ void __launch_bounds__(256) k_head_max(const __grid_constant__ MaxParams P)
+__global__ void __launch_bounds__(256) k_head_max(const __grid_constant__ MaxOfTwo both)
 {
     __shared__ uint32_t red[8];
+    const MaxParams &P = both.of[blockIdx.y];
+    follow();
     const int lane = threadIdx.x & 31;
     const int64_t warps = (int64_t)gridDim.x * 8, pieces = (P.cols + PIECE - 1) / PIECE;
     uint32_t m = 0;
@@ -811,6 +826,7 @@ __global__ void __launch_bounds__(256) k_head_join(const __grid_constant__ JoinP
     constexpr int Y = 256 / X, AHEAD = 8;
     __shared__ float sm[8][X], sz[8][X];
     __shared__ double sh[8][X];
+    follow();
     const int x = threadIdx.x % X, y = threadIdx.x / X, warp = threadIdx.x >> 5;
     const int64_t row = (int64_t)blockIdx.x * X + x;
     float m = -INFINITY, z = 0.0f;
@@ -877,7 +893,7 @@ struct PackParams {
     RowOperand src;
     int64_t col_stride, cols, ld, plane;
     uint16_t *dst;
-    int32_t to, copies;
+    int32_t to, copies, vec;
     const uint32_t *max; // of the whole matrix, for its scale; or null
     float *un;          // PACK_SPLIT: scale every row by its own greatest element instead, and put the factor that undoes it here
     const int32_t *ids;
@@ -900,7 +916,7 @@ PSK_DEV uint32_t split_f16(float x)
 
 // VEC: the source's rows contiguous and on 16-byte boundaries, cols = ld: eight elements a lane.
 template <int TO, bool VEC>
-__global__ void __launch_bounds__(256) k_head_pack(const __grid_constant__ PackParams P)
+PSK_DEV void pack_matrix(const PackParams &P)
 {
     const int lane = threadIdx.x & 31;
     const int64_t warps = (int64_t)gridDim.x * 8, width = P.un ? P.ld : PIECE, pieces = (P.ld + width - 1) / width, again = P.s.rows * P.ld;
@@ -992,6 +1008,17 @@ __global__ void __launch_bounds__(256) k_head_pack(const __grid_constant__ PackP
     }
 }
 
+struct Packs { PackParams of[4]; };
+
+static __global__ void __launch_bounds__(256) k_head_pack(const __grid_constant__ Packs all)
+{
+    const PackParams &P = all.of[blockIdx.y];
+    follow();
+    if (P.to == PACK_SPLIT) { if (P.vec) pack_matrix<PACK_SPLIT, true>(P); else pack_matrix<PACK_SPLIT, false>(P); }
+    else if (P.to == PACK_F16) { if (P.vec) pack_matrix<PACK_F16, true>(P); else pack_matrix<PACK_F16, false>(P); }
+    else { if (P.vec) pack_matrix<PACK_SAME, true>(P); else pack_matrix<PACK_SAME, false>(P); }
+}
+
 // A gradient from its f32 partial sums into its place: the splits' sums in their order (and, of few rows, those of g's
 // remainder `fold` rows below), times what undoes the scales, rounded once. Four columns a thread.
 struct SumParams {
@@ -1007,6 +1034,7 @@ struct SumParams {
 
 static __global__ void __launch_bounds__(256) k_head_sum(const __grid_constant__ SumParams P)
 {
+    follow();
     const int64_t quads = (P.cols + 3) / 4, warps = (int64_t)gridDim.x * 8, chunks = (quads + 31) / 32;
     const int lane = threadIdx.x & 31;
     const float un = undo(P.scales, P.un);
