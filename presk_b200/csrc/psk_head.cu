@@ -331,7 +331,7 @@ int head_run(HeadContext &x, const psk_launch *l, void *const *table)
             T.s = s; T.ids = rids; T.t = row_operand(l->in[3], table[3], no); T.ct = rct; T.lse = rlse;
             T.ids_k = I.stride[ax_k]; T.t_k = l->in[3].stride[ax_k]; T.classes = V; T.top = (int32_t)K; T.inv_tau = inv_tau;
             T.out_ids = ids; T.start = start; T.parts = parts; T.out_p = p; T.plogp = plogp; T.coef = coef; T.lse2 = lse2; T.status = x.status; T.ctmax = g_scaled ? &scales->max_ct : nullptr;
-            HEAD_START(k_head_teacher, N, 1, (unsigned)up(K, 32), (size_t)K * 8, 1, T);
+            HEAD_START(k_head_teacher, N, 1, (unsigned)std::max<int64_t>(up(K, 32), N <= 2 * x.sms ? 256 : 128), (size_t)K * 8, 1, T);
         } else {
             LabelParams T;
             memset(&T, 0, sizeof T);
@@ -456,6 +456,7 @@ int head_run(HeadContext &x, const psk_launch *l, void *const *table)
         J.loss = rout; J.ovf = x.ovf; J.guarded = x.guarded;
         if (LSE) J.lse = row_operand(*LSE, table[h.lse], no);
         if (N >= 32 * x.sms) HEAD_START(k_head_join<32>, (N + 31) / 32, 1, 256, 0, 1, J);
+        else if (N <= 2 * x.sms) HEAD_START(k_head_join<1>, N, 1, 256, 0, 1, J);
         else HEAD_START(k_head_join<8>, (N + 7) / 8, 1, 256, 0, 1, J);
     } else if (N > 0 && !dxo.straight) {
         SumParams S;

@@ -859,7 +859,7 @@ __global__ void __launch_bounds__(256) k_head_join(const __grid_constant__ JoinP
     }
     if (X < 32) {
 #pragma unroll
-        for (int o = X; o < 32; o <<= 1) {
+        for (int o = X; o < 32; o <<= 1) { // lanes of the same row
             const float am = __shfl_xor_sync(0xffffffffu, m, o), az = __shfl_xor_sync(0xffffffffu, z, o);
             h += __shfl_xor_sync(0xffffffffu, h, o);
             join(am, az);
