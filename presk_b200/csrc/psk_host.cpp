@@ -159,6 +159,7 @@ struct Realization {
     bool blockwise_attention = false; // "order": {"kind": "device", "attention": "blockwise"} or "online"
     bool online_attention = false;    // "attention": "online": the one-pass form of the same launch
     bool merged_launches = false;     // "order": {..., "launches": "merged"}: bit-preserving rewrites of the launch list
+    bool loss_in_pieces = false;      // "loss": "pieces": the head and its loss as one launch, the logits never stored
 
     static Realization parse(const char *text)
     {
@@ -220,6 +221,12 @@ struct Realization {
             if (const Json *ml = o->get("launches")) {
                 if (ml->str == "merged") r.merged_launches = true;
                 else if (ml->str != "reference") raise(PSK_E7005, "realization: the launch list `" + ml->str + "` is not one this executor has (reference, merged)");
+            }
+            if (const Json *lo = o->get("loss")) {
+                if (lo->str == "pieces") {
+                    if (r.order != PSK_ORDER_DEVICE) raise(PSK_E7005, "realization: `loss: pieces` is part of the order `device`");
+                    r.loss_in_pieces = true;
+                } else if (lo->str != "logits") raise(PSK_E7005, "realization: the loss order `" + lo->str + "` is not one this executor has (logits, pieces)");
             }
             if (const Json *at = o->get("attention")) {
                 if (at->str == "blockwise") {
@@ -921,6 +928,81 @@ struct psk_host {
         return out;
     }
 
+    // The head's contraction and its loss as one launch that takes the vocabulary in pieces and never stores the logits
+    // (PSK_OP_HEAD_XENT; with a teacher's logits PSK_OP_HEAD_DISTILL), under the declared order `loss: pieces`. x over
+    // (rows, model), w over (model, vocab), targets over the rows (and a list, with a teacher). While magnitudes are
+    // being measured, or where the logits' site is stored in an affine format, the launches stay apart.
+    struct HeadLoss { Tensor loss, lse; };
+    bool in_pieces(const std::string &logits_site) const { return rz.loss_in_pieces && !calibrating && !rz.scaled.count(logits_site); }
+    void head_operands(psk_launch &l, const Tensor &x, const Tensor &w, const Tensor &targets, const Tensor *teacher, double tau, std::vector<const Tensor *> &ins)
+    {
+        const int no = (int)x.axes.size() - 1, list = teacher ? 1 : 0;
+        if (w.axes.size() != 2 || w.axes[0].len != x.axes.back().len || (int)targets.axes.size() != no + list) raise(PSK_E7001, "the head's loss: " + show(x.axes) + " through " + show(w.axes) + " against " + show(targets.axes));
+        for (int i = 0; i < no; ++i)
+            if (targets.axes[i].len != x.axes[i].len) raise(PSK_E7001, "the head's loss: " + show(x.axes) + " against " + show(targets.axes));
+        if (teacher && (teacher->axes.size() != targets.axes.size() || teacher->numel() != targets.numel())) raise(PSK_E7001, "the head's loss: the teacher's classes " + show(targets.axes) + " and logits " + show(teacher->axes));
+        std::vector<int64_t> inner = {w.axes[1].len, w.axes[0].len};
+        if (teacher) inner.push_back(targets.axes.back().len);
+        set_space(l, Axes(x.axes.begin(), x.axes.end() - 1), inner);
+        l.fparam[0] = tau;
+        const int naxes = no + 2 + list;
+        std::vector<int> rows, xm, tm;
+        for (int i = 0; i < no; ++i) rows.push_back(i);
+        xm = rows; xm.push_back(no + 1);
+        tm = rows;
+        if (teacher) tm.push_back(no + 2);
+        std::vector<int64_t> st, ss;
+        view(x, xm, naxes, st, ss); set_operand(l.in[0], x, st, ss);
+        view(w, {no + 1, no}, naxes, st, ss); set_operand(l.in[1], w, st, ss);
+        view(targets, tm, naxes, st, ss); set_operand(l.in[2], targets, st, ss);
+        ins = {&x, &w, &targets};
+        if (teacher) {
+            view(*teacher, tm, naxes, st, ss);
+            set_operand(l.in[3], *teacher, st, ss);
+            ins.push_back(teacher);
+        }
+    }
+    bool head_loss(const std::string &site, const Tensor &x, const Tensor &w, const Tensor &targets, const Tensor *teacher, double tau, HeadLoss &r)
+    {
+        psk_launch l;
+        memset(&l, 0, sizeof l);
+        l.op = teacher ? PSK_OP_HEAD_DISTILL : PSK_OP_HEAD_XENT;
+        std::vector<const Tensor *> ins;
+        head_operands(l, x, w, targets, teacher, tau, ins);
+        const Axes outer(x.axes.begin(), x.axes.end() - 1);
+        l.dtype = site_dtype(site);
+        r.loss = fresh(outer, l.dtype);
+        r.lse = fresh(outer, PSK_F32);
+        set_operand(l.in[ins.size()], r.lse, contiguous(outer), {});
+        ins.push_back(&r.lse);
+        set_operand(l.out, r.loss, contiguous(outer), {});
+        return run(l, teacher ? "head_distill[pieces]" : "head_xent[pieces]", ins, r.loss, !teacher);
+    }
+    // Its gradients: dx returned, dw beside it, both in the operands' type.
+    Tensor head_loss_vjp(const std::string &site, const Tensor &x, const Tensor &w, const Tensor &targets, const Tensor *teacher, double tau, const Tensor &ct, const HeadLoss &r, Tensor *dw)
+    {
+        psk_launch l;
+        memset(&l, 0, sizeof l);
+        l.op = teacher ? PSK_OP_HEAD_DISTILL_VJP : PSK_OP_HEAD_XENT_VJP;
+        std::vector<const Tensor *> ins;
+        head_operands(l, x, w, targets, teacher, tau, ins);
+        const int no = (int)x.axes.size() - 1, naxes = no + 2 + (teacher ? 1 : 0);
+        std::vector<int> rows, xm;
+        for (int i = 0; i < no; ++i) rows.push_back(i);
+        xm = rows; xm.push_back(no + 1);
+        std::vector<int64_t> st, ss;
+        l.dtype = x.dtype;
+        current_site = site;
+        Tensor dx = fresh(x.axes, x.dtype);
+        *dw = fresh(w.axes, w.dtype);
+        view(ct, rows, naxes, st, ss); set_operand(l.in[ins.size()], ct, st, ss); ins.push_back(&ct);
+        view(r.lse, rows, naxes, st, ss); set_operand(l.in[ins.size()], r.lse, st, ss); ins.push_back(&r.lse);
+        view(*dw, {no + 1, no}, naxes, st, ss); set_operand(l.in[ins.size()], *dw, st, ss); ins.push_back(dw);
+        view(dx, xm, naxes, st, ss); set_operand(l.out, dx, st, {});
+        run(l, teacher ? "head_distill_vjp[pieces]" : "head_xent_vjp[pieces]", ins, dx);
+        return dx;
+    }
+
     // ---- indexing (lower.rs:1421-1437, 1554-1750) ------------------------------------------
     Tensor embed(const std::string &site, const Tensor &table, const Tensor &ids)
     {
@@ -1544,6 +1626,14 @@ struct psk_host {
     // llama.psk:121-134. %0 θ, %1 ids.
     Tensor llama_apply(const Tensor &ids)
     {
+        Tensor logits = dot("Llama.apply/%11", llama_hidden(ids), param("head"));
+        logits.axes.back().name = "vocab";
+        return logits;
+    }
+
+    // `apply` up to the last norm: the rows that the head reads.
+    Tensor llama_hidden(const Tensor &ids)
+    {
         const std::string f = "Llama.apply";
         const int64_t T = ids.axes[1].len, L = C("L");
         Tensor mask = causal_mask(f + "/%2", "seq", T);
@@ -1552,18 +1642,42 @@ struct psk_host {
         Tensor phi = llama_angles(T);
         Tensor x = e;
         for (int64_t l = 0; l < L; ++l) x = llama_block(l, x, mask, phi);
-        Tensor h = llama_rmsnorm(param("norm.γ"), x);
-        Tensor logits = dot(f + "/%11", h, param("head"));
-        logits.axes.back().name = "vocab";
-        return logits;
+        return llama_rmsnorm(param("norm.γ"), x);
+    }
+
+    Tensor llama_head()
+    {
+        Tensor head = param("head");
+        head.axes = {{"model", C("D")}, {"vocab", C("V")}};
+        return head;
     }
 
     // llama.psk:140-142. %0 θ, %1 batch, %2 x, %3 y.
     Tensor llama_loss(const Tensor &ids, const Tensor &y)
     {
-        Tensor logits = llama_apply(ids);
+        Tensor h = llama_hidden(ids);
+        HeadLoss r;
+        if (in_pieces("Llama.apply/%11") && head_loss("loss/%5", h, llama_head(), y, nullptr, 1.0, r)) return reduce_all("loss/%6", PSK_REDUCE_MEAN, r.loss);
+        Tensor logits = dot("Llama.apply/%11", h, param("head"));
+        logits.axes.back().name = "vocab";
         Tensor ce = cross_entropy("loss/%5", logits, y);
         return reduce_all("loss/%6", PSK_REDUCE_MEAN, ce);
+    }
+
+    // Distillation from a teacher's top logits in the place of `loss`: the mean over the rows of the divergence of the
+    // teacher's distribution over `classes` [batch, seq, top] (its logits `teacher`) from softmax(logits / TEMP). No
+    // counterpart in the reference; one launch, so only under `loss: pieces`.
+    double distill_temperature()
+    {
+        if (!in_pieces("Llama.apply/%11")) raise(PSK_E7005, "distill: the loss is taken in pieces of the vocabulary (\"order\": {\"kind\": \"device\", \"loss\": \"pieces\"}), the logits' site in a float type");
+        return (double)C("TEMP", 1);
+    }
+    Tensor llama_distill(const Tensor &ids, const Tensor &classes, const Tensor &teacher)
+    {
+        const double tau = distill_temperature();
+        HeadLoss r;
+        head_loss("distill/loss", llama_hidden(ids), llama_head(), classes, &teacher, tau, r);
+        return reduce_all("distill/mean", PSK_REDUCE_MEAN, r.loss);
     }
 
     // `prefill`: `apply` on a window, keeping every layer's keys and values. `step`: one new position a sequence.
@@ -2177,8 +2291,10 @@ struct psk_host {
         return g;
     }
 
-    Tensor llama_loss_grad(const Tensor &ids, const Tensor &y)
+    // With a teacher's logits (`distill_grad`) `y` holds its classes, and the loss is llama_distill's.
+    Tensor llama_loss_grad(const Tensor &ids, const Tensor &y, const Tensor *teacher = nullptr)
     {
+        const double tau = teacher ? distill_temperature() : 1.0;
         const std::string f = "loss_grad";
         const int64_t T = ids.axes[1].len, L = C("L");
         Tensor mask = causal_mask("Llama.apply/%2", "seq", T);
@@ -2199,19 +2315,31 @@ struct psk_host {
         }
         NormKept nf;
         Tensor hn = train_norm(param("norm.γ"), x, nf);
-        Tensor head = param("head");
-        head.axes = {{"model", C("D")}, {"vocab", C("V")}};
-        Tensor logits = dot("Llama.apply/%11", hn, head);
-        logits.axes.back().name = "vocab";
-        Tensor ce = cross_entropy("loss/%5", logits, y);
+        Tensor head = llama_head();
         // the reverse pass
-        Tensor ct1 = scalar(f + "/ct", 1.0);
-        Tensor c_ce = fused(f + "/mean_vjp", {U(PSK_DIV_N, 0, (int)ce.numel())}, {&ct1}, "mean_vjp", nullptr, &ce.axes);
-        Tensor c_logits = cross_entropy_vjp(f + "/cross_entropy_vjp", logits, y, c_ce);
-        const std::vector<std::string> xm = {"batch", "seq", "model"}, xv = {"batch", "seq", "vocab"};
-        Tensor c_hn = ein(f + "/head.dot_vjp_l", xm, {xv, {"model", "vocab"}}, {&c_logits, &head}, "dot_vjp_l");
         std::map<std::string, Tensor> out;
-        out["head"] = ein(f + "/head.dot_vjp_r", {"model", "vocab"}, {xm, xv}, {&hn, &c_logits}, "dot_vjp_r");
+        Tensor c_hn;
+        auto mean_vjp = [&](const Tensor &loss) {
+            Tensor ct1 = scalar(f + "/ct", 1.0);
+            return fused(f + "/mean_vjp", {U(PSK_DIV_N, 0, (int)loss.numel())}, {&ct1}, "mean_vjp", nullptr, &loss.axes);
+        };
+        // in pieces: the loss and both of the head's gradients without the logits or their cotangent, where the gradients' sites are of the operands' type
+        HeadLoss r;
+        const bool same = site_dtype(f + "/head.dot_vjp_l") == hn.dtype && site_dtype(f + "/head.dot_vjp_r") == head.dtype;
+        if (teacher && !same) raise(PSK_E7005, "distill_grad: the head's gradients are stored in its operands' type");
+        if (in_pieces("Llama.apply/%11") && same && head_loss(teacher ? "distill/loss" : "loss/%5", hn, head, y, teacher, tau, r)) {
+            Tensor c_ce = mean_vjp(r.loss);
+            c_hn = head_loss_vjp(f + "/head.dot_vjp_l", hn, head, y, teacher, tau, c_ce, r, &out["head"]);
+        } else {
+            Tensor logits = dot("Llama.apply/%11", hn, head);
+            logits.axes.back().name = "vocab";
+            Tensor ce = cross_entropy("loss/%5", logits, y);
+            Tensor c_ce = mean_vjp(ce);
+            Tensor c_logits = cross_entropy_vjp(f + "/cross_entropy_vjp", logits, y, c_ce);
+            const std::vector<std::string> xm = {"batch", "seq", "model"}, xv = {"batch", "seq", "vocab"};
+            c_hn = ein(f + "/head.dot_vjp_l", xm, {xv, {"model", "vocab"}}, {&c_logits, &head}, "dot_vjp_l");
+            out["head"] = ein(f + "/head.dot_vjp_r", {"model", "vocab"}, {xm, xv}, {&hn, &c_logits}, "dot_vjp_r");
+        }
         Tensor ct = train_norm_bwd(param("norm.γ"), nf, c_hn, &out["norm.γ"]);
         static const char *stacked[] = {"blocks.n1.γ", "blocks.n2.γ", "blocks.attn.wq", "blocks.attn.wk", "blocks.attn.wv", "blocks.attn.wo", "blocks.ff.gate.w", "blocks.ff.up.w", "blocks.ff.down.w"};
         for (auto path : stacked) out[path] = zeros(f + "/" + path, param(path).axes);
@@ -2546,6 +2674,8 @@ struct psk_host {
             if (entry == "apply") { need(1); return llama_apply(in[0]); }
             if (entry == "loss") { need(2); return llama_loss(in[0], in[1]); }
             if (entry == "loss_grad") { need(2); return llama_loss_grad(in[0], in[1]); }
+            if (entry == "distill") { need(3); return llama_distill(in[0], in[1], in[2]); }
+            if (entry == "distill_grad") { need(3); return llama_loss_grad(in[0], in[1], &in[2]); }
             if (entry == "prefill") { need(1); return llama_prefill(in[0]); }
             if (entry == "step") { need(1); return llama_step(in[0]); }
             if (entry == "attention" || entry == "attention3") {
@@ -2597,6 +2727,7 @@ struct psk_host {
     {
         std::vector<std::string> names;
         if (model == "llama" && (entry == "attention" || entry == "attention3")) names = {"batch", "seq", "model"};
+        else if (model == "llama" && (entry == "distill" || entry == "distill_grad") && i > 0) names = {"batch", "seq", "top"};
         else if (model == "llama" || model == "gpt") names = {"batch", "seq"};
         else if (model == "mlp") names = i == 0 ? std::vector<std::string>{"batch", "model"} : std::vector<std::string>{"batch"};
         else if (model == "mlp_spec") names = {"batch", "model"};
