@@ -125,52 +125,65 @@ int pairs_of(K kernel, const HeadContext &x)
     return n;
 }
 
-template <int MODE, bool REST, bool PAIR>
-int launch(HeadContext &x, const CUtensorMap &ma, const CUtensorMap &mb, const Params &P)
+template <int MODE, bool REST, bool PAIR, int JOBS>
+int launch(HeadContext &x, const Jobs<JOBS> &jobs)
 {
-    // once a device: the kernel's shared memory, and how many pairs fit (bits 0: set; the rest the number)
+    auto kernel = k_head<MODE, PAIR, REST, JOBS>;
+    // once a device: the kernel's shared memory, and how many pairs fit (bit 0: known; the rest the number)
     static std::atomic<int> known[64];
     int device = 0;
     HEAD_TRY(cudaGetDevice(&device));
     int k = device < 64 ? known[device].load(std::memory_order_relaxed) : 0;
     if (!k) {
-        HEAD_TRY(cudaFuncSetAttribute(k_head<MODE, PAIR, REST>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_TOTAL));
-        k = 1 + 2 * (PAIR ? pairs_of(k_head<MODE, PAIR, REST>, x) : 0);
+        HEAD_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_TOTAL));
+        k = 1 + 2 * (PAIR ? pairs_of(kernel, x) : 0);
         if (device < 64) known[device].store(k, std::memory_order_relaxed);
     }
-    const int64_t tiles = (int64_t)P.tiles_m * P.tiles_n * P.splits;
+    int64_t tiles = 0;
+    for (int j = 0; j < JOBS; ++j) tiles += (int64_t)jobs.of[j].p.tiles_m * jobs.of[j].p.tiles_n * jobs.of[j].p.splits;
     if (PAIR && k >> 1 < 1) return fail(x, PSK_E10001, "head: no pair of SMs for a cluster");
-    return enqueue(x, k_head<MODE, PAIR, REST>, PAIR ? 2 * std::min<int64_t>(tiles, k >> 1) : std::min<int64_t>(tiles, x.sms), 1, THREADS, Cfg::SMEM_TOTAL, PAIR ? 2 : 1, ma, mb, P);
+    return enqueue(x, kernel, PAIR ? 2 * std::min<int64_t>(tiles, k >> 1) : std::min<int64_t>(tiles, x.sms), 1, THREADS, Cfg::SMEM_TOTAL, PAIR ? 2 : 1, jobs);
 }
 
-// One product a·bᵀ and what MODE makes of it.
-template <int MODE, bool REST = false>
-int product(HeadContext &x, Params P, const Operand &a, const Operand &b, int f16)
+// A product a·bᵀ: its division into tiles and its tensor maps. `together`: with another in one launch, whose ring the
+// two then share (whole tiles of a).
+template <int MODE>
+int describe(HeadContext &x, Job &j, Params P, const Operand &a, const Operand &b, int f16, bool together, bool *pair)
 {
     P.m = a.rows; P.n = b.rows;
     if (MODE != MODE_OUT) P.splits = 1;
     const int64_t tiles = ((P.m + BM - 1) / BM) * ((P.n + BN - 1) / BN);
     // pairs of CTAs where there are rows for two and tiles for everybody (see Cfg)
-    const bool pair = P.m > BM && tiles >= x.sms;
-    P.tiles_m = (uint32_t)((P.m + (pair ? 2 : 1) * BM - 1) / ((pair ? 2 : 1) * BM)); P.tiles_n = (uint32_t)((P.n + BN - 1) / BN);
-    if (tiles > 0x7fffffff / std::max<int64_t>(1, P.splits)) return fail(x, PSK_E7005, "head: more tiles than one launch counts");
-    const int a_rows = !pair && a.k_contiguous ? (int)std::min<int64_t>(BM, up(P.m, 8)) : BM;
+    *pair = P.m > BM && tiles >= x.sms;
+    P.tiles_m = (uint32_t)((P.m + (*pair ? 2 : 1) * BM - 1) / ((*pair ? 2 : 1) * BM)); P.tiles_n = (uint32_t)((P.n + BN - 1) / BN);
+    if (tiles > 0x3fffffff / std::max<int64_t>(1, P.splits)) return fail(x, PSK_E7005, "head: more tiles than one launch counts");
+    const int a_rows = !*pair && !together && a.k_contiguous ? (int)std::min<int64_t>(BM, up(P.m, 8)) : BM;
     P.a_stage = a_rows * BK * 2;
-    P.stages = Cfg::stages(P.a_stage, (pair ? BN / 2 : BN) * BK * 2, MODE != MODE_STATS);
-    CUtensorMap ma, mb;
-    if (!map_of(x, &ma, a, f16, a_rows, &P.a_blocks) || !map_of(x, &mb, b, f16, pair ? BN / 2 : BN, &P.b_blocks)) return fail(x, PSK_E10001, "head: an operand's layout does not make a tensor map");
+    P.stages = Cfg::stages(P.a_stage, (*pair ? BN / 2 : BN) * BK * 2, MODE != MODE_STATS);
+    if (!map_of(x, &j.a, a, f16, a_rows, &P.a_blocks) || !map_of(x, &j.b, b, f16, *pair ? BN / 2 : BN, &P.b_blocks)) return fail(x, PSK_E10001, "head: an operand's layout does not make a tensor map");
     P.kb_k = (int32_t)((a.k + BK - 1) / BK);
-    P.nprod = a.planes == 2 ? 3 : 1;
+    P.nprod = a.planes == 2 ? b.planes + 1 : 1;
     if (MODE != MODE_OUT) P.kb_split = P.kb_k;
     // Steps an accumulator: 512 products of the summed axis (384 of f32's, three a block). Results of 16 bits, dx and dw, keep one
     // accumulator throughout, and g's logits 1024 products: what truncation loses there is far below their rounding.
-    P.chunk = MODE == MODE_OUT && a.planes == 1 ? 1 << 28 : P.nprod == 3 ? 6 : MODE == MODE_GRAD ? 16 : 8;
+    P.chunk = MODE == MODE_OUT && P.nprod < 3 ? 1 << 28 : P.nprod == 3 ? 6 : MODE == MODE_GRAD ? 16 : 8;
     // a panel's columns of b stay in a part of the L2 while a's rows stream past them
     P.panel = (uint32_t)std::min<int64_t>(P.tiles_n, std::max<int64_t>(8, (16ll << 20) / std::max<int64_t>(1, BN * a.k * 2 * a.planes)));
     P.in_f16 = f16; P.a_m_major = !a.k_contiguous; P.b_n_major = !b.k_contiguous;
     P.status = x.status;
     x.flops += 2.0 * (double)P.m * (double)P.n * (double)a.k;
-    return pair ? launch<MODE, REST, true>(x, ma, mb, P) : launch<MODE, REST, false>(x, ma, mb, P);
+    j.p = P;
+    return PSK_OK;
+}
+
+template <int MODE, bool REST = false>
+int product(HeadContext &x, const Params &P, const Operand &a, const Operand &b, int f16)
+{
+    Jobs<1> jobs;
+    bool pair;
+    const int r = describe<MODE>(x, jobs.of[0], P, a, b, f16, false, &pair);
+    if (r != PSK_OK) return r;
+    return pair ? launch<MODE, REST, true, 1>(x, jobs) : launch<MODE, REST, false, 1>(x, jobs);
 }
 
 // Blocks of eight warps for `work` warps' worth.
@@ -261,6 +274,9 @@ int head_run(HeadContext &x, const psk_launch *l, void *const *table)
     // copies of x and w in binary16 (6 bytes an element of w), which is what bf16 takes for more.
     const bool rest = vjp && !f32 && N <= 256, conv = vjp && dt == PSK_BF16 && !rest;
     const int64_t Ng = rest ? 2 * N : N;
+    // For dx the remainder is rows of the same tile where the head is large (up to 64 rows: w then passes once) and a second
+    // plane of g otherwise, whose product lands in the same sums.
+    const bool small = D * V <= 16 << 20, fold = rest && 2 * N <= BM && !small;
     const int g_f16 = f32 || conv || dt == PSK_F16, in_f16 = f32 || dt == PSK_F16;
     const bool g_scaled = vjp && g_f16, any_scale = f32 || g_scaled;
 
@@ -290,7 +306,7 @@ int head_run(HeadContext &x, const psk_launch *l, void *const *table)
     const bool dw_v_inner = DW && (DW->stride[ax_v] == 1 || V == 1);
     const int64_t dw_ld = DW ? DW->stride[dw_v_inner ? ax_d : ax_v] : 0, dx_ld = vjp ? row_stride(O) : 0;
     Out dxo{}, dwo{};
-    if (vjp && N) dxo = plan(Ng, D, Vc, !rest && pieces == 1 && dx_ld && O.stride[ax_d] == 1);
+    if (vjp && N) dxo = plan(fold ? Ng : N, D, Vc, !fold && pieces == 1 && dx_ld && O.stride[ax_d] == 1);
     if (DW && N) dwo = plan(dw_v_inner ? D : Vc, dw_v_inner ? Vc : D, Ng, DW->stride[dw_v_inner ? ax_v : ax_d] == 1);
 
     int32_t *ids;
@@ -422,23 +438,43 @@ int head_run(HeadContext &x, const psk_launch *l, void *const *table)
         Q.un = dxo.straight ? UN_DX : UN_NONE; Q.accumulate = piece > 0;
         Q.out_vec = !dxo.straight || (aligned(rout.p) && dx_ld * eb % 16 == 0 && D * eb % 16 == 0);
         Q.ovf = x.guarded && dxo.straight ? x.ovf : nullptr;
-        const Operand gk{g, Ng, vn, g_ld, true, planes, N * g_ld}, wk{bd.p, D, vn, bd.ld, v_inner, planes, bd.plane};
-        r = product<MODE_OUT>(x, Q, gk, wk, g_f16);
-        if (r != PSK_OK) return r;
-        // 7. dw of the piece = xᵀ·g: both operands along the rows
-        if (DW) {
+        const Operand gk = f32 || (rest && !fold) ? Operand{g, N, vn, g_ld, true, 2, N * g_ld} : Operand{g, Ng, vn, g_ld, true, 1, 0};
+        const Operand wk{bd.p, D, vn, bd.ld, v_inner, planes, bd.plane};
+        // 7. dw of the piece = xᵀ·g: both operands along the rows. Small ones go with dx in one launch (vjp of 16 x 704 x 392:
+        // WITH us against WITHOUT); where dx streams a large head, its ring is better kept to itself.
+        if (!DW) {
+            r = product<MODE_OUT>(x, Q, gk, wk, g_f16);
+            if (r != PSK_OK) return r;
+        } else {
             uint8_t *dst = (uint8_t *)table[h.dw] + (DW->offset + v0 * DW->stride[ax_v]) * eb;
             const Operand xr{xd, D, Ng, Dp, false, planes, N * Dp}, gr{g, vn, Ng, g_ld, false, planes, N * g_ld};
             const int64_t cols = dw_v_inner ? vn : D;
-            memset(&Q, 0, sizeof Q);
-            Q.scales = scales;
-            Q.splits = (uint32_t)dwo.splits; Q.kb_split = dwo.kb_split;
-            Q.out = dwo.straight ? (void *)dst : dwp; Q.out_ld = dwo.straight ? dw_ld : dwo.ld; Q.out_dtype = dwo.straight ? dt : PSK_F32;
-            Q.un = dwo.straight ? UN_DW : UN_NONE;
-            Q.out_vec = !dwo.straight || (aligned(dst) && dw_ld * eb % 16 == 0 && cols * eb % 16 == 0);
-            Q.ovf = x.guarded && dwo.straight ? x.ovf : nullptr;
-            r = product<MODE_OUT>(x, Q, dw_v_inner ? xr : gr, dw_v_inner ? gr : xr, g_f16);
-            if (r != PSK_OK) return r;
+            Params R;
+            memset(&R, 0, sizeof R);
+            R.scales = scales;
+            R.splits = (uint32_t)dwo.splits; R.kb_split = dwo.kb_split;
+            R.out = dwo.straight ? (void *)dst : dwp; R.out_ld = dwo.straight ? dw_ld : dwo.ld; R.out_dtype = dwo.straight ? dt : PSK_F32;
+            R.un = dwo.straight ? UN_DW : UN_NONE;
+            R.out_vec = !dwo.straight || (aligned(dst) && dw_ld * eb % 16 == 0 && cols * eb % 16 == 0);
+            R.ovf = x.guarded && dwo.straight ? x.ovf : nullptr;
+            const Operand &da = dw_v_inner ? xr : gr, &db = dw_v_inner ? gr : xr;
+            const double flops = x.flops;
+            bool pair0 = false, pair1 = false;
+            Jobs<2> two;
+            if (small) {
+                r = describe<MODE_OUT>(x, two.of[0], Q, gk, wk, g_f16, true, &pair0);
+                if (r == PSK_OK) r = describe<MODE_OUT>(x, two.of[1], R, da, db, g_f16, true, &pair1);
+                if (r != PSK_OK) return r;
+            }
+            if (small && pair0 == pair1) {
+                r = pair0 ? launch<MODE_OUT, false, true, 2>(x, two) : launch<MODE_OUT, false, false, 2>(x, two);
+                if (r != PSK_OK) return r;
+            } else {
+                x.flops = flops;
+                r = product<MODE_OUT>(x, Q, gk, wk, g_f16);
+                if (r == PSK_OK) r = product<MODE_OUT>(x, R, da, db, g_f16);
+                if (r != PSK_OK) return r;
+            }
             if (!dwo.straight) {
                 SumParams S;
                 memset(&S, 0, sizeof S);
@@ -461,7 +497,7 @@ int head_run(HeadContext &x, const psk_launch *l, void *const *table)
     } else if (N > 0 && !dxo.straight) {
         SumParams S;
         memset(&S, 0, sizeof S);
-        S.s = s; S.part = dxp; S.parts = dxo.splits; S.part_rows = dxo.m; S.ld = dxo.ld; S.fold = rest ? N : 0; S.cols = D; S.col_stride = O.stride[ax_d];
+        S.s = s; S.part = dxp; S.parts = dxo.splits; S.part_rows = dxo.m; S.ld = dxo.ld; S.fold = fold ? N : 0; S.cols = D; S.col_stride = O.stride[ax_d];
         S.scales = scales; S.un = UN_DX; S.dst = rout; S.ovf = x.ovf; S.guarded = x.guarded;
         HEAD_START(k_head_sum, warps_of(x, N * ((D + 127) / 128)), 1, 256, 0, 1, S);
     } else if (N == 0 && DW) { // no rows: a gradient of zeros

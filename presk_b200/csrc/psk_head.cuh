@@ -56,9 +56,10 @@ constexpr int COLS = 64; // columns of a tile an epilogue thread holds: a part o
 
 enum { MODE_STATS = 0, MODE_GRAD = 1, MODE_OUT = 2 };
 
-// Planes of the partial product q of two operands of two planes: hi·hi, hi·lo, lo·hi.
-PSK_DEV int plane_a(int q) { return q == 2; }
-PSK_DEV int plane_b(int q) { return q == 1; }
+// Planes of the partial product q: of two operands of two planes (3 products) hi·hi, hi·lo, lo·hi; of a's two and b's
+// one (2 products) hi·b, lo·b.
+PSK_DEV int plane_a(int q, int nprod) { return q == nprod - 1; }
+PSK_DEV int plane_b(int q, int nprod) { return nprod == 3 && q == 1; }
 
 // The greatest finite |element| of the operands, as f32 bits (0: not scaled), and the powers of two made of them.
 struct Scales {
@@ -87,7 +88,7 @@ PSK_DEV float undo(const Scales *s, int un)
 struct Params {
     int64_t m, n;                 // rows and columns of the product
     uint32_t tiles_m, tiles_n, splits, panel; // their product below 2^31
-    int32_t kb_k, nprod;          // blocks of 64 along the summed axis; partial products a block (1, or 3 of two planes)
+    int32_t kb_k, nprod;          // blocks of 64 along the summed axis; partial products a block (1; 2 where a has two planes; 3 where both have)
     int32_t kb_split;             // blocks of the summed axis a split
     int32_t chunk;                // steps (block, partial product) in one accumulator before it is added into registers
     int32_t in_f16, a_m_major, b_n_major;
@@ -274,13 +275,25 @@ PSK_DEV void store_rows_any(uint4 *stage, int lane, const uint32_t (&w)[16], uin
     __syncwarp();
 }
 
+// A product and its tensor maps. Two of them (dx and dw, which read the same g) go in one launch where that is one
+// kernel's latency less: the second's tiles follow the first's.
+struct Job {
+    CUtensorMap a, b;
+    Params p;
+};
+template <int JOBS>
+struct Jobs {
+    Job of[JOBS];
+};
+
 // The product of a persistent CTA's tiles, and what MODE makes of it. Bounds: the tensor pipe (2·m·n·k flops) for many
 // rows; for few, the bytes of the second operand.
-template <int MODE, bool PAIR, bool REST = false>
-__global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ Params P)
+template <int MODE, bool PAIR, bool REST = false, int JOBS = 1>
+__global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ Jobs<JOBS> jobs)
 {
     constexpr int B_BYTES = (PAIR ? BN / 2 : BN) * BK * 2, MOST = Cfg::MOST_STAGES, STAGE_OUT = MODE == MODE_STATS ? 0 : EPILOGUE * 32 * 64;
-    const int STAGES = P.stages, A_BYTES = P.a_stage;
+    const int STAGES = jobs.of[0].p.stages, A_BYTES = jobs.of[0].p.a_stage; // the same for both
+    uint32_t *const status = jobs.of[0].p.status;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     // a's ring before b's: a short tile of a is read past its end, into what lies behind
@@ -319,10 +332,12 @@ __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ CUt
     const uint32_t tmem_base = *tmem_slot;
     follow();
 
-    const uint32_t per_split = P.tiles_m * P.tiles_n, total = per_split * P.splits;
+    auto tiles_of = [&](const Params &P) { return P.tiles_m * P.tiles_n * P.splits; };
+    const uint32_t total0 = tiles_of(jobs.of[0].p), total = JOBS == 2 ? total0 + tiles_of(jobs.of[JOBS - 1].p) : total0;
     const uint32_t tile0 = PAIR ? blockIdx.x >> 1 : blockIdx.x, tile_step = PAIR ? gridDim.x >> 1 : gridDim.x;
+    auto job_of = [&](uint32_t t) { return JOBS == 2 && t >= total0 ? JOBS - 1 : 0; };
     // the steps of a split: blocks kb_first .. of the summed axis, nprod partial products each
-    auto steps_of = [&](uint32_t sp, int &kb_first) {
+    auto steps_of = [&](const Params &P, uint32_t sp, int &kb_first) {
         kb_first = (int)sp * P.kb_split;
         const int left = P.kb_k - kb_first;
         return (left < P.kb_split ? left : P.kb_split) * P.nprod;
@@ -337,27 +352,29 @@ __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ CUt
             const bool of_a = warp == 0;
             uint32_t stage = 0, phase = 0;
             bool ok = true;
-            const CUtensorMap *map = of_a ? &map_a : &map_b;
             const uint32_t dst0 = tc::smem_u32(of_a ? smem_a : smem_b), dst_step = of_a ? (uint32_t)A_BYTES : (uint32_t)B_BYTES;
-            const uint32_t full_at = PAIR ? tc2::map_to_rank(full0, 0) : full0, bytes = (PAIR ? 2 : 1) * (A_BYTES + B_BYTES), nprod = P.nprod;
-            const bool counts = of_a && (!PAIR || rank == 0), blocks = (of_a ? P.a_blocks : P.b_blocks) != 0;
-            const int boxes = (of_a ? P.a_m_major : P.b_n_major) && !blocks ? (int)(dst_step / 8192) : 0; // 64 x 64 each; 0: one load
-            const bool k_first = !(of_a ? P.a_m_major : P.b_n_major);
-            auto load = [&](uint32_t dst, uint32_t bar, int c0, int c1, int c2, int c3) {
-                if (PAIR) tc2::tma_load_4d_pair(dst, map, bar, c0, c1, c2, c3);
-                else tc::tma_load_4d(dst, map, bar, c0, c1, c2, c3);
-            };
+            const uint32_t full_at = PAIR ? tc2::map_to_rank(full0, 0) : full0, bytes = (PAIR ? 2 : 1) * (A_BYTES + B_BYTES);
+            const bool counts = of_a && (!PAIR || rank == 0);
             for (uint32_t t = tile0; t < total && ok; t += tile_step) {
+                const int which = job_of(t);
+                const Params &P = jobs.of[which].p;
+                const CUtensorMap *map = of_a ? &jobs.of[which].a : &jobs.of[which].b;
+                auto load = [&](uint32_t dst, uint32_t bar, int c0, int c1, int c2, int c3) {
+                    if (PAIR) tc2::tma_load_4d_pair(dst, map, bar, c0, c1, c2, c3);
+                    else tc::tma_load_4d(dst, map, bar, c0, c1, c2, c3);
+                };
+                const bool k_first = !(of_a ? P.a_m_major : P.b_n_major), blocks = (of_a ? P.a_blocks : P.b_blocks) != 0;
+                const int boxes = (int)(dst_step / 8192), nprod = P.nprod; // boxes: of 64 x 64, where a tile is not one load
                 uint32_t mt, nt;
-                const uint32_t sp = t / per_split;
-                tile_at(t - sp * per_split, P.tiles_m, P.tiles_n, P.panel, mt, nt);
+                const uint32_t tl = which ? t - total0 : t, per_split = P.tiles_m * P.tiles_n, sp = tl / per_split;
+                tile_at(tl - sp * per_split, P.tiles_m, P.tiles_n, P.panel, mt, nt);
                 const int r0 = of_a ? (int)(PAIR ? mt * 2 + rank : mt) * BM : (int)nt * BN + (PAIR ? (int)rank * (BN / 2) : 0);
                 int kb0;
-                const int steps = steps_of(sp, kb0);
-                int k0 = kb0 * BK, plane = 0;
-                uint32_t q = 0;
+                const int steps = steps_of(P, sp, kb0);
+                int k0 = kb0 * BK, plane = 0, q = 0;
+                if (nprod > 1) plane = of_a ? plane_a(0, nprod) : plane_b(0, nprod);
                 for (int s = 0; s < steps; ++s) {
-                    ok = wait(empty0 + 8 * stage, phase ^ 1u, abort_flag, P.status, 1u);
+                    ok = wait(empty0 + 8 * stage, phase ^ 1u, abort_flag, status, 1u);
                     if (!ok) break;
                     const uint32_t dst = dst0 + stage * dst_step, fb = full_at + 8 * stage;
                     if (counts) tc::mbar_expect_tx(full0 + 8 * stage, bytes);
@@ -369,31 +386,35 @@ __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ CUt
                     if (nprod == 1) k0 += BK;
                     else {
                         if (++q == nprod) { q = 0; k0 += BK; }
-                        plane = of_a ? plane_a(q) : plane_b(q);
+                        plane = of_a ? plane_a(q, nprod) : plane_b(q, nprod);
                     }
                 }
             }
         }
         if (warp == 1 && lane == 0 && rank == 0) {
-            const uint32_t idesc = PAIR ? tc2::instr_desc_pair(P.in_f16, P.b_n_major) | (P.a_m_major ? 1u << 15 : 0u) : tc::instr_desc(P.in_f16, P.b_n_major, BN, P.a_m_major);
-            const uint64_t ad = P.a_m_major ? tc::smem_desc(tc::smem_u32(smem_a), 8192, 1024) : tc::smem_desc(tc::smem_u32(smem_a), 16, 1024);
-            const uint64_t bd = P.b_n_major ? tc::smem_desc(tc::smem_u32(smem_b), 8192, 1024) : tc::smem_desc(tc::smem_u32(smem_b), 16, 1024);
-            const uint32_t a_hi = (uint32_t)(ad >> 32), b_hi = (uint32_t)(bd >> 32), a_lo0 = (uint32_t)ad, b_lo0 = (uint32_t)bd; // (shared memory ends below 2^18: the address never carries out of its 14 bits)
-            const uint32_t ak = P.a_m_major ? 2048 >> 4 : 32 >> 4, bk = P.b_n_major ? 2048 >> 4 : 32 >> 4; // 16 further along the summed axis
-            const uint32_t a_step = (uint32_t)A_BYTES >> 4, chunk = (uint32_t)P.chunk;
-            uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0, a_lo = a_lo0, b_lo = b_lo0;
+            const uint32_t a_step = (uint32_t)A_BYTES >> 4;
+            uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
             bool ok = true;
             for (uint32_t t = tile0; t < total && ok; t += tile_step) {
+                const int which = job_of(t);
+                const Params &P = jobs.of[which].p;
+                const uint32_t idesc = PAIR ? tc2::instr_desc_pair(P.in_f16, P.b_n_major) | (P.a_m_major ? 1u << 15 : 0u) : tc::instr_desc(P.in_f16, P.b_n_major, BN, P.a_m_major);
+                const uint64_t ad = P.a_m_major ? tc::smem_desc(tc::smem_u32(smem_a), 8192, 1024) : tc::smem_desc(tc::smem_u32(smem_a), 16, 1024);
+                const uint64_t bd = P.b_n_major ? tc::smem_desc(tc::smem_u32(smem_b), 8192, 1024) : tc::smem_desc(tc::smem_u32(smem_b), 16, 1024);
+                const uint32_t a_hi = (uint32_t)(ad >> 32), b_hi = (uint32_t)(bd >> 32), a_lo0 = (uint32_t)ad, b_lo0 = (uint32_t)bd; // (shared memory ends below 2^18: the address never carries out of its 14 bits)
+                const uint32_t ak = P.a_m_major ? 2048 >> 4 : 32 >> 4, bk = P.b_n_major ? 2048 >> 4 : 32 >> 4; // 16 further along the summed axis
+                const uint32_t chunk = (uint32_t)P.chunk;
+                uint32_t a_lo = a_lo0 + stage * a_step, b_lo = b_lo0 + stage * (B_BYTES >> 4);
                 int kb0;
-                int left = steps_of(t / per_split, kb0);
+                int left = steps_of(P, (which ? t - total0 : t) / (P.tiles_m * P.tiles_n), kb0);
                 while (left > 0 && ok) { // a chunk
                     const uint32_t n = (uint32_t)left < chunk ? (uint32_t)left : chunk;
                     left -= (int)n;
-                    ok = wait(tempty0 + 8 * acc, acc_phase ^ 1u, abort_flag, P.status, 2u);
+                    ok = wait(tempty0 + 8 * acc, acc_phase ^ 1u, abort_flag, status, 2u);
                     if (!ok) break;
                     const uint32_t tacc = tmem_base + acc * BN;
                     for (uint32_t s = 0; s < n; ++s) {
-                        ok = wait(full0 + 8 * stage, phase, abort_flag, P.status, 3u);
+                        ok = wait(full0 + 8 * stage, phase, abort_flag, status, 3u);
                         if (!ok) break;
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                         umma<PAIR>(tacc, a_lo, a_hi, b_lo, b_hi, idesc, s);
@@ -419,12 +440,14 @@ __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ CUt
         uint32_t acc = 0, acc_phase = 0;
         bool ok = true;
         for (uint32_t t = tile0; t < total && ok; t += tile_step) {
+            const int which = job_of(t);
+            const Params &P = jobs.of[which].p;
             uint32_t mt, nt;
-            const uint32_t sp = t / per_split;
-            tile_at(t - sp * per_split, P.tiles_m, P.tiles_n, P.panel, mt, nt);
+            const uint32_t tl = which ? t - total0 : t, per_split = P.tiles_m * P.tiles_n, sp = tl / per_split;
+            tile_at(tl - sp * per_split, P.tiles_m, P.tiles_n, P.panel, mt, nt);
             const int64_t cbase = (int64_t)nt * BN + part * COLS;
             int kb0;
-            const int steps = steps_of(sp, kb0), chunks = (steps + P.chunk - 1) / P.chunk;
+            const int steps = steps_of(P, sp, kb0), chunks = (steps + P.chunk - 1) / P.chunk;
             const int64_t row0 = (int64_t)(PAIR ? mt * 2 + rank : mt) * BM + quad * 32, row = row0 + lane;
             // what the row's epilogue reads, asked for while the products still run: its factors and its first target here
             const bool own = MODE != MODE_OUT && row < P.rows && cbase < P.n;
@@ -456,7 +479,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ CUt
             }
             float v[COLS];
             for (int ch = 0; ch < chunks; ++ch) {
-                ok = tc::mbar_wait(tfull0 + 8 * acc, acc_phase, abort_flag, P.status, 4u);
+                ok = tc::mbar_wait(tfull0 + 8 * acc, acc_phase, abort_flag, status, 4u);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");

@@ -71,6 +71,10 @@ CASES = [
     dict(outer=(301,), vocab=10001, model=2052, dtype=abi.BF16, vocab_major=True),
     dict(outer=(290,), vocab=9999, model=2051, dtype=abi.F16),
     dict(outer=(5000,), vocab=520, model=4100, dtype=abi.BF16, top=5, tau=2.0),
+    # few rows under a large head: g's remainder as rows of dx's own tile
+    dict(outer=(10,), vocab=17000, model=1000, dtype=abi.BF16),
+    dict(outer=(64,), vocab=17001, model=1001, dtype=abi.F16, vocab_major=True, top=3),
+    dict(outer=(65,), vocab=17000, model=1000, dtype=abi.BF16),
     # every row without a target; none
     dict(outer=(17,), vocab=100, model=32, dtype=abi.BF16, ignored=1.1),
     dict(outer=(17,), vocab=100, model=32, dtype=abi.F32, ignored=1.1, top=3),
