@@ -141,12 +141,15 @@ typedef enum {
                              attention's). A label below zero is a row without a target: loss, log-sum-exp and gradient 0,
                              whatever x holds there; one that the vocabulary does not have is reported at the next
                              psk_exec_sync (E7001) and counts as none. x and w are both bf16, f16 or f32. PSK_ORDER_DEVICE
-                             only; an executor may decline the launch (E7005), and the caller then issues the two. */
+                             only; an executor may decline the launch (E7005), and the caller then issues the two. Its
+                             workspace (some bytes a row and 64 classes; for f32 or misaligned heads a copy of up to
+                             768 MB) comes from the executor's pool, so it is refused while the stream is captured. */
     PSK_OP_HEAD_XENT_VJP = 18, /* its gradients. Space as PSK_OP_HEAD_XENT. Inputs: x, w, labels, ct (over the rows, any
                              stride), the log-sum-exp of the forward launch and, as a sixth, the place of a second result,
                              dw over (classes, model). Output: dx over (rows, model). With g = (exp(l - lse) -
                              [v = label])·ct, dx = g·wᵀ and dw = xᵀ·g, both stored in the operands' type; 16-bit
-                             operands have g rounded to their type before the two products. */
+                             operands have g rounded (to binary16 or their own type, with its remainder where rows are
+                             few) before the two products. dx may lie over x; dw overlaps no other operand. */
     PSK_OP_HEAD_DISTILL = 19, /* Kullback-Leibler divergence from a teacher's top logits to the student's distribution:
                              inner axes (classes, model, top), fparam[0] the temperature τ. Inputs: x, w, the teacher's
                              classes (i64) and logits (bf16, f16 or f32) over (rows, top), and, as a fifth, the place of

@@ -1671,8 +1671,12 @@ int psk_exec_run(psk_exec *e, const psk_launch *l, void *const *table)
     case PSK_OP_HEAD_XENT: case PSK_OP_HEAD_XENT_VJP: case PSK_OP_HEAD_DISTILL: case PSK_OP_HEAD_DISTILL_VJP: {
         e->last_kernel = "k_head";
         HeadContext x{e, e->stream, e->encode, e->sms, e->status, L.ovf, L.guarded != 0};
-        rc = head_run(x, l, table);
-        if (rc != PSK_OK) e->error = x.error;
+        try {
+            rc = head_run(x, l, table);
+            if (rc != PSK_OK) e->error = x.error;
+        } catch (const std::exception &err) {
+            rc = fail(e, PSK_E10001, std::string(l->name ? l->name : "head") + ": " + err.what());
+        }
         e->kernels += x.kernels;
         e->last_flops = x.flops;
         break;

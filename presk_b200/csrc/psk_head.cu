@@ -37,6 +37,10 @@ struct Slab {
     bool take()
     {
         if (want.empty()) return true;
+        // eight sizes an octave: the pool keeps buffers by their size, and batches of ever other lengths would each leave one
+        size_t octave = 4096;
+        while (octave * 2 <= total) octave *= 2;
+        total = (total + octave / 8 - 1) / (octave / 8) * (octave / 8);
         base = psk_exec_alloc(x.e, total);
         if (!base) return false;
         for (auto &w : want) *w.first = (uint8_t *)base + w.second;
@@ -154,7 +158,7 @@ int describe(HeadContext &x, Job &j, Params P, const Operand &a, const Operand &
     if (MODE != MODE_OUT) P.splits = 1;
     const int64_t tiles = ((P.m + BM - 1) / BM) * ((P.n + BN - 1) / BN);
     // pairs of CTAs where there are rows for two and tiles for everybody (see Cfg)
-    *pair = P.m > BM && tiles >= x.sms;
+    *pair = P.m > BM && tiles * (int64_t)P.splits >= x.sms;
     P.tiles_m = (uint32_t)((P.m + (*pair ? 2 : 1) * BM - 1) / ((*pair ? 2 : 1) * BM)); P.tiles_n = (uint32_t)((P.n + BN - 1) / BN);
     if (tiles > 0x3fffffff / std::max<int64_t>(1, P.splits)) return fail(x, PSK_E7005, "head: more tiles than one launch counts");
     const int a_rows = !*pair && !together && a.k_contiguous ? (int)std::min<int64_t>(BM, up(P.m, 8)) : BM;
@@ -296,10 +300,17 @@ int head_run(HeadContext &x, const psk_launch *l, void *const *table)
     auto plan = [&](int64_t m, int64_t n, int64_t k, bool may_be_straight) {
         Out o{m, n, up(n, 4), 1, 0, may_be_straight};
         const int64_t kb = (k + BK - 1) / BK, tiles = ((m + BM - 1) / BM) * ((n + BN - 1) / BN);
-        // few tiles: cut the summed axis, so that every SM has some of it
-        const int64_t want = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(x.sms / tiles, 32), kb / 4));
-        o.kb_split = (int32_t)((kb + want - 1) / want);
-        o.splits = (kb + o.kb_split - 1) / o.kb_split;
+        // Few tiles, or a last wave of few: cut the summed axis where the estimate says that it pays. A block of the summed axis
+        // costs a tile 0.3 us (three products of f32's planes each); partial sums are written and read, and their sum is
+        // a launch.
+        double best = 0.0;
+        int64_t splits = 1;
+        for (int64_t want = 1; want <= std::min<int64_t>(std::max<int64_t>(8, x.sms / tiles), kb / 4 + 1); ++want) {
+            const int64_t each = (kb + want - 1) / want, n = (kb + each - 1) / each, waves = (tiles * n + x.sms - 1) / x.sms;
+            const double us = 0.3 * planes * (f32 ? 1.5 : 1.0) * (double)(waves * each) + (n > 1 || !may_be_straight ? 4.0 + (double)n * (double)m * (double)o.ld * 8.0 / 3e6 : 0.0);
+            if (want == 1 || us < best * 0.95) { best = us; splits = n; o.kb_split = (int32_t)each; }
+        }
+        o.splits = splits;
         if (o.splits > 1) o.straight = false;
         return o;
     };

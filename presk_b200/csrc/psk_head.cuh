@@ -258,7 +258,8 @@ PSK_DEV void store_rows(uint4 *stage, int lane, const uint32_t (&w)[16], uint8_t
     __syncwarp();
 }
 
-// The same where rows begin at any element: the lanes write neighbouring elements (T: 16 or 32 bits) of one row.
+// The same where rows begin at any element: the lanes write neighbouring elements (T: 16 or 32 bits) of one row. (Words
+// put together of two elements, for half the stores, are slower: 43 us against 35 for the vjp of 16 x 704 x 395.)
 template <class T>
 PSK_DEV void store_rows_any(uint4 *stage, int lane, const uint32_t (&w)[16], uint8_t *base, int64_t ld_bytes, int rows_live, int bytes)
 {
