@@ -168,9 +168,10 @@ int describe(HeadContext &x, Job &j, Params P, const Operand &a, const Operand &
     P.kb_k = (int32_t)((a.k + BK - 1) / BK);
     P.nprod = a.planes == 2 ? b.planes + 1 : 1;
     if (MODE != MODE_OUT) P.kb_split = P.kb_k;
-    // Steps an accumulator: 512 products of the summed axis (384 of f32's, three a block). Results of 16 bits, dx and dw, keep one
-    // accumulator throughout, and g's logits 1024 products: what truncation loses there is far below their rounding.
-    P.chunk = MODE == MODE_OUT && P.nprod < 3 ? 1 << 28 : P.nprod == 3 ? 6 : MODE == MODE_GRAD ? 16 : 8;
+    // Steps an accumulator: 512 products of the summed axis (384 of f32's, three a block), of g's logits 1024. dx and dw in
+    // 16 bits take 4096: what truncation loses there (1.4e-5 at most) is far below their rounding; one accumulator throughout
+    // would lose 4.5e-4 (measured) of a sum of 131072 products of one sign, as much as binary16's half step.
+    P.chunk = P.nprod == 3 ? 6 : MODE == MODE_OUT ? 64 : MODE == MODE_GRAD ? 16 : 8;
     // a panel's columns of b stay in a part of the L2 while a's rows stream past them
     P.panel = (uint32_t)std::min<int64_t>(P.tiles_n, std::max<int64_t>(8, (16ll << 20) / std::max<int64_t>(1, BN * a.k * 2 * a.planes)));
     P.in_f16 = f16; P.a_m_major = !a.k_contiguous; P.b_n_major = !b.k_contiguous;
@@ -282,7 +283,9 @@ int head_run(HeadContext &x, const psk_launch *l, void *const *table)
     // plane of g otherwise, whose product lands in the same sums.
     const bool small = D * V <= 16 << 20, fold = rest && 2 * N <= BM && !small;
     const int g_f16 = f32 || conv || dt == PSK_F16, in_f16 = f32 || dt == PSK_F16;
-    const bool g_scaled = vjp && g_f16, any_scale = f32 || g_scaled;
+    // (row_scaled: a row of dx is as exact as its ct is, whatever the others' are; binary16 operands, whose x is not copied
+    // into the top of the range, have 2^19 between the rows' ct before it shows beside dx's rounding)
+    const bool row_scaled = f32 || conv, g_scaled = vjp && g_f16, any_scale = f32 || g_scaled;
 
     // the vocabulary's pieces
     const int64_t per_col = (vjp ? Ng * planes * 2 : 0) + (w_direct ? 0 : D * planes * 2) + (conv ? D * 2 : 0);
@@ -403,7 +406,7 @@ int head_run(HeadContext &x, const psk_launch *l, void *const *table)
     if (xd && N) {
         PackParams k = kx;
         k.dst = xd; k.plane = N * Dp; k.to = f32 ? PACK_SPLIT : conv ? PACK_F16 : PACK_SAME; k.copies = (int32_t)(Ng / N);
-        k.max = f32 || conv ? &scales->max_x : nullptr;
+        if (row_scaled) { k.max = &scales->max_x; k.coef = coef; k.max_ct = &scales->max_ct; }
         copies.add(x, k);
     }
     const Operand a = x_direct ? Operand{rx.p, N, D, x_ld, true, 1, 0} : Operand{xl ? xl : xd, N, D, Dp, true, planes, N * Dp};
@@ -436,7 +439,7 @@ int head_run(HeadContext &x, const psk_launch *l, void *const *table)
             if (r != PSK_OK) return r;
             continue;
         }
-        P.lse2 = lse2; P.coef = coef; P.g = g; P.g_f16 = g_f16; P.g_ld = g_ld; P.g_rest = N * g_ld;
+        P.lse2 = lse2; P.coef = coef; P.g = g; P.g_f16 = g_f16; P.row_scaled = row_scaled; P.g_ld = g_ld; P.g_rest = N * g_ld;
         r = rest || f32 ? product<MODE_GRAD, true>(x, P, a, b, in_f16) : product<MODE_GRAD>(x, P, a, b, in_f16);
         if (r != PSK_OK) return r;
         // 6. dx = g·wᵀ summed over the pieces: both operands along the classes
@@ -446,13 +449,13 @@ int head_run(HeadContext &x, const psk_launch *l, void *const *table)
         Q.kb_split = dxo.kb_split;
         Q.splits = (uint32_t)(((vn + BK - 1) / BK + dxo.kb_split - 1) / dxo.kb_split); // a shorter last piece may have fewer
         Q.out = dxo.straight ? const_cast<void *>(rout.p) : dxp; Q.out_ld = dxo.straight ? dx_ld : dxo.ld; Q.out_dtype = dxo.straight ? dt : PSK_F32;
-        Q.un = dxo.straight ? UN_DX : UN_NONE; Q.accumulate = piece > 0;
+        Q.coef = row_scaled ? coef : nullptr; Q.un = dxo.straight ? UN_DX : UN_NONE; Q.accumulate = piece > 0;
         Q.out_vec = !dxo.straight || (aligned(rout.p) && dx_ld * eb % 16 == 0 && D * eb % 16 == 0);
         Q.ovf = x.guarded && dxo.straight ? x.ovf : nullptr;
         const Operand gk = f32 || (rest && !fold) ? Operand{g, N, vn, g_ld, true, 2, N * g_ld} : Operand{g, Ng, vn, g_ld, true, 1, 0};
         const Operand wk{bd.p, D, vn, bd.ld, v_inner, planes, bd.plane};
         // 7. dw of the piece = xᵀ·g: both operands along the rows. Small ones go with dx in one launch (vjp of 16 x 704 x 392:
-        // WITH us against WITHOUT); where dx streams a large head, its ring is better kept to itself.
+        // 32 us against 38); where dx streams a large head, its ring is better kept to itself.
         if (!DW) {
             r = product<MODE_OUT>(x, Q, gk, wk, g_f16);
             if (r != PSK_OK) return r;
@@ -509,7 +512,7 @@ int head_run(HeadContext &x, const psk_launch *l, void *const *table)
         SumParams S;
         memset(&S, 0, sizeof S);
         S.s = s; S.part = dxp; S.parts = dxo.splits; S.part_rows = dxo.m; S.ld = dxo.ld; S.fold = fold ? N : 0; S.cols = D; S.col_stride = O.stride[ax_d];
-        S.scales = scales; S.un = UN_DX; S.dst = rout; S.ovf = x.ovf; S.guarded = x.guarded;
+        S.scales = scales; S.coef = row_scaled ? coef : nullptr; S.un = UN_DX; S.dst = rout; S.ovf = x.ovf; S.guarded = x.guarded;
         HEAD_START(k_head_sum, warps_of(x, N * ((D + 127) / 128)), 1, 256, 0, 1, S);
     } else if (N == 0 && DW) { // no rows: a gradient of zeros
         SumParams S;

@@ -14,9 +14,10 @@
 //
 // Types. bf16 and binary16 operands are multiplied as they are. f32 operands are two binary16 planes, hi + lo, 22 bits
 // of the number, of which three partial products are taken (lo·lo is below 2^-22 of the product): half the tensor
-// work of three bf16 planes and their six products, which this was first (333 us at 2044 x 1024 x 16384, against
-// 183 us). Binary16's range is met by powers of two: w is scaled by its greatest |element|, x by a row's, g by the greatest
-// |ct|, each to the top of the range, 2^14 to 2^15, so that what falls below 2^-24 there is 2^-39 of the greatest.
+// work of three bf16 planes and their six products, which this was first (the logits of 2044 x 1024 x 16384: 333 us, 183 with
+// two planes on the same tiles, 156 on pairs). Binary16's range is met by powers of two: w is scaled by its greatest |element|, x by a row's, g by a row's
+// |ct| (binary16 operands: by the greatest), each to the top of the range, 2^14 to 2^15, so that what falls below 2^-24
+// there is 2^-39 of the greatest. For dw, which sums over the rows, x's copy carries what their scales differ by.
 // g itself is kept in binary16 for f32 and, for many rows, for bf16 operands too, x and w being copied into it (exactly:
 // eight bits into eleven): g in bf16 would cost its 2^-9 an entry, as much again as the result's own rounding.
 #pragma once
@@ -29,17 +30,18 @@ namespace head {
 
 constexpr int BM = 128, BN = 256, BK = 64;
 // Five warpgroups: warps 0 and 2 issue the TMA loads, warp 1 the products (3 is idle); warps 4 to 19 are the epilogue, four
-// a quadrant of tensor memory, 64 columns each. Eight warps of 128 columns had too little to issue from (an instruction
-// every six cycles a warp, half the rate of the tiles of a model of 216). An epilogue thread keeps its 64 sums in
-// registers, so the first warpgroup gives up most of its share: 128·32 + 512·112 = 640·96, what the block is launched with.
+// a quadrant of tensor memory, 64 columns each: 325 us where eight warps of 128 columns took 331 to 342 (logits of 1521 x
+// 216 x 137k before the issuing threads were relieved), and one part a thread. A thread keeps its 64 sums in registers, so the first warpgroup gives up most of its share: 128·32 + 512·112 = 640·96, what the block is launched with.
 constexpr int EPILOGUE = 16, THREADS = 128 + 32 * EPILOGUE;
 constexpr int REGS_FEW = 32, REGS_MANY = 112, REGS_LAUNCH = 96;
 static_assert(128 * REGS_FEW + 32 * EPILOGUE * REGS_MANY <= THREADS * REGS_LAUNCH, "setmaxnreg waits for registers that the block does not have");
 // A tile is 128 rows by 256 columns a CTA. Two forms:
 //   PAIR   two CTAs of a cluster compute 256 x 256: each loads its own 128 rows of a and one half of b's columns, and
-//          the products (cta_group::2) read either half from either SM. What a CTA takes from the L2 a block of 64 of
-//          the summed axis is 32 KB where it is 48 alone; at 16 to 17 TB/s the L2 is what bounds the single form.
+//          the products (cta_group::2) read either half from either SM: half the instructions to issue, and 32 KB from
+//          the L2 a block of 64 of the summed axis where a CTA alone takes 48.
 //   single for few rows (up to 128: there b's bytes from memory are the bound) and few tiles.
+// Pair against single, us, 2048 rows and 32000 classes, logits/g/dx/dw: a model of 4096 361/381/349/393 against
+// 370/393/391/404; of 512 63/80/51/61 against 61/80/60/65; of 128 the same.
 struct Cfg {
     static constexpr int A_BYTES = BM * BK * 2, BARS = 256, MOST_STAGES = 8;
     static constexpr int SMEM_TOTAL = 227 * 1024;
@@ -78,11 +80,14 @@ PSK_DEV int scale_of(uint32_t max_bits)
     return k > 60 ? 60 : k; // 1/(g·w) and 1/(g·x) are f32 numbers then
 }
 
+PSK_DEV int scale_of(float coef) { return scale_of(__float_as_uint(coef) & 0x7fffffffu); }
+
 enum { UN_NONE = 0, UN_DX = 1, UN_DW = 2 }; // what a product's sums are multiplied by: 1, 1/(g·w), 1/(g·x)
-PSK_DEV float undo(const Scales *s, int un)
+// (`coef`: of the row, where g's rows have scales of their own)
+PSK_DEV float undo(const Scales *s, int un, const float *coef)
 {
     if (!s || un == UN_NONE) return 1.0f;
-    return pow2(-scale_of(s->max_ct) - scale_of(un == UN_DX ? s->max_w : s->max_x));
+    return pow2(-(coef ? scale_of(*coef) : scale_of(s->max_ct)) - scale_of(un == UN_DX ? s->max_w : s->max_x));
 }
 
 struct Params {
@@ -111,9 +116,9 @@ struct Params {
     float2 *part;                 // [part][row]: (max, sum of 2^((l - max)·c))
     float *hit;                   // rows x top: the entries' logits
     // MODE_GRAD
-    const float *lse2, *coef;     // a row's log-sum-exp in base 2, and ct/τ (0 where it has no target)
+    const float *lse2, *coef;     // a row's log-sum-exp in base 2, and ct/τ (0 where it has no target); MODE_OUT: coef where it undoes a row's scale, or null
     uint16_t *g;
-    int32_t g_f16;                // g in binary16, scaled by max_ct where there are scales; else bf16
+    int32_t g_f16, row_scaled;    // g in binary16, scaled by its row's coef or by max_ct; else bf16
     int64_t g_ld, g_rest;         // row stride; REST: how much further on what the rounding leaves is kept
     // MODE_OUT
     void *out;                    // [split][m][out_ld]
@@ -475,7 +480,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ Job
                 if (MODE == MODE_GRAD) {
                     lse2 = P.lse2[row];
                     coef = P.coef[row];
-                    if (P.scales && P.g_f16) coef = __fmul_rn(coef, pow2(scale_of(P.scales->max_ct)));
+                    if (P.scales && P.g_f16) coef = __fmul_rn(coef, pow2(P.row_scaled ? scale_of(coef) : scale_of(P.scales->max_ct)));
                 }
             }
             float v[COLS];
@@ -566,7 +571,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ Job
                     if constexpr (REST) store_rows<false>(stage_out, lane, rest, base + (g + P.g_rest) * 2, P.g_ld * 2, rows_live, bytes);
                 }
             } else {
-                const float f = undo(P.scales, P.un);
+                const float f = undo(P.scales, P.un, P.coef && row < P.m ? P.coef + row : nullptr);
 #pragma unroll
                 for (int i = 0; i < COLS; ++i) v[i] = __fmul_rn(v[i], f);
                 const int eb = P.out_dtype == PSK_F32 ? 4 : 2;
@@ -614,6 +619,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ Job
         }
     }
 
+    if (*abort_flag) // a wait ran out: what was queued before it gets a millisecond to land before the block leaves
+        for (const long long since = clock64(); clock64() - since < 2000000;) {}
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if (PAIR) tc2::cluster_sync(); // nobody leaves, or frees tensor memory the pair's products write, while the other works
@@ -668,7 +675,7 @@ PSK_DEV void row_factors(const RowSpace &s, const RowOperand &ct, const RowOpera
     const float c = none ? 0.0f : __fmul_rn(load_real(ct.p, ct.dtype, row_offset(s, ct.stride, row)), inv_tau);
     coef[row] = c;
     lse2[row] = none ? 0.0f : (float)((double)load_real(lse.p, lse.dtype, row_offset(s, lse.stride, row)) * 1.4426950408889634);
-    if (ctmax && !none && fabsf(c) <= 3.4e38f) atomicMax(ctmax, __float_as_uint(fabsf(c))); // non-negative floats order as their bits do: no order of the rows changes it
+    if (ctmax && !none && fabsf(c) < INFINITY) atomicMax(ctmax, __float_as_uint(fabsf(c))); // non-negative floats order as their bits do: no order of the rows changes it
 }
 
 static __global__ void __launch_bounds__(256) k_head_labels(const __grid_constant__ LabelParams P)
@@ -919,6 +926,8 @@ struct PackParams {
     uint16_t *dst;
     int32_t to, copies, vec;
     const uint32_t *max; // of the whole matrix, for its scale; or null
+    const float *coef;   // with max_ct: what the rows of g are scaled by more than the greatest is taken from them here
+    const uint32_t *max_ct;
     float *un;          // PACK_SPLIT: scale every row by its own greatest element instead, and put the factor that undoes it here
     const int32_t *ids;
     int32_t top;
@@ -951,9 +960,9 @@ PSK_DEV void pack_matrix(const PackParams &P)
         const int live = no_target(P.ids, P.top, row) ? 0 : (int)((P.cols - c0) < n ? P.cols - c0 : n); // of which the matrix has
         const int64_t cs = P.col_stride, off = row_offset(P.s, P.src.stride, row) + c0 * cs;
         uint16_t *dst = P.dst + row * P.ld + c0;
+        float f = P.coef ? __fmul_rn(whole, pow2(scale_of(*P.max_ct) - scale_of(P.coef[row]))) : whole;
         if constexpr (TO == PACK_SPLIT) {
             const float *src = (const float *)P.src.p + off;
-            float f = whole;
             if (P.un) {
                 uint32_t m = 0;
 #pragma unroll 8
@@ -1008,7 +1017,7 @@ PSK_DEV void pack_matrix(const PackParams &P)
                     if constexpr (TO == PACK_F16) {
                         uint32_t *w = &u.x;
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) w[k] = pack_f16x2_hw(__fmul_rn(bf16_up(w[k] & 0xffffu), whole), __fmul_rn(bf16_up(w[k] >> 16), whole));
+                        for (int k = 0; k < 4; ++k) w[k] = pack_f16x2_hw(__fmul_rn(bf16_up(w[k] & 0xffffu), f), __fmul_rn(bf16_up(w[k] >> 16), f));
                     }
                     *reinterpret_cast<uint4 *>(dst + c) = u;
                     if (P.copies > 1) *reinterpret_cast<uint4 *>(dst + c + again) = u;
@@ -1022,7 +1031,7 @@ PSK_DEV void pack_matrix(const PackParams &P)
                     for (int k = 0; k < 16; ++k) {
                         const int c = cb + k * 32;
                         if (c >= n) break;
-                        const uint16_t w = packed<TO>(in[k], whole);
+                        const uint16_t w = packed<TO>(in[k], f);
                         dst[c] = w;
                         if (P.copies > 1) dst[c + again] = w;
                     }
@@ -1050,6 +1059,7 @@ struct SumParams {
     const float *part;
     int64_t parts, part_rows, ld, fold, cols, col_stride; // ld: a multiple of 4
     const Scales *scales;
+    const float *coef; // a row's, where it undoes its scale; or null
     int32_t un; // UN_DX, UN_DW
     RowOperand dst;
     uint32_t *ovf;
@@ -1061,11 +1071,11 @@ static __global__ void __launch_bounds__(256) k_head_sum(const __grid_constant__
     follow();
     const int64_t quads = (P.cols + 3) / 4, warps = (int64_t)gridDim.x * 8, chunks = (quads + 31) / 32;
     const int lane = threadIdx.x & 31;
-    const float un = undo(P.scales, P.un);
     uint32_t ovf = 0;
     for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < P.s.rows * chunks; i += warps) {
         const int64_t row = i / chunks, c = ((i - row * chunks) * 32 + lane) * 4;
         if (c >= P.cols) continue;
+        const float un = undo(P.scales, P.un, P.coef ? P.coef + row : nullptr);
         float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         const float *src = P.part + row * P.ld + c;
 #pragma unroll 4

@@ -321,6 +321,38 @@ def test_rows_of_other_magnitudes(cuda):
     assert (got["lse"][7].double() - big).abs() <= t9["lse"][7]
 
 
+@pytest.mark.parametrize("dtype,rows", [(abi.F32, 20), (abi.F32, 300), (abi.BF16, 300), (abi.BF16, 20)])
+def test_rows_of_other_weights(cuda, dtype, rows):
+    """A power of two taken from a row's cotangent is taken from its gradient, exactly: g of a row is scaled about itself."""
+    s = hc.make((rows,), 700, 96, dtype, device="cuda", ignored=0.0)
+    got = run(cuda, s)
+    less = torch.exp2(-(torch.arange(rows, device="cuda") % 30).float())
+    s["ct"] = s["ct"] * less
+    want, tol = hc.plain(s)
+    again = run(cuda, s)
+    compare(again, want, tol)
+    assert torch.equal(again["dx"], (got["dx"].float() * less[:, None]).to(got["dx"].dtype))
+
+
+def test_gradients_summed_over_a_large_vocabulary(cuda):
+    """dx of 131072 products of one sign (x = 0: g is 2^-17, exactly, beside the labels' class, whose weight is 0). Added by
+    truncation alone it is 4.5e-4 too small on average. Its rounding to binary16, at most 2^-11, is zero on average over
+    2048 outputs to 2^-11 / sqrt(3 x 2048) = 6e-6, four times which and 1.4e-5 of truncation are below 5e-5."""
+    rows, vocab, model = 2304, 131072, 2048  # tiles for one wave: the sums are not split
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    s = hc.make((rows,), 64, model, abi.F16, device="cuda", ignored=0.0)
+    s["x"].zero_()
+    s["vocab"], s["w"] = vocab, torch.rand(model, vocab, generator=gen, device="cuda").add_(1.0).to(torch.float16)
+    s["labels"].zero_()
+    s["w"][:, 0] = 0
+    s["ct"] = torch.ones_like(s["ct"])
+    got = run(cuda, s)
+    want = s["w"].double().sum(1) / vocab
+    off = (got["dx"].double() / want - 1)
+    assert float(off.abs().max()) <= 2 ** -11 + 1.4e-5 + 2 ** -20
+    assert abs(float(off[0].mean())) < 5e-5, float(off[0].mean())
+
+
 def test_a_class_the_vocabulary_does_not_have(cuda):
     for top in (0, 4):
         s = hc.make((10,), 100, 32, abi.BF16, device="cuda", top=top, ignored=0.0)
