@@ -203,8 +203,9 @@ struct Copies {
     void add(const HeadContext &x, PackParams k)
     {
         const int64_t unit = k.to == PACK_SPLIT ? 4 : 8; // elements of 16 bytes
-        k.vec = k.col_stride == 1 && k.cols == k.ld && ((uintptr_t)k.src.p & 15u) == 0;
-        for (int a = 0; a < k.s.no; ++a) k.vec = k.vec && (k.s.dims[a] == 1 || k.src.stride[a] % unit == 0);
+        bool aligned = k.cols == k.ld && ((uintptr_t)k.src.p & 15u) == 0;
+        for (int a = 0; a < k.s.no; ++a) aligned = aligned && (k.s.dims[a] == 1 || k.src.stride[a] % unit == 0);
+        k.vec = k.col_stride != 1 ? VEC_NOT : aligned ? VEC_ALIGNED : VEC_SHIFTED;
         grid = std::max<int64_t>(grid, warps_of(x, k.un ? k.s.rows : k.s.rows * ((k.ld + PIECE - 1) / PIECE)));
         all.of[n++] = k;
     }

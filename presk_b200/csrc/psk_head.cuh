@@ -30,8 +30,8 @@ namespace head {
 
 constexpr int BM = 128, BN = 256, BK = 64;
 // Five warpgroups: warps 0 and 2 issue the TMA loads, warp 1 the products (3 is idle); warps 4 to 19 are the epilogue, four
-// a quadrant of tensor memory, 64 columns each: 325 us where eight warps of 128 columns took 331 to 342 (logits of 1521 x
-// 216 x 137k before the issuing threads were relieved), and one part a thread. A thread keeps its 64 sums in registers, so the first warpgroup gives up most of its share: 128·32 + 512·112 = 640·96, what the block is launched with.
+// a quadrant of tensor memory, 64 columns each: 325 us where eight warps of 128 columns took 331 to 342 (27924 tiles
+// of a model of 216, before the issuing threads were relieved), and one part a thread. A thread keeps its 64 sums in registers, so the first warpgroup gives up most of its share: 128·32 + 512·112 = 640·96, what the block is launched with.
 constexpr int EPILOGUE = 16, THREADS = 128 + 32 * EPILOGUE;
 constexpr int REGS_FEW = 32, REGS_MANY = 112, REGS_LAUNCH = 96;
 static_assert(128 * REGS_FEW + 32 * EPILOGUE * REGS_MANY <= THREADS * REGS_LAUNCH, "setmaxnreg waits for registers that the block does not have");
@@ -947,8 +947,31 @@ PSK_DEV uint32_t split_f16(float x)
     return hi | (fabsf(r) < 65504.0f ? pack_f16x2_hw(r, 0.0f) << 16 : 0u);
 }
 
-// VEC: the source's rows contiguous and on 16-byte boundaries, cols = ld: eight elements a lane.
-template <int TO, bool VEC>
+// Eight 16-bit elements that begin `shift` bytes (an even number below 16) into 32: the same shift in all of a row.
+PSK_DEV uint4 eight_from(uint4 a, uint4 b, uint32_t shift)
+{
+    uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    if (shift & 8) {
+#pragma unroll
+        for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+    }
+    if (shift & 4) {
+#pragma unroll
+        for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+    }
+    if (shift & 2) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 16);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Bound by memory: a head of 1000 x 30011 whose rows begin at any element is copied in 28 us, 4.3 TB/s of the 6.5 of a
+// plain copy (two 16-byte loads an eight elements, shifted; with a load an element it was 43). Four blocks an SM: the
+// loads ahead would take 125 registers otherwise, and 131 us where this takes 104 (4096 x 32000 with 8192 rows of x).
+// VEC: the source's rows contiguous; VEC_ALIGNED: on 16-byte boundaries too, and cols = ld. Eight elements a lane then.
+enum { VEC_NOT = 0, VEC_ALIGNED = 1, VEC_SHIFTED = 2 };
+template <int TO, int VEC>
 PSK_DEV void pack_matrix(const PackParams &P)
 {
     const int lane = threadIdx.x & 31;
@@ -960,7 +983,8 @@ PSK_DEV void pack_matrix(const PackParams &P)
         const int live = no_target(P.ids, P.top, row) ? 0 : (int)((P.cols - c0) < n ? P.cols - c0 : n); // of which the matrix has
         const int64_t cs = P.col_stride, off = row_offset(P.s, P.src.stride, row) + c0 * cs;
         uint16_t *dst = P.dst + row * P.ld + c0;
-        float f = P.coef ? __fmul_rn(whole, pow2(scale_of(*P.max_ct) - scale_of(P.coef[row]))) : whole;
+        float f = whole;
+        if (P.coef) f = __fmul_rn(f, pow2(scale_of(*P.max_ct) - scale_of(P.coef[row])));
         if constexpr (TO == PACK_SPLIT) {
             const float *src = (const float *)P.src.p + off;
             if (P.un) {
@@ -973,7 +997,7 @@ PSK_DEV void pack_matrix(const PackParams &P)
                 f = pow2(e);
                 if (lane == 0) P.un[row] = pow2(-e);
             }
-            if constexpr (VEC) {
+            if constexpr (VEC == VEC_ALIGNED) {
                 for (int cb = lane * 4; cb < n; cb += 4 * 128) {
                     float4 in[4]; // (all loads of a batch before its stores: the compiler cannot tell the buffers apart)
 #pragma unroll
@@ -1005,15 +1029,43 @@ PSK_DEV void pack_matrix(const PackParams &P)
             }
         } else {
             const uint16_t *src = (const uint16_t *)P.src.p + off;
-            if constexpr (VEC) {
-                uint4 in[PIECE / 256];
+            if constexpr (VEC != VEC_NOT) {
+                constexpr int EACH = PIECE / 256;
+                uint4 in[EACH], next[VEC == VEC_SHIFTED ? EACH : 1];
+                const uint32_t shift = (uint32_t)((uintptr_t)src & 15u);
+                const uint16_t *const begin = src - c0, *const end = begin + P.cols; // of the row
+                auto inside = [&](int c) { // the 32 bytes around it are the row's
+                    const uint16_t *q = src + c - shift / 2;
+                    return q >= begin && q + 16 <= end;
+                };
 #pragma unroll
-                for (int k = 0; k < PIECE / 256; ++k) in[k] = live && lane * 8 + k * 256 < n ? *reinterpret_cast<const uint4 *>(src + lane * 8 + k * 256) : make_uint4(0u, 0u, 0u, 0u);
+                for (int k = 0; k < EACH; ++k) {
+                    const int c = lane * 8 + k * 256;
+                    in[k] = make_uint4(0u, 0u, 0u, 0u);
+                    if constexpr (VEC == VEC_ALIGNED) {
+                        if (live && c < n) in[k] = *reinterpret_cast<const uint4 *>(src + c);
+                    } else {
+                        if (live && inside(c)) {
+                            const uint4 *q = reinterpret_cast<const uint4 *>(src + c - shift / 2);
+                            in[k] = q[0];
+                            next[k] = q[1]; // (the next lane's first: from the L1)
+                        }
+                    }
+                }
 #pragma unroll
-                for (int k4 = 0; k4 < PIECE / 256; ++k4) {
+                for (int k4 = 0; k4 < EACH; ++k4) {
                     const int c = lane * 8 + k4 * 256;
                     if (c >= n) break;
                     uint4 u = in[k4];
+                    if constexpr (VEC == VEC_SHIFTED) {
+                        if (live && inside(c)) u = eight_from(u, next[k4], shift);
+                        else { // the row's ends
+                            uint32_t w[4];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) w[j] = (c + 2 * j < live ? src[c + 2 * j] : 0u) | (c + 2 * j + 1 < live ? (uint32_t)src[c + 2 * j + 1] << 16 : 0u);
+                            u = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                    }
                     if constexpr (TO == PACK_F16) {
                         uint32_t *w = &u.x;
 #pragma unroll
@@ -1043,13 +1095,22 @@ PSK_DEV void pack_matrix(const PackParams &P)
 
 struct Packs { PackParams of[4]; };
 
-static __global__ void __launch_bounds__(256) k_head_pack(const __grid_constant__ Packs all)
+static __global__ void __launch_bounds__(256, 4) k_head_pack(const __grid_constant__ Packs all)
 {
     const PackParams &P = all.of[blockIdx.y];
     follow();
-    if (P.to == PACK_SPLIT) { if (P.vec) pack_matrix<PACK_SPLIT, true>(P); else pack_matrix<PACK_SPLIT, false>(P); }
-    else if (P.to == PACK_F16) { if (P.vec) pack_matrix<PACK_F16, true>(P); else pack_matrix<PACK_F16, false>(P); }
-    else { if (P.vec) pack_matrix<PACK_SAME, true>(P); else pack_matrix<PACK_SAME, false>(P); }
+    if (P.to == PACK_SPLIT) {
+        if (P.vec == VEC_ALIGNED) pack_matrix<PACK_SPLIT, VEC_ALIGNED>(P);
+        else pack_matrix<PACK_SPLIT, VEC_NOT>(P);
+    } else if (P.to == PACK_F16) {
+        if (P.vec == VEC_ALIGNED) pack_matrix<PACK_F16, VEC_ALIGNED>(P);
+        else if (P.vec == VEC_SHIFTED) pack_matrix<PACK_F16, VEC_SHIFTED>(P);
+        else pack_matrix<PACK_F16, VEC_NOT>(P);
+    } else {
+        if (P.vec == VEC_ALIGNED) pack_matrix<PACK_SAME, VEC_ALIGNED>(P);
+        else if (P.vec == VEC_SHIFTED) pack_matrix<PACK_SAME, VEC_SHIFTED>(P);
+        else pack_matrix<PACK_SAME, VEC_NOT>(P);
+    }
 }
 
 // A gradient from its f32 partial sums into its place: the splits' sums in their order (and, of few rows, those of g's
