@@ -350,7 +350,10 @@ int head_run(HeadContext &x, const psk_launch *l, void *const *table)
     slab.need(dwp, DW && N && !dwo.straight ? dwo.splits * dwo.m * dwo.ld : 0);
     slab.need(scales, any_scale ? 1 : 0);
     if (!slab.take()) return fail(x, PSK_E10001, nm + ": no memory for a workspace of " + std::to_string(slab.total) + " bytes (" + psk_last_error(x.e) + ")");
-    if (any_scale) HEAD_TRY(cudaMemsetAsync(scales, 0, sizeof *scales, x.stream));
+    // the maxima begin at zero: written by the targets' launch where a launch for the maxima follows, else (binary16, whose
+    // only maximum is ct's, taken by the targets' launch itself) by a memset
+    const bool maxima = f32 || conv;
+    if (any_scale && !maxima) HEAD_TRY(cudaMemsetAsync(scales, 0, sizeof *scales, x.stream));
 
     if (N > 0) {
         // 1. targets
@@ -361,37 +364,38 @@ int head_run(HeadContext &x, const psk_launch *l, void *const *table)
             memset(&T, 0, sizeof T);
             T.s = s; T.ids = rids; T.t = row_operand(l->in[3], table[3], no); T.ct = rct; T.lse = rlse;
             T.ids_k = I.stride[ax_k]; T.t_k = l->in[3].stride[ax_k]; T.classes = V; T.top = (int32_t)K; T.inv_tau = inv_tau;
-            T.out_ids = ids; T.start = start; T.parts = parts; T.out_p = p; T.plogp = plogp; T.coef = coef; T.lse2 = lse2; T.status = x.status; T.ctmax = g_scaled ? &scales->max_ct : nullptr;
+            T.out_ids = ids; T.start = start; T.parts = parts; T.out_p = p; T.plogp = plogp; T.coef = coef; T.lse2 = lse2; T.status = x.status; T.ctmax = g_scaled && !maxima ? &scales->max_ct : nullptr; T.zero = maxima ? scales : nullptr;
             HEAD_START(k_head_teacher, N, 1, (unsigned)std::max<int64_t>(up(K, 32), N <= 2 * x.sms ? 256 : 128), (size_t)K * 8, 1, T);
         } else {
             LabelParams T;
             memset(&T, 0, sizeof T);
             T.s = s; T.ids = rids; T.ct = rct; T.lse = rlse; T.classes = V; T.inv_tau = inv_tau;
-            T.ids_out = ids; T.coef = coef; T.lse2 = lse2; T.status = x.status; T.ctmax = g_scaled ? &scales->max_ct : nullptr;
+            T.ids_out = ids; T.coef = coef; T.lse2 = lse2; T.status = x.status; T.ctmax = g_scaled && !maxima ? &scales->max_ct : nullptr; T.zero = maxima ? scales : nullptr;
             HEAD_START(k_head_labels, (N + 255) / 256, 1, 256, 0, 1, T);
         }
         // 2. the powers of two
-        if (any_scale) {
-            const bool of_x = DW && (f32 || conv), of_w = f32 || conv;
+        if (maxima) {
             MaxOfTwo both;
             memset(&both, 0, sizeof both);
             unsigned n = 0;
             int64_t grid = 1;
-            if (of_x) {
+            if (vjp) { // (the rows first: their factors' maximum is taken over the same number of rows)
                 MaxParams &M = both.of[n++];
-                M.s = s; M.src = rx; M.col_stride = X.stride[ax_d]; M.cols = D; M.ids = ids; M.top = (int32_t)K; M.out = &scales->max_x;
+                M.s = s; M.src = rx; M.col_stride = X.stride[ax_d]; M.cols = DW ? D : 0; M.ids = ids; M.top = (int32_t)K; M.out = &scales->max_x;
                 M.vec = x_ld && M.col_stride == 1 && aligned(rx.p) && x_ld * eb % 16 == 0 && D * eb % 16 == 0;
                 grid = warps_of(x, N * ((D + PIECE - 1) / PIECE));
             }
-            if (of_w) {
+            {
                 MaxParams &M = both.of[n++];
                 M.s.no = 1; M.s.rows = M.s.dims[0] = v_inner ? D : V; M.src.p = wp; M.src.dtype = dt; M.src.stride[0] = v_inner ? w_d : w_v;
                 M.col_stride = v_inner ? w_v : w_d; M.cols = v_inner ? V : D; M.out = &scales->max_w;
                 M.vec = M.col_stride == 1 && aligned(wp) && M.src.stride[0] * eb % 16 == 0 && M.cols * eb % 16 == 0;
                 grid = std::max<int64_t>(grid, warps_of(x, M.s.rows * ((M.cols + PIECE - 1) / PIECE)));
             }
-            if (n && f32) HEAD_START(k_head_max<true>, grid, n, 256, 0, 1, both);
-            else if (n) HEAD_START(k_head_max<false>, grid, n, 256, 0, 1, both);
+            both.operands = (int32_t)n; both.coef = coef; both.max_ct = &scales->max_ct;
+            if (vjp) n += 1;
+            if (f32) HEAD_START(k_head_max<true>, grid, n, 256, 0, 1, both);
+            else HEAD_START(k_head_max<false>, grid, n, 256, 0, 1, both);
         }
     }
     // 3. x for the logits, and (rows without a target zeros) for dw: made together with the first piece's copies of the head

@@ -31,7 +31,8 @@ namespace head {
 constexpr int BM = 128, BN = 256, BK = 64;
 // Five warpgroups: warps 0 and 2 issue the TMA loads, warp 1 the products (3 is idle); warps 4 to 19 are the epilogue, four
 // a quadrant of tensor memory, 64 columns each: 325 us where eight warps of 128 columns took 331 to 342 (27924 tiles
-// of a model of 216, before the issuing threads were relieved), and one part a thread. A thread keeps its 64 sums in registers, so the first warpgroup gives up most of its share: 128·32 + 512·112 = 640·96, what the block is launched with.
+// of a model of 216, before the issuing threads were relieved), and one part a thread. A thread keeps its 64 sums in
+// registers, so the first warpgroup gives up most of its share: 128·32 + 512·112 = 640·96, what the block is launched with.
 constexpr int EPILOGUE = 16, THREADS = 128 + 32 * EPILOGUE;
 constexpr int REGS_FEW = 32, REGS_MANY = 112, REGS_LAUNCH = 96;
 static_assert(128 * REGS_FEW + 32 * EPILOGUE * REGS_MANY <= THREADS * REGS_LAUNCH, "setmaxnreg waits for registers that the block does not have");
@@ -293,7 +294,11 @@ struct Jobs {
 };
 
 // The product of a persistent CTA's tiles, and what MODE makes of it. Bounds: the tensor pipe (2·m·n·k flops) for many
-// rows; for few, the bytes of the second operand.
+// rows; for few, the bytes of the second operand. Measured (bf16, a head of 4096 x 32000): 8192 rows, the logits' maxima
+// and sums 1446 us, g 1452, dx 1376, dw 1414, 1.48 to 1.56 PFLOP/s of cuBLAS's 1.65; one after the other in a training
+// step, at the power limit's clock, a sixth longer. 16 rows: 46 us for the head's 262 MB, 5.6 TB/s.
+// f32 (2044 x 1024 x 16384, three products): 156, 196, 169, 177 us, 1.05 to 1.3 PFLOP/s: sums that leave the accumulator
+// every six steps, twice the bytes of g, and dx and dw in whole waves of tiles.
 template <int MODE, bool PAIR, bool REST = false, int JOBS = 1>
 __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ Jobs<JOBS> jobs)
 {
@@ -657,7 +662,7 @@ PSK_DEV int64_t row_offset(const RowSpace &s, const int64_t *stride, int64_t row
 }
 
 // Labels as lists of one class (0x7fffffff where a row has none) and, backward, a row's factor ct/τ and its log-sum-exp in
-// base 2. A class that the vocabulary does not have is reported and counts as no target.
+// base 2. A class that the vocabulary does not have is reported and counts as no target. 3 us, with ct 6: a launch's latency.
 struct LabelParams {
     RowSpace s;
     RowOperand ids, ct, lse;
@@ -666,33 +671,38 @@ struct LabelParams {
     int32_t *ids_out;
     float *coef, *lse2;
     uint32_t *status, *ctmax;
+    Scales *zero; // to be zeroed for the maxima that follow; or null
 };
 
 // ct and lse of a row, for either kind of target. Rows that a launch's weight leaves out keep the value they have.
-PSK_DEV void row_factors(const RowSpace &s, const RowOperand &ct, const RowOperand &lse, int64_t row, bool none, float inv_tau, float *coef, float *lse2, uint32_t *ctmax)
+// The result: the bits of |ct/τ| where that is finite, else 0 (non-negative floats order as their bits do).
+PSK_DEV uint32_t row_factors(const RowSpace &s, const RowOperand &ct, const RowOperand &lse, int64_t row, bool none, float inv_tau, float *coef, float *lse2)
 {
-    if (!coef) return;
+    if (!coef) return 0u;
     const float c = none ? 0.0f : __fmul_rn(load_real(ct.p, ct.dtype, row_offset(s, ct.stride, row)), inv_tau);
     coef[row] = c;
     lse2[row] = none ? 0.0f : (float)((double)load_real(lse.p, lse.dtype, row_offset(s, lse.stride, row)) * 1.4426950408889634);
-    if (ctmax && !none && fabsf(c) < INFINITY) atomicMax(ctmax, __float_as_uint(fabsf(c))); // non-negative floats order as their bits do: no order of the rows changes it
+    return fabsf(c) < INFINITY ? __float_as_uint(fabsf(c)) : 0u;
 }
 
 static __global__ void __launch_bounds__(256) k_head_labels(const __grid_constant__ LabelParams P)
 {
     follow();
     const int64_t row = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (P.zero && blockIdx.x == 0 && threadIdx.x == 0) *P.zero = Scales{0u, 0u, 0u, 0u};
     if (row >= P.s.rows) return;
     const int64_t y = ((const int64_t *)P.ids.p)[row_offset(P.s, P.ids.stride, row)];
     if (y >= P.classes) atomicOr(P.status, 2u);
     const bool none = y < 0 || y >= P.classes;
     P.ids_out[row] = none ? 0x7fffffff : (int32_t)y;
-    row_factors(P.s, P.ct, P.lse, row, none, P.inv_tau, P.coef, P.lse2, P.ctmax);
+    const uint32_t c = row_factors(P.s, P.ct, P.lse, row, none, P.inv_tau, P.coef, P.lse2);
+    if (P.ctmax) atomicMax(P.ctmax, c); // the rows' order changes nothing
 }
 
 // A teacher's entries of one row a block: p = softmax(t/τ) over those kept (an id of zero or more, a logit above
 // minus infinity), sum of p·ln p, and the entries by ascending class (each entry counts those before it: top² integer
-// comparisons in shared memory), so that a tile's epilogue finds its own by bisection.
+// comparisons in shared memory), with a table of where each part of the vocabulary begins in them. 23 us for 4096 rows of 64
+// entries beside 740 of the logits, bound by a block's latency (seven barriers).
 struct TeacherParams {
     RowSpace s;
     RowOperand ids, t, ct, lse;
@@ -706,6 +716,7 @@ struct TeacherParams {
     float *out_p, *plogp;
     float *coef, *lse2;
     uint32_t *status, *ctmax;
+    Scales *zero;
 };
 
 template <bool MAX>
@@ -763,12 +774,15 @@ static __global__ void __launch_bounds__(1024) k_head_teacher(const __grid_const
     for (int64_t c = j; c <= P.parts; c += blockDim.x) P.start[row * (P.parts + 1) + c] = (uint16_t)lower_bound(list + P.top, P.top, c * COLS < 0x7fffffff ? (int32_t)(c * COLS) : 0x7fffffff);
     if (j == 0) {
         P.plogp[row] = sum;
-        row_factors(P.s, P.ct, P.lse, row, none, P.inv_tau, P.coef, P.lse2, P.ctmax);
+        const uint32_t c = row_factors(P.s, P.ct, P.lse, row, none, P.inv_tau, P.coef, P.lse2);
+        if (P.ctmax) atomicMax(P.ctmax, c);
+        if (P.zero && row == 0) *P.zero = Scales{0u, 0u, 0u, 0u};
     }
 }
 
 // The greatest finite |element| of a matrix, as f32 bits (non-negative floats order as their bits do, so the blocks'
-// order changes nothing): rows of `cols` elements `col_stride` apart; rows without a target are passed over.
+// order changes nothing): rows of `cols` elements `col_stride` apart; rows without a target are passed over. Bound by
+// memory: 72 us for 329 MB.
 struct MaxParams {
     RowSpace s;
     RowOperand src;
@@ -788,18 +802,26 @@ PSK_DEV uint32_t finite_bits(float x)
 
 constexpr int PIECE = 1024; // columns of a row that a warp takes at a time
 
-struct MaxOfTwo { MaxParams of[2]; };
+struct MaxOfTwo {
+    MaxParams of[2];
+    int32_t operands;  // behind them, of the grid's y: the rows' factors
+    const float *coef;
+    uint32_t *max_ct;
+};
 
 template <bool F32>
 __global__ void __launch_bounds__(256) k_head_max(const __grid_constant__ MaxOfTwo both)
 {
     __shared__ uint32_t red[8];
-    const MaxParams &P = both.of[blockIdx.y];
+    const bool of_ct = blockIdx.y == both.operands;
+    const MaxParams &P = both.of[of_ct ? 0 : blockIdx.y];
     follow();
     const int lane = threadIdx.x & 31;
     const int64_t warps = (int64_t)gridDim.x * 8, pieces = (P.cols + PIECE - 1) / PIECE;
     uint32_t m = 0;
-    for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < P.s.rows * pieces; i += warps) {
+    if (of_ct)
+        for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < P.s.rows; i += (int64_t)gridDim.x * 256) m = max(m, finite_bits(both.coef[i]));
+    else for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < P.s.rows * pieces; i += warps) {
         const int64_t row = i / pieces, c0 = (i - row * pieces) * PIECE, c1 = c0 + PIECE < P.cols ? c0 + PIECE : P.cols;
         if (no_target(P.ids, P.top, row)) continue;
         const int64_t off = row_offset(P.s, P.src.stride, row);
@@ -830,11 +852,13 @@ __global__ void __launch_bounds__(256) k_head_max(const __grid_constant__ MaxOfT
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int w = 1; w < 8; ++w) m = max(m, red[w]);
-        if (m) atomicMax(P.out, m);
+        if (m) atomicMax(of_ct ? both.max_ct : P.out, m);
     }
 }
 
-// The parts' (m, z) of a row put together, and its loss. X neighbouring rows a block, 256 / X threads a row.
+// The parts' (m, z) of a row put together, and its loss. X neighbouring rows a block, 256 / X threads a row: 32 where
+// rows are many (a part's rows lie together: 13 us for 8192 rows of 500 parts, 33 MB), 1 where they are few and the parts
+// of one are what takes time (16 rows: 6 us).
 struct JoinParams {
     RowSpace s;
     int64_t parts;
@@ -1114,7 +1138,8 @@ static __global__ void __launch_bounds__(256, 4) k_head_pack(const __grid_consta
 }
 
 // A gradient from its f32 partial sums into its place: the splits' sums in their order (and, of few rows, those of g's
-// remainder `fold` rows below), times what undoes the scales, rounded once. Four columns a thread.
+// remainder `fold` rows below), times what undoes the scales, rounded once. Four columns a thread; 16 us for three sums of
+// 1524 x 1000, which is latency: their 21 MB are 4 us.
 struct SumParams {
     RowSpace s;
     const float *part;
