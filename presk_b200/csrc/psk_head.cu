@@ -306,7 +306,8 @@ int head_run(HeadContext &x, const psk_launch *l, void *const *table)
         const int64_t kb = (k + BK - 1) / BK, tiles = ((m + BM - 1) / BM) * ((n + BN - 1) / BN);
         // Few tiles, or a last wave of few: cut the summed axis where the estimate says that it pays. A block of the summed axis
         // costs a tile 0.3 us (three products of f32's planes each); partial sums are written and read, and their sum is
-        // a launch.
+        // a launch. dx with the cuts it chooses, and uncut: of f32 2044 x 1024 x 16384 169 + 16 us against 303, of 1524 x 1000 x
+        // 30011 72 + 16 against 175, of 51 x 2048 x 50021 41 + 9 against 281 + 5.
         double best = 0.0;
         int64_t splits = 1;
         for (int64_t want = 1; want <= std::min<int64_t>(std::max<int64_t>(8, x.sms / tiles), kb / 4 + 1); ++want) {
