@@ -284,7 +284,7 @@ int head_run(HeadContext &x, const psk_launch *l, void *const *table)
     // plane of g otherwise, whose product lands in the same sums.
     const bool small = D * V <= 16 << 20, fold = rest && 2 * N <= BM && !small;
     const int g_f16 = f32 || conv || dt == PSK_F16, in_f16 = f32 || dt == PSK_F16;
-    // (row_scaled: a row of dx is as exact as its ct is, whatever the others' are; binary16 operands, whose x is not copied
+    // (row_scaled: rows of other ct keep their digits, see psk_head.cuh; binary16 operands, whose x is not copied
     // into the top of the range, have 2^19 between the rows' ct before it shows beside dx's rounding)
     const bool row_scaled = f32 || conv, g_scaled = vjp && g_f16, any_scale = f32 || g_scaled;
 

@@ -15,9 +15,10 @@
 // Types. bf16 and binary16 operands are multiplied as they are. f32 operands are two binary16 planes, hi + lo, 22 bits
 // of the number, of which three partial products are taken (lo·lo is below 2^-22 of the product): half the tensor
 // work of three bf16 planes and their six products, which this was first (the logits of 2044 x 1024 x 16384: 333 us, 183 with
-// two planes on the same tiles, 156 on pairs). Binary16's range is met by powers of two: w is scaled by its greatest |element|, x by a row's, g by a row's
-// |ct| (binary16 operands: by the greatest), each to the top of the range, 2^14 to 2^15, so that what falls below 2^-24
-// there is 2^-39 of the greatest. For dw, which sums over the rows, x's copy carries what their scales differ by.
+// two planes on the same tiles, 156 on pairs). Binary16's range is met by powers of two: w is scaled by its greatest |element|, x by a row's, g by the greatest
+// |ct|, each to the top of the range, 2^14 to 2^15, so that what falls below 2^-24 there is 2^-39 of the greatest. A row
+// whose ct is 2^-k of the greatest (f32, and bf16 with copies) has g scaled by 2^(k/2) more and its x for dw, which sums
+// over the rows, by as much less: what is lost of either is 2^(k/2 - 39) of it, where one alone would lose 2^(k - 39).
 // g itself is kept in binary16 for f32 and, for many rows, for bf16 operands too, x and w being copied into it (exactly:
 // eight bits into eleven): g in bf16 would cost its 2^-9 an entry, as much again as the result's own rounding.
 #pragma once
@@ -81,14 +82,20 @@ PSK_DEV int scale_of(uint32_t max_bits)
     return k > 60 ? 60 : k; // 1/(g·w) and 1/(g·x) are f32 numbers then
 }
 
-PSK_DEV int scale_of(float coef) { return scale_of(__float_as_uint(coef) & 0x7fffffffu); }
+// A row's, half way (see above). A row with ct = 0 has the common one: its x must not leave the range, 0 times infinity is no 0.
+PSK_DEV int scale_of_row(float coef, uint32_t max_ct)
+{
+    const uint32_t b = __float_as_uint(coef) & 0x7fffffffu;
+    const int e = scale_of(max_ct);
+    return b == 0 ? e : e + ((scale_of(b) - e) >> 1);
+}
 
 enum { UN_NONE = 0, UN_DX = 1, UN_DW = 2 }; // what a product's sums are multiplied by: 1, 1/(g·w), 1/(g·x)
 // (`coef`: of the row, where g's rows have scales of their own)
 PSK_DEV float undo(const Scales *s, int un, const float *coef)
 {
     if (!s || un == UN_NONE) return 1.0f;
-    return pow2(-(coef ? scale_of(*coef) : scale_of(s->max_ct)) - scale_of(un == UN_DX ? s->max_w : s->max_x));
+    return pow2(-(coef ? scale_of_row(*coef, s->max_ct) : scale_of(s->max_ct)) - scale_of(un == UN_DX ? s->max_w : s->max_x));
 }
 
 struct Params {
@@ -485,7 +492,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_head(const __grid_constant__ Job
                 if (MODE == MODE_GRAD) {
                     lse2 = P.lse2[row];
                     coef = P.coef[row];
-                    if (P.scales && P.g_f16) coef = __fmul_rn(coef, pow2(P.row_scaled ? scale_of(coef) : scale_of(P.scales->max_ct)));
+                    if (P.scales && P.g_f16) coef = __fmul_rn(coef, pow2(P.row_scaled ? scale_of_row(coef, P.scales->max_ct) : scale_of(P.scales->max_ct)));
                 }
             }
             float v[COLS];
@@ -1008,7 +1015,7 @@ PSK_DEV void pack_matrix(const PackParams &P)
         const int64_t cs = P.col_stride, off = row_offset(P.s, P.src.stride, row) + c0 * cs;
         uint16_t *dst = P.dst + row * P.ld + c0;
         float f = whole;
-        if (P.coef) f = __fmul_rn(f, pow2(scale_of(*P.max_ct) - scale_of(P.coef[row])));
+        if (P.coef) f = __fmul_rn(f, pow2(scale_of(*P.max_ct) - scale_of_row(P.coef[row], *P.max_ct)));
         if constexpr (TO == PACK_SPLIT) {
             const float *src = (const float *)P.src.p + off;
             if (P.un) {

@@ -111,7 +111,11 @@ def plain(s, lse_in=None):
     # one accumulator throughout: truncation below 2^-23 of a partial sum an instruction of 16
     acc = (max(s["vocab"], 2 * rows) // 16 + 8) * 2.0**-23 + planes
     low = small * (g.abs().sum(1, keepdim=True) * w.abs().amax() if x.numel() else 0.0)  # copies of w and x in binary16
-    low_w = small * (g.abs().sum(0)[:, None] * x.abs().amax() if x.numel() else 0.0)
+    # of x where a row's ct is 2^-k of the greatest: its copy is scaled by 2^(k/2) less (k counts powers of two: at most
+    # one more than the quotient's)
+    less = torch.sqrt(2 * ct.abs().amax() / ct.abs().clamp(min=1e-300)) if x.numel() else ct
+    less = torch.where(ct == 0, 1.0, less)
+    low_w = small * ((g.abs() * (1 + 2 * less)[:, None]).sum(0)[:, None] * x.abs().amax() if x.numel() else 0.0)
     b_dx = eg @ w.abs() + acc * (g.abs() @ w.abs()) + low + dx.abs() * HALF[dt] * 1.01 + LEAST[dt]
     b_dw = eg.t() @ x.abs() + acc * (g.abs().t() @ x.abs()) + low_w + dw.abs() * HALF[dt] * 1.01 + LEAST[dt]
     if not s["vocab_major"]:
