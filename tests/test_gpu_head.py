@@ -374,6 +374,58 @@ def test_gradients_summed_over_a_large_vocabulary(cuda):
     assert abs(float(off[0].mean())) < 5e-5, float(off[0].mean())
 
 
+def normals(rows, cols, scale, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    t = torch.empty(rows, cols, dtype=torch.bfloat16, device="cuda")
+    for lo in range(0, rows, 1 << 16):
+        t[lo:lo + (1 << 16)] = torch.randn(min(1 << 16, rows - lo), cols, generator=g, device="cuda") * scale
+    return t
+
+
+@pytest.mark.parametrize("rows,vocab", [(4, 600_001), (600_001, 200)])
+def test_offsets_beyond_32_bits(cuda, rows, vocab):
+    """x or the head of 2.5e9 elements (4.9 GB, its gradient as much): the last of them against 64 bits."""
+    model = 4096
+    s = dict(outer=(rows,), vocab=vocab, model=model, dtype=abi.BF16, top=0, tau=1.0, vocab_major=True)
+    s["x"], s["w"] = normals(rows, model, 1.0, 1), normals(vocab, model, 2.0 / model**0.5, 2)
+    s["labels"] = vocab - 1 - torch.arange(rows, device="cuda") % min(vocab, 150)
+    s["ct"] = torch.full((rows,), 1.0 / rows, device="cuda")
+    loss, lse = Fenced((rows,), torch.float32), Fenced((rows,), torch.float32)
+    dx, dw = Fenced((rows, model), torch.bfloat16), Fenced((vocab, model), torch.bfloat16)
+    fwd, bwd = hc.launches(s)
+    torch.cuda.synchronize()
+    cuda.run(fwd, [t.data_ptr() for t in hc.given(s) + [lse.t, loss.t]])
+    cuda.run(bwd, [t.data_ptr() for t in hc.given(s) + [s["ct"], lse.t, dw.t, dx.t]])
+    cuda.sync()
+    last = slice(max(0, rows - 100), rows)
+    x, step = s["x"][last].double(), 20_000
+    z = torch.cat([x @ s["w"][lo:lo + step].double().t() for lo in range(0, vocab, step)], 1)
+    want = torch.logsumexp(z, 1)
+    # a logit of 4096 products: accumulators of 512 (32 additions by truncation of sums below 100), eight of them added
+    assert ((lse.check()[last].double() - want).abs() <= 100 * 40 * 2.0**-23).all()
+    assert ((loss.check()[last].double() - (want - z.gather(1, s["labels"][last][:, None])[:, 0])).abs() <= 2 * 100 * 40 * 2.0**-23).all()
+    g = torch.exp(z - want[:, None])
+    g[torch.arange(len(x), device="cuda"), s["labels"][last]] -= 1.0
+    g /= rows
+    want_dx = sum(g[:, lo:lo + step] @ s["w"][lo:lo + step].double() for lo in range(0, vocab, step))
+    off = (dx.check()[last].double() - want_dx).norm() / want_dx.norm()
+    assert float(off) <= 2.0**-8  # the result's half step at most everywhere
+    end = slice(max(0, vocab - 100), vocab)
+    want_dw = torch.zeros(100, model, dtype=torch.float64, device="cuda")
+    for lo in range(0, rows, step):  # every row's part of the last classes
+        xb, y = s["x"][lo:lo + step].double(), s["labels"][lo:lo + step]
+        if rows > 100:
+            zb = xb @ s["w"].double().t()
+            gb = torch.exp(zb - torch.logsumexp(zb, 1, keepdim=True))[:, end]
+        else:
+            gb = torch.exp(z - want[:, None])[:, end]
+        hit = y - end.start
+        gb[torch.arange(len(y), device="cuda")[hit >= 0], hit[hit >= 0]] -= 1.0
+        want_dw += gb.t() @ xb / rows
+    off = (dw.check()[end].double() - want_dw).norm() / want_dw.norm()
+    assert float(off) <= 2.0**-8
+
+
 def test_a_class_the_vocabulary_does_not_have(cuda):
     for top in (0, 4):
         s = hc.make((10,), 100, 32, abi.BF16, device="cuda", top=top, ignored=0.0)
