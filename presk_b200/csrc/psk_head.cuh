@@ -302,7 +302,7 @@ struct Jobs {
 
 // The product of a persistent CTA's tiles, and what MODE makes of it. Bounds: the tensor pipe (2·m·n·k flops) for many
 // rows; for few, the bytes of the second operand. Measured (bf16, a head of 4096 x 32000): 8192 rows, the logits' maxima
-// and sums 1446 us, g 1452, dx 1376, dw 1414, 1.48 to 1.56 PFLOP/s of cuBLAS's 1.65; one after the other in a training
+// and sums 1446 us, g 1452, dx 1376, dw 1414, 1.48 to 1.56 PFLOP/s where a plain library product reaches 1.65; one after the other in a training
 // step, at the power limit's clock, a sixth longer. 16 rows: 46 us for the head's 262 MB, 5.6 TB/s.
 // f32 (2044 x 1024 x 16384, three products): 156, 196, 169, 177 us, 1.05 to 1.3 PFLOP/s: sums that leave the accumulator
 // every six steps, twice the bytes of g, and dx and dw in whole waves of tiles.
