@@ -152,13 +152,13 @@ int launch(HeadContext &x, const Jobs<JOBS> &jobs)
 // A product a·bᵀ: its division into tiles and its tensor maps. `together`: with another in one launch, whose ring the
 // two then share (whole tiles of a).
 template <int MODE>
-int describe(HeadContext &x, Job &j, Params P, const Operand &a, const Operand &b, int f16, bool together, bool *pair)
+int describe(HeadContext &x, Job &j, Params P, const Operand &a, const Operand &b, int f16, bool together, bool *pair, bool pairs = true)
 {
     P.m = a.rows; P.n = b.rows;
     if (MODE != MODE_OUT) P.splits = 1;
     const int64_t tiles = ((P.m + BM - 1) / BM) * ((P.n + BN - 1) / BN);
     // pairs of CTAs where there are rows for two and tiles for everybody (see Cfg)
-    *pair = P.m > BM && tiles * (int64_t)P.splits >= x.sms;
+    *pair = pairs && P.m > BM && tiles * (int64_t)P.splits >= x.sms;
     P.tiles_m = (uint32_t)((P.m + (*pair ? 2 : 1) * BM - 1) / ((*pair ? 2 : 1) * BM)); P.tiles_n = (uint32_t)((P.n + BN - 1) / BN);
     if (tiles > 0x3fffffff / std::max<int64_t>(1, P.splits)) return fail(x, PSK_E7005, "head: more tiles than one launch counts");
     const int a_rows = !*pair && !together && a.k_contiguous ? (int)std::min<int64_t>(BM, up(P.m, 8)) : BM;
@@ -484,6 +484,13 @@ int head_run(HeadContext &x, const psk_launch *l, void *const *table)
             if (small) {
                 r = describe<MODE_OUT>(x, two.of[0], Q, gk, wk, g_f16, true, &pair0);
                 if (r == PSK_OK) r = describe<MODE_OUT>(x, two.of[1], R, da, db, g_f16, true, &pair1);
+                // (both single where one alone would go in pairs and sums are short, for which pairs gain nothing: the two of
+                // 57 x 256 x 32055 in one launch 33 us, in two 19 + 29)
+                if (r == PSK_OK && pair0 != pair1 && Ng <= 512) {
+                    x.flops = flops;
+                    r = describe<MODE_OUT>(x, two.of[0], Q, gk, wk, g_f16, true, &pair0, false);
+                    if (r == PSK_OK) r = describe<MODE_OUT>(x, two.of[1], R, da, db, g_f16, true, &pair1, false);
+                }
                 if (r != PSK_OK) return r;
             }
             if (small && pair0 == pair1) {
